@@ -154,6 +154,13 @@ def lib() -> C.CDLL:
         L.lsam_mlp_block_fwd_proj.argtypes = [vp, vp, i, vp, vp, vp, vp, vp, vp, vp, vp, i, vp, vp, i, i, f, vp]
         L.lsam_mlp_block_fwd.argtypes = [vp, vp, vp, vp, vp, vp, i, i, f, vp]
         L.lsam_mlp_block_fwd_next_norm.argtypes = [vp, vp, vp, vp, vp, vp, vp, i, vp, vp, i, i, f, vp]
+        ll = C.c_longlong
+        sz = C.c_size_t
+        L.lsam_linear_ce_state_bytes.restype = L.lsam_linear_ce_ws_bytes.restype = sz
+        L.lsam_linear_ce_state_bytes.argtypes = [i, i, i]
+        L.lsam_linear_ce_ws_bytes.argtypes = [i, i, i, i, vp, l, f, i]
+        L.lsam_linear_ce_fwd.argtypes = [i, vp, l, vp, l, vp, vp, i, i, i, ll, f, i, vp, vp, vp, sz, vp]
+        L.lsam_linear_ce_bwd.argtypes = [i, vp, l, vp, vp, i, i, i, f, i, vp, vp, l, vp, l, vp, vp, sz, vp]
         L.lsam_prof_arm.argtypes = [i]
         L.lsam_prof_read.argtypes = [i, vp, vp, vp, vp]
         L.lsam_prof_bracket_cost.argtypes = [vp, i, vp]
@@ -202,5 +209,6 @@ EXPORTED = [
     "lsam_window_block_attention_fwd", "lsam_mlp_block_proj_image_bytes", "lsam_mlp_block_proj_pack", "lsam_mlp_block_fwd_proj",
     "lsam_qkv_window4_attention_image_bytes", "lsam_qkv_window4_attention_pack", "lsam_qkv_window4_attention_fwd",
     "lsam_stream_linear_image_bytes", "lsam_stream_linear_pack", "lsam_stream_linear_fwd",
+    "lsam_linear_ce_state_bytes", "lsam_linear_ce_ws_bytes", "lsam_linear_ce_fwd", "lsam_linear_ce_bwd",
     "lsam_outer_reduce_static_max_ws", "lsam_outer_reduce_static_init", "lsam_outer_reduce_static",
 ]

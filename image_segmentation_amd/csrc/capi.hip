@@ -359,4 +359,29 @@ int lsam_outer_reduce_static(int dtype, const void* X, int ldx, const void* Y, i
                                               out, out_cs, out_ks, s));
 }
 
+size_t lsam_linear_ce_state_bytes(int dtype, int M, int D) {
+    if (M < 0 || D <= 0) return 0;
+    return dtype == LSAM_F32 ? ce_state_bytes<float>(M, D) : ce_state_bytes<bf16>(M, D);
+}
+size_t lsam_linear_ce_ws_bytes(int dtype, int M, int D, int V, const void* w, long ldw, float smooth, int grads) {
+    if (M < 0 || D <= 0 || V <= 0) return 0;
+    return dtype == LSAM_F32 ? ce_ws_bytes<float>(M, D, V, w, ldw, smooth, grads) : ce_ws_bytes<bf16>(M, D, V, w, ldw, smooth, grads);
+}
+int lsam_linear_ce_fwd(int dtype, const void* x, long ldx, const void* w, long ldw, const float* bias, const long long* target, int M,
+                       int D, int V, long long ignore, float smooth, int reduction, float* loss, void* state, void* ws, size_t ws_bytes,
+                       lsam_stream_t stream) {
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    DISPATCH(dtype,
+             launch_linear_ce_fwd<float>(x, ldx, w, ldw, bias, target, M, D, V, ignore, smooth, reduction, loss, state, ws, ws_bytes, s),
+             launch_linear_ce_fwd<bf16>(x, ldx, w, ldw, bias, target, M, D, V, ignore, smooth, reduction, loss, state, ws, ws_bytes, s));
+}
+int lsam_linear_ce_bwd(int dtype, const void* w, long ldw, const float* bias, const float* gout, int M, int D, int V, float smooth,
+                       int reduction, const void* state, void* dx, long lddx, void* dw, long lddw, float* db, void* ws, size_t ws_bytes,
+                       lsam_stream_t stream) {
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    DISPATCH(dtype,
+             launch_linear_ce_bwd<float>(w, ldw, bias, gout, M, D, V, smooth, reduction, state, dx, lddx, dw, lddw, db, ws, ws_bytes, s),
+             launch_linear_ce_bwd<bf16>(w, ldw, bias, gout, M, D, V, smooth, reduction, state, dx, lddx, dw, lddw, db, ws, ws_bytes, s));
+}
+
 }  // extern "C"

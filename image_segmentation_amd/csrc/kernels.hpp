@@ -237,4 +237,14 @@ template <typename T>
 int launch_outer_reduce_static(const T* X, int ldx, const T* Y, int ldy, int M, int C, int R, float* out,
                                long out_cs, long out_ks, hipStream_t s);
 
+// softmax cross entropy of x W^T + b without the scores in memory, and its gradient (vocab_ce.hip)
+template <typename T> size_t ce_state_bytes(int M, int D);
+template <typename T> size_t ce_ws_bytes(int M, int D, int V, const void* w, long ldw, float smooth, int grads);
+template <typename T>
+int launch_linear_ce_fwd(const void* x, long ldx, const void* w, long ldw, const float* bias, const long long* target, int M, int D, int V,
+                         long long ignore, float smooth, int reduction, float* loss, void* state, void* ws, size_t ws_bytes, hipStream_t s);
+template <typename T>
+int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float* gout, int M, int D, int V, float smooth, int reduction,
+                         const void* state, void* dx, long lddx, void* dw, long lddw, float* db, void* ws, size_t ws_bytes, hipStream_t s);
+
 }  // namespace lsam

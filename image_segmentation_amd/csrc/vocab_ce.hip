@@ -1,0 +1,804 @@
+// Softmax cross entropy over a large table of classes, with its gradient, without the [rows, classes] scores ever in memory.
+//
+//   z = x W^T + b,  lse_m = log sum_v exp z_mv,  loss_m = (1-e)(lse_m - z_mt) + e (lse_m - mean_v z_mv)
+//   dz_mv = c_m (exp(z_mv - lse_m) - (1-e)[v = t_m] - e/V),  dx = dz W,  dW = dz^T x,  db = sum_m dz
+//
+// Forward: every 256-wide tile of z lives in accumulators only; its epilogue leaves one (max, sum of exponentials) pair a row and
+// tile.  Backward: a piece of the classes at a time, z is formed again, dz of the piece goes to a workspace in the operand type T,
+// and two more products read it.  Rows whose target is ignored are taken out first (order kept): they cost nothing, and what they
+// hold (NaN included) reaches no gradient.
+#include "kernels.hpp"
+
+namespace lsam {
+namespace {
+
+using lds_p = __attribute__((address_space(3))) void*;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int ROW_BAD = -1;   // target outside [0, V): the row's loss and gradient become NaN
+
+// ---------------------------------------------------------------------------------------------------------------------
+// The product: Out[j][i] = sum_k A(i, k) B(j, k), i contiguous in Out.  An operand is stored "KC" ([i][k], k contiguous) or
+// transposed ([k][i]).  Tile IT x JT, k-tiles of 128 bytes, two LDS stages filled by LDS-DMA.
+// ---------------------------------------------------------------------------------------------------------------------
+enum Mode { STATS, DZ, ACC, OUT };
+
+struct CeArgs {
+    const void* A; long lda;   // elements
+    const void* B; long ldb;
+    int I, J, K;               // limits; J (STATS, DZ, ACC) or K (OUT) is further limited by *n
+    const int* n;              // number of rows that count (device)
+    // STATS / DZ
+    const float* bias;         // [I] or null
+    const int* tgt;            // [rows]
+    int i_base;                // class of column 0
+    float smooth_z;            // != 0: the sum of z over the classes is wanted too
+    float* part;               // STATS: planes [tiles_i][rows_cap] of (base, sum of exponentials, sum of z)
+    float* zt;                 // STATS: z of the target
+    const float* base2;        // DZ: the row's base, and its coefficient c and c / (sum of exponentials)
+    const float* coef;
+    const float* coef_s;
+    float sm, keep;            // DZ: e / V, 1 - e
+    float* dbp;                // DZ: [tiles_j][I_cap] partial column sums or null
+    long dbp_ld;
+    int rows_cap;
+    // outputs
+    void* out; long ldo;       // DZ: T; ACC: fp32; OUT: T, or fp32 partials when splits > 1
+    long split_stride;         // elements between the splits' outputs
+    int splits, accumulate;
+    int cols, vec;             // OUT: columns to write; whether 4 at a time may be stored at once
+};
+
+template <typename T> struct Ce;
+template <> struct Ce<bf16> {
+    static __device__ __forceinline__ void mma(const uint4& a, const uint4& b, f32x4& c) {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Ce<float> {
+    static __device__ __forceinline__ void mma(const uint4& a, const uint4& b, f32x4& c) {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
+    }
+};
+
+// One operand's tile in LDS.  KC: R rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7).  Transposed: 128 / sizeof(T) rows of
+// R * sizeof(T) bytes; bf16 is read with the transposing LDS load (16 lanes take 4 k-rows x 16 columns), whose 8 rows of a half
+// wave must fall on different banks: 32-byte column pairs p of row k at p ^ h(k); fp32 is read one dword a lane, 64-byte column
+// groups at group ^ ((k >> 2) & 3).
+template <typename T, bool KC, int R, int NW> struct Tile {
+    static constexpr int ES = sizeof(T), EPC = 16 / ES, KE = 128 / ES, RB = R * ES;
+    static constexpr int NI = R * 128 / 1024 / NW;   // DMA instructions a wave and stage
+    static_assert(R * 128 % (1024 * NW) == 0, "whole DMA instructions");
+    unsigned vo[NI];   // byte offsets of this lane's chunks in the k-tile's slab; 0xFFFFFFFF reads zeros
+    short ke[NI];      // first k of the chunk
+    __device__ __forceinline__ void init(int wave, int lane, long ld, int r0, int lim) {
+#pragma unroll
+        for (int q = 0; q < NI; ++q) {
+            const int b = (wave + NW * q) * 1024 + lane * 16;
+            if constexpr (KC) {
+                const int row = b >> 7, c = ((b >> 4) & 7) ^ (row & 7);
+                vo[q] = r0 + row < lim ? (unsigned)((long)row * ld * ES + c * 16) : 0xFFFFFFFFu;
+                ke[q] = (short)(c * EPC);
+            } else {
+                const int k = b / RB, pos = (b % RB) >> 4;
+                const int c = ES == 2 ? pos ^ (2 * ((k & 3) | (((k >> 3) & 1) << 2))) : pos ^ (4 * ((k >> 2) & 3));
+                vo[q] = r0 + c * EPC < lim ? (unsigned)((long)k * ld * ES + c * 16) : 0xFFFFFFFFu;
+                ke[q] = (short)k;
+            }
+        }
+    }
+    // k-tile slab: KC advances 128 bytes along the rows, transposed KE rows
+    static __device__ __forceinline__ const char* slab(const void* base, long ld, int r0, long k0) {
+        const char* p = static_cast<const char*>(base);
+        return KC ? p + ((long)r0 * ld + k0) * ES : p + (k0 * ld + r0) * ES;
+    }
+    __device__ __forceinline__ void issue(const char* slab_p, char* dst, int wave, int left) const {
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(slab_p), 0, 0x7FFFFFFF, 0x00020000);
+        if (left >= KE) {
+#pragma unroll
+            for (int q = 0; q < NI; ++q)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_p)(dst + (wave + NW * q) * 1024), 16, vo[q], 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int q = 0; q < NI; ++q)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_p)(dst + (wave + NW * q) * 1024), 16,
+                                                         ke[q] < left ? vo[q] : 0xFFFFFFFFu, 0, 0, 0);
+        }
+    }
+    // fragments of NT 16-wide tiles starting at tile t0, k-step ks (0, 1)
+    template <int NT> static __device__ __forceinline__ void read(const char* s, int t0, int ks, int g, int lr, uint4 (&f)[NT]) {
+        if constexpr (KC) {
+            const char* p = s + (t0 * 16 + lr) * 128 + (((ks * 4 + g) ^ (lr & 7)) << 4);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) f[t] = *reinterpret_cast<const uint4*>(p + t * 2048);
+        } else if constexpr (ES == 2) {
+            using s4 = __attribute__((ext_vector_type(4))) short;
+            using s4p = __attribute__((address_space(3))) s4*;
+            const int h = (lr >> 2) | ((g & 1) << 2);
+            const char* p = s + (ks * 32 + 8 * g + (lr >> 2)) * RB + (lr & 3) * 8;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const char* a = p + (((t0 + t) ^ h) << 5);
+                const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)a), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)(a + 4 * RB));
+                const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, hi);
+                f[t] = make_uint4(x.x, x.y, y.x, y.y);
+            }
+        } else {
+            const char* p = s + (ks * 16 + 4 * g) * RB + lr * 4;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const char* a = p + (((t0 + t) ^ g) << 6);
+                f[t] = make_uint4(*reinterpret_cast<const unsigned*>(a), *reinterpret_cast<const unsigned*>(a + RB),
+                                  *reinterpret_cast<const unsigned*>(a + 2 * RB), *reinterpret_cast<const unsigned*>(a + 3 * RB));
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ float row16_sum(float x) {   // over the 16 lanes that share lane >> 4
+    x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x128, 0xf, 0xf, false));
+    x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x124, 0xf, 0xf, false));
+    x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x122, 0xf, 0xf, false));
+    x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x121, 0xf, 0xf, false));
+    return x;
+}
+
+template <typename T, bool AKC, bool BKC, int MODE, int WI, int WJ, int TI, int TJ, int OCC>
+__global__ __launch_bounds__(64 * WI * WJ, OCC) void ce_gemm_kernel(const CeArgs p) {
+#if defined(__HIP_DEVICE_COMPILE__)   // the host pass needs the launch stub only, and cannot form the LDS builtins
+    constexpr int NW = WI * WJ, IT = WI * TI * 16, JT = WJ * TJ * 16;
+    constexpr int KE = 128 / (int)sizeof(T);
+    using TA = Tile<T, AKC, IT, NW>;
+    using TB = Tile<T, BKC, JT, NW>;
+    __shared__ __attribute__((aligned(1024))) char st0[(IT + JT) * 128];
+    __shared__ __attribute__((aligned(1024))) char st1[(IT + JT) * 128];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wi = wave % WI, wj = wave / WI, g = lane >> 4, lr = lane & 15;
+    const int n = *p.n;
+    const int J = MODE == OUT ? p.J : min(p.J, n), K = MODE == OUT ? min(p.K, n) : p.K;
+
+    // tile order: runs of 8 j-tiles against one i-tile, so the workgroups that an XCD holds at a time share operands in its L2
+    const int tiles_i = (p.I + IT - 1) / IT, tiles_j = (p.J + JT - 1) / JT;
+    int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int split = id / (tiles_i * tiles_j);
+    id -= split * tiles_i * tiles_j;
+    const int per = 8 * tiles_i, grp = id / per, in = id - grp * per, gj = min(8, tiles_j - grp * 8);
+    const int jt = grp * 8 + in % gj, it = in / gj;
+    const int i0 = it * IT, j0 = jt * JT;
+    if (j0 >= J) return;
+
+    const int kt_all = (K + KE - 1) / KE;
+    const int per_split = (kt_all + p.splits - 1) / p.splits;
+    const int kt0 = min(split * per_split, kt_all), kt1 = min(kt0 + per_split, kt_all);
+
+    f32x4 acc[TI][TJ];
+#pragma unroll
+    for (int a = 0; a < TI; ++a)
+#pragma unroll
+        for (int b = 0; b < TJ; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    if (kt0 < kt1) {
+        TA ta;
+        TB tb;
+        ta.init(wave, lane, p.lda, i0, p.I);
+        tb.init(wave, lane, p.ldb, j0, J);
+        auto issue = [&](int kt, char* s) {
+            const int left = K - kt * KE;
+            ta.issue(TA::slab(p.A, p.lda, i0, (long)kt * KE), s, wave, left);
+            tb.issue(TB::slab(p.B, p.ldb, j0, (long)kt * KE), s + IT * 128, wave, left);
+        };
+        auto mma = [&](const uint4 (&a)[TI], const uint4 (&b)[TJ]) {
+#pragma unroll
+            for (int x = 0; x < TI; ++x)
+#pragma unroll
+                for (int y = 0; y < TJ; ++y) Ce<T>::mma(a[x], b[y], acc[x][y]);
+        };
+        uint4 a0[TI], b0[TJ], a1[TI], b1[TJ];
+        auto read = [&](const char* s, int ks, uint4 (&a)[TI], uint4 (&b)[TJ]) {
+            TA::template read<TI>(s, wi * TI, ks, g, lr, a);
+            TB::template read<TJ>(s + IT * 128, wj * TJ, ks, g, lr, b);
+        };
+        // k-tile q:  read ks1(q) | MFMA ks0(q) | own DMA(q+1) landed, own reads of q done, barrier | read ks0(q+1), issue DMA(q+2) | MFMA ks1(q)
+        auto step = [&](int kt, char* cur, char* nxt) {
+            read(cur, 1, a1, b1);
+            mma(a0, b0);
+            if (kt + 1 < kt1) {
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                read(nxt, 0, a0, b0);
+                if (kt + 2 < kt1) issue(kt + 2, cur);
+            }
+            mma(a1, b1);
+        };
+        issue(kt0, st0);
+        if (kt0 + 1 < kt1) issue(kt0 + 1, st1);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        read(st0, 0, a0, b0);
+        for (int kt = kt0; kt < kt1; kt += 2) {
+            step(kt, st0, st1);
+            if (kt + 1 < kt1) step(kt + 1, st1, st0);
+        }
+    }
+
+    // ---- epilogues: lane (g, lr), tile (x, y), register r holds Out[j = j0 + (wj TJ + y) 16 + lr][i = i0 + (wi TI + x) 16 + 4 g + r]
+    const int ib = i0 + wi * TI * 16 + 4 * g, jb = j0 + wj * TJ * 16 + lr;
+    if constexpr (MODE == STATS || MODE == DZ) {
+        __shared__ float red[(MODE == STATS ? WI * 3 * JT : WJ * IT)];
+#pragma unroll
+        for (int x = 0; x < TI; ++x) {
+            const int i = ib + 16 * x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float b = p.bias && i + r < p.I ? p.bias[i + r] : 0.f;
+                // a class masked with the type's lowest value: a base of its size would not be a whole number's step away from its
+                // scores; -inf and NaN stay what they are
+                if (fabsf(b) > 1e9f && fabsf(b) != INFINITY) b = copysignf(1e9f, b);
+#pragma unroll
+                for (int y = 0; y < TJ; ++y) acc[x][y][r] = i + r < p.I ? acc[x][y][r] + b : -INFINITY;
+            }
+        }
+        if constexpr (MODE == STATS) {
+#pragma unroll
+            for (int y = 0; y < TJ; ++y) {
+                const int m = jb + 16 * y;
+                const int t = m < J ? p.tgt[m] - p.i_base : ROW_BAD;
+                float mx = -INFINITY, zs = 0.f;
+#pragma unroll
+                for (int x = 0; x < TI; ++x)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float z = acc[x][y][r];
+                        mx = fmaxf(mx, z);
+                        if (ib + 16 * x + r == t) p.zt[m] = z;
+                    }
+                if (p.smooth_z != 0.f) {
+#pragma unroll
+                    for (int x = 0; x < TI; ++x)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) zs += ib + 16 * x + r < p.I ? acc[x][y][r] : 0.f;
+                    zs = group4_sum(zs);
+                }
+                // exponentials are taken as 2^(z log2e - base) with a whole-number base: one fused multiply-add an element, and bases
+                // of different tiles differ by exact powers of two.  (Scores beyond 1e9 would need z - max in a step of its own.)
+                mx = group4_max(mx);
+                const float base = __builtin_ceilf(mx * LOG2E);
+                const float sub = base == -INFINITY ? 0.f : base;   // every class of the tile at -inf: its exponentials are 0
+                float s = 0.f;
+#pragma unroll
+                for (int x = 0; x < TI; ++x)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[x][y][r], LOG2E, -sub));
+                s = group4_sum(s);
+                if (g == 0) {
+                    const int c = (wj * TJ + y) * 16 + lr;
+                    red[(wi * 3 + 0) * JT + c] = base;
+                    red[(wi * 3 + 1) * JT + c] = s;
+                    red[(wi * 3 + 2) * JT + c] = zs;
+                }
+            }
+            __syncthreads();
+            for (int c = tid; c < JT; c += 64 * NW) {
+                if (j0 + c >= J) continue;
+                float mx = red[c], s = 0.f, zs = 0.f;
+#pragma unroll
+                for (int w = 1; w < WI; ++w) mx = fmaxf(mx, red[w * 3 * JT + c]);
+#pragma unroll
+                for (int w = 0; w < WI; ++w) {
+                    const float mw = red[w * 3 * JT + c];
+                    s += red[(w * 3 + 1) * JT + c] * (mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mw - mx));
+                    zs += red[(w * 3 + 2) * JT + c];
+                }
+                const size_t o = (size_t)it * p.rows_cap + j0 + c, plane = (size_t)tiles_i * p.rows_cap;
+                p.part[o] = mx;
+                p.part[plane + o] = s;
+                if (p.smooth_z != 0.f) p.part[2 * plane + o] = zs;
+            }
+        } else {
+            T* out = static_cast<T*>(p.out);
+#pragma unroll
+            for (int y = 0; y < TJ; ++y) {
+                const int m = jb + 16 * y;
+                const bool ok = m < J;
+                const float base = ok ? p.base2[m] : 0.f, c = ok ? p.coef[m] : 0.f, cs = ok ? p.coef_s[m] : 0.f;
+                const float low = -c * p.sm, hit = c * p.keep;
+                const int t = ok ? p.tgt[m] - p.i_base : ROW_BAD;
+                T* rowp = out + (size_t)(ok ? m : 0) * p.ldo + i0 + wi * TI * 16;
+#pragma unroll
+                for (int x = 0; x < TI; ++x)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int i = ib + 16 * x + r;
+                        float q = fmaf(__builtin_amdgcn_exp2f(fmaf(acc[x][y][r], LOG2E, -base)), cs, low);
+                        if (i == t) q -= hit;
+                        acc[x][y][r] = ok && i < p.I ? q : 0.f;
+                    }
+                if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                    for (int x = 0; x < TI; x += 2) store_bf16_tile_pair(rowp + 16 * x, g, acc[x][y], acc[x + 1][y], ok);
+                } else {
+                    if (ok) {
+#pragma unroll
+                        for (int x = 0; x < TI; ++x) store4(rowp + 16 * x + 4 * g, acc[x][y]);
+                    }
+                }
+            }
+            if (p.dbp) {
+#pragma unroll
+                for (int x = 0; x < TI; ++x)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float s = 0.f;
+#pragma unroll
+                        for (int y = 0; y < TJ; ++y) s += acc[x][y][r];
+                        s = row16_sum(s);
+                        if (lr == 0) red[wj * IT + (wi * TI + x) * 16 + 4 * g + r] = s;
+                    }
+                __syncthreads();
+                for (int c = tid; c < IT; c += 64 * NW) {
+                    float s = 0.f;
+#pragma unroll
+                    for (int w = 0; w < WJ; ++w) s += red[w * IT + c];
+                    if (i0 + c < p.I) p.dbp[(size_t)jt * p.dbp_ld + i0 + c] = s;
+                }
+            }
+        }
+    } else {
+        const bool f32out = MODE == ACC || p.splits > 1;
+#pragma unroll
+        for (int y = 0; y < TJ; ++y) {
+            const int j = jb + 16 * y;
+            if (j >= J) continue;
+#pragma unroll
+            for (int x = 0; x < TI; ++x) {
+                const int i = ib + 16 * x;
+                if (i >= (f32out ? p.I : p.cols)) continue;
+                if (f32out) {   // workspace: I padded to whole chunks, rows 16-byte aligned
+                    float* o = static_cast<float*>(p.out) + split * p.split_stride + (size_t)j * p.ldo + i;
+                    f32x4 v = acc[x][y];
+                    if (MODE == ACC && p.accumulate) v += load4(o);
+                    store4(o, v);
+                } else {
+                    T* o = static_cast<T*>(p.out) + (size_t)j * p.ldo + i;
+                    if (p.vec) store4(o, acc[x][y]);
+                    else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (i + r < p.cols) o[r] = from_f<T>(acc[x][y][r]);
+                    }
+                }
+            }
+        }
+    }
+#endif
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Row selection: the rows whose target is not ignored, in order.  One workgroup; 8 rows a thread and step.
+// ---------------------------------------------------------------------------------------------------------------------
+struct CeState {   // what the forward leaves for the backward
+    int* n;        // rows that count
+    int* idx;      // [M] compact row -> row
+    int* pos;      // [M] row -> compact row, -1 where ignored
+    int* tgt;      // [M] compact; ROW_BAD outside [0, V)
+    float* base2;  // [M] compact: lse = (base2 + log2(sum)) / log2(e)
+    float* sum;
+    char* xc;      // T [M][Dp] compact rows, columns padded with zeros
+};
+
+__global__ __launch_bounds__(1024) void ce_rows_kernel(const long long* __restrict__ target, int M, int V, long long ignore, CeState st,
+                                                       float* __restrict__ loss_none) {
+    __shared__ int wsum[16], total;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int base = 0;
+    for (int m0 = 0; m0 < M; m0 += 8192) {
+        const int b = m0 + tid * 8;
+        long long t[8];
+        int cnt = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            t[j] = b + j < M ? target[b + j] : ignore;
+            cnt += b + j < M && t[j] != ignore;
+        }
+        int inc = cnt;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 63) wsum[wave] = inc;
+        __syncthreads();
+        int before = 0;
+        for (int w = 0; w < 16; ++w) before += w < wave ? wsum[w] : 0;
+        int r = base + before + inc - cnt;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (b + j >= M) break;
+            if (t[j] != ignore) {
+                st.idx[r] = b + j;
+                st.tgt[r] = t[j] >= 0 && t[j] < V ? (int)t[j] : ROW_BAD;
+                st.pos[b + j] = r++;
+            } else {
+                st.pos[b + j] = -1;
+                if (loss_none) loss_none[b + j] = 0.f;
+            }
+        }
+        if (tid == 1023) total = before + inc;
+        __syncthreads();
+        base += total;
+    }
+    if (tid == 0) *st.n = base;
+}
+
+// rows of `src` (through idx, or all of them) to [rows][Dp], columns D.. filled with zeros
+template <typename T>
+__global__ __launch_bounds__(256) void ce_gather_kernel(const T* __restrict__ src, long ld, const int* __restrict__ idx, const int* __restrict__ n,
+                                                        int rows, int D, int Dp, int vec, T* __restrict__ dst) {
+    constexpr int EPC = 16 / (int)sizeof(T);
+    const int cpr = Dp / EPC, lim = n ? min(rows, *n) : rows;
+    const long total = (long)lim * cpr;
+    for (long id = (long)blockIdx.x * 256 + threadIdx.x; id < total; id += (long)gridDim.x * 256) {
+        const int r = (int)(id / cpr), c = (int)(id - (long)r * cpr) * EPC;
+        const T* s = src + (idx ? idx[r] : r) * ld + c;
+        uint4 v;
+        if (vec) v = *reinterpret_cast<const uint4*>(s);
+        else {
+            T e[EPC];
+#pragma unroll
+            for (int j = 0; j < EPC; ++j) e[j] = c + j < D ? s[j] : from_f<T>(0.f);
+            __builtin_memcpy(&v, e, 16);
+        }
+        *reinterpret_cast<uint4*>(dst + (size_t)r * Dp + c) = v;
+    }
+}
+
+// 16 rows a workgroup, 64 threads a row: joins the tiles' (base, sum) pairs; the loss of the row.  With one workgroup the sum over
+// the rows too.  base + log2(sum) and the target's score are subtracted in 64 bits: a learned row's loss is their small difference.
+__global__ __launch_bounds__(1024) void ce_loss_kernel(const float* __restrict__ part, const float* __restrict__ zt, int tiles, int cap, int V,
+                                                       float smooth, CeState st, float* __restrict__ row_loss, float* __restrict__ loss,
+                                                       int reduction) {
+    __shared__ float sb[64][17], ss[64][17], sz[64][17];
+    __shared__ double sl[16];
+    const int tid = threadIdx.x, c = tid & 15, sl_ = tid >> 4, n = *st.n;
+    const int r = blockIdx.x * 16 + c;
+    const size_t plane = (size_t)tiles * cap;
+    float b = -INFINITY, s = 0.f, z = 0.f;
+    if (r < n) {
+        for (int t = sl_; t < tiles; t += 64) {
+            const size_t o = (size_t)t * cap + r;
+            const float bt = part[o], v = part[plane + o];
+            const float nb = fmaxf(b, bt);
+            s = (b == -INFINITY ? s : s * exp2f(b - nb)) + (bt == -INFINITY ? v : v * exp2f(bt - nb));
+            b = nb;
+            if (smooth != 0.f) z += part[2 * plane + o];
+        }
+    }
+    sb[sl_][c] = b; ss[sl_][c] = s; sz[sl_][c] = z;
+    __syncthreads();
+    if (tid < 16) {
+        double out = 0.;
+        if (r < n) {
+            float B = -INFINITY, S = 0.f, Z = 0.f;
+            for (int k = 0; k < 64; ++k) B = fmaxf(B, sb[k][c]);
+            for (int k = 0; k < 64; ++k) {
+                S += ss[k][c] * (sb[k][c] == -INFINITY ? 1.f : exp2f(sb[k][c] - B));
+                Z += sz[k][c];
+            }
+            st.base2[r] = B;
+            st.sum[r] = S;
+            const double L = (double)LOG2E, l2 = (double)B + log2((double)S);
+            if (st.tgt[r] == ROW_BAD) out = (double)NAN;
+            else out = (l2 - L * (double)zt[r]) / L * (1. - (double)smooth) + (smooth != 0.f ? (double)smooth * (l2 / L - (double)Z / V) : 0.);
+            if (reduction == LSAM_REDUCE_NONE) loss[st.idx[r]] = (float)out;
+            else row_loss[r] = (float)out;
+        }
+        sl[c] = out;
+    }
+    if (gridDim.x == 1 && reduction != LSAM_REDUCE_NONE) {
+        __syncthreads();
+        if (tid == 0) {
+            double a = 0.;
+            for (int k = 0; k < 16; ++k) a += sl[k];
+            loss[0] = (float)(reduction == LSAM_REDUCE_MEAN ? a / (double)n : a);
+        }
+    }
+}
+
+__global__ __launch_bounds__(1024) void ce_sum_kernel(const float* __restrict__ row_loss, const int* __restrict__ np, float* __restrict__ loss,
+                                                      int reduction) {
+    __shared__ double part[1024];
+    const int n = *np;
+    double a = 0.;
+    for (int r = threadIdx.x; r < n; r += 1024) a += (double)row_loss[r];
+    part[threadIdx.x] = a;
+    __syncthreads();
+    for (int o = 512; o; o >>= 1) {
+        if ((int)threadIdx.x < o) part[threadIdx.x] += part[threadIdx.x + o];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) loss[0] = (float)(reduction == LSAM_REDUCE_MEAN ? part[0] / (double)n : part[0]);
+}
+
+__global__ __launch_bounds__(256) void ce_coef_kernel(const float* __restrict__ gout, int reduction, CeState st, float* __restrict__ coef,
+                                                      float* __restrict__ coef_s) {
+    const int r = blockIdx.x * 256 + threadIdx.x, n = *st.n;
+    if (r >= n) return;
+    float c = reduction == LSAM_REDUCE_NONE ? gout[st.idx[r]] : gout[0];
+    if (reduction == LSAM_REDUCE_MEAN) c = c / (float)n;
+    if (st.tgt[r] == ROW_BAD) c = NAN;
+    coef[r] = c;
+    coef_s[r] = c / st.sum[r];
+}
+
+// dx[m] = sum of the splits' rows, or zeros where the row was ignored
+template <typename T>
+__global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ acc, long stride, int splits, const int* __restrict__ pos, int M, int D,
+                                                    int Dp, int vec, T* __restrict__ dx, long lddx) {
+    const int cpr = Dp / 4;
+    for (long id = (long)blockIdx.x * 256 + threadIdx.x; id < (long)M * cpr; id += (long)gridDim.x * 256) {
+        const int m = (int)(id / cpr), c = (int)(id - (long)m * cpr) * 4, r = pos ? pos[m] : m;
+        if (c >= D) continue;
+        f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (r >= 0)
+            for (int s = 0; s < splits; ++s) v += load4(acc + s * stride + (size_t)r * Dp + c);
+        T* o = dx + (size_t)m * lddx + c;
+        if (vec) store4(o, v);
+        else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c + j < D) o[j] = from_f<T>(v[j]);
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void ce_db_kernel(const float* __restrict__ dbp, long ld, const int* __restrict__ np, int rows_tile, int V,
+                                                    float* __restrict__ db) {
+    const int v = blockIdx.x * 256 + threadIdx.x, tiles = (*np + rows_tile - 1) / rows_tile;
+    if (v >= V) return;
+    float s = 0.f;
+    for (int t = 0; t < tiles; ++t) s += dbp[(size_t)t * ld + v];
+    db[v] = s;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr size_t DZ_CAP = (size_t)256 << 20;   // a piece's dz is kept within the last-level cache (256 MB)
+constexpr int CU = 256;
+
+struct Carve {
+    char* p;
+    size_t used = 0;
+    template <typename U> U* take(size_t n) {
+        U* r = reinterpret_cast<U*>(p + used);
+        used += align_up(n * sizeof(U), 256);
+        return p ? r : nullptr;
+    }
+};
+
+template <typename T> struct CePlan {
+    static constexpr int EPC = 16 / (int)sizeof(T), TILE = 256;
+    int M, D, V, Dp, tiles_v, tiles_m, tiles_d;
+    bool pack_w;
+    int piece, pieces, s_dx, s_dw;
+    CePlan(int M_, int D_, int V_, bool pack) : M(M_), D(D_), V(V_), pack_w(pack) {
+        Dp = (D + EPC - 1) / EPC * EPC;
+        tiles_v = cdiv(V, TILE);
+        tiles_m = M > 0 ? cdiv(M, TILE) : 1;
+        tiles_d = cdiv(Dp, TILE);
+        const size_t col = (size_t)M * sizeof(T) * TILE;
+        size_t pt = DZ_CAP / (col ? col : 1);
+        if (pt < 1) pt = 1;
+        if (pt > (size_t)tiles_v) pt = tiles_v;
+        pieces = cdiv(tiles_v, (int)pt);
+        piece = cdiv(tiles_v, pieces) * TILE;
+        pieces = cdiv(V, piece);
+        const int kt = 128 / (int)sizeof(T);
+        auto splits = [&](int tiles, int ksteps) {
+            int s = tiles >= CU ? 1 : CU / tiles;
+            const int most = ksteps / 4 > 0 ? ksteps / 4 : 1;   // at least four k-tiles a split
+            return s < most ? (s > 0 ? s : 1) : most;
+        };
+        s_dx = splits(tiles_m * tiles_d, cdiv(piece, kt));
+        s_dw = splits(piece / TILE * tiles_d, cdiv(M, kt));
+    }
+    size_t state(char* base, CeState* st) const {
+        Carve c{base};
+        CeState s;
+        s.n = c.take<int>(1);
+        s.idx = c.take<int>(M);
+        s.pos = c.take<int>(M);
+        s.tgt = c.take<int>(M);
+        s.base2 = c.take<float>(M);
+        s.sum = c.take<float>(M);
+        s.xc = c.take<char>((size_t)M * Dp * sizeof(T));
+        if (st) *st = s;
+        return c.used;
+    }
+    struct Fwd { char* wp; float *part, *zt, *row_loss; };
+    size_t fwd(char* base, Fwd* f, bool smooth) const {
+        Carve c{base};
+        Fwd w;
+        w.wp = c.take<char>(pack_w ? (size_t)V * Dp * sizeof(T) : 0);
+        w.part = c.take<float>((size_t)tiles_v * M * (smooth ? 3 : 2));
+        w.zt = c.take<float>(M);
+        w.row_loss = c.take<float>(M);
+        if (f) *f = w;
+        return c.used;
+    }
+    struct Bwd { char *wp, *dz; float *coef, *coef_s, *dx, *dw, *dbp; };
+    size_t bwd(char* base, Bwd* f, bool want_dx, bool want_dw, bool want_db) const {
+        Carve c{base};
+        Bwd w;
+        w.wp = c.take<char>(pack_w ? (size_t)V * Dp * sizeof(T) : 0);
+        w.dz = c.take<char>((size_t)M * piece * sizeof(T));
+        w.coef = c.take<float>(M);
+        w.coef_s = c.take<float>(M);
+        w.dx = c.take<float>(want_dx ? (size_t)s_dx * M * Dp : 0);
+        w.dw = c.take<float>(want_dw && s_dw > 1 ? (size_t)s_dw * piece * Dp : 0);
+        w.dbp = c.take<float>(want_db ? (size_t)tiles_m * V : 0);
+        if (f) *f = w;
+        return c.used;
+    }
+};
+
+template <typename T, bool AKC, bool BKC, int MODE, int WI, int WJ, int TI, int TJ, int OCC> int ce_gemm(const CeArgs& a, hipStream_t s) {
+    constexpr int IT = WI * TI * 16, JT = WJ * TJ * 16;
+    const int tiles = cdiv(a.I, IT) * cdiv(a.J, JT) * a.splits;
+    ce_gemm_kernel<T, AKC, BKC, MODE, WI, WJ, TI, TJ, OCC><<<tiles, 64 * WI * WJ, 0, s>>>(a);
+    LSAM_LAUNCH_CHECK();
+    return LSAM_OK;
+}
+
+template <typename T> bool rows_direct(const void* p, long ld, int D) {   // rows that 16-byte chunks can be fetched from in place
+    constexpr int EPC = 16 / (int)sizeof(T);
+    return D % EPC == 0 && ld % EPC == 0 && aligned16(p) && ld < (1l << 20);
+}
+
+template <typename T> int gather(const void* src, long ld, const int* idx, const int* n, int rows, int D, int Dp, void* dst, hipStream_t s) {
+    const long chunks = (long)rows * (Dp / (16 / (int)sizeof(T)));
+    const long blocks = (chunks + 255) / 256;
+    ce_gather_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(static_cast<const T*>(src), ld, idx, n, rows, D, Dp,
+                                                                             rows_direct<T>(src, ld, D), static_cast<T*>(dst));
+    LSAM_LAUNCH_CHECK();
+    return LSAM_OK;
+}
+}  // namespace
+
+int ce_check(int M, int D, int V, int reduction, float smooth) {
+    LSAM_REQUIRE(M >= 0 && D > 0 && V > 0, LSAM_ERR_BAD_ARG, "linear_ce: %d rows, %d columns, %d classes", M, D, V);
+    LSAM_REQUIRE(M <= (1 << 28) && V <= (1 << 28) && D <= (1 << 18), LSAM_ERR_UNSUPPORTED, "linear_ce: %d rows, %d columns, %d classes", M, D, V);
+    LSAM_REQUIRE(((long)M / 256 + 1) * ((long)V / 256 + 1) < (1l << 30), LSAM_ERR_UNSUPPORTED, "linear_ce: %d rows x %d classes", M, V);
+    LSAM_REQUIRE(reduction >= 0 && reduction <= 2, LSAM_ERR_BAD_ARG, "linear_ce: reduction %d", reduction);
+    LSAM_REQUIRE(smooth >= 0.f && smooth <= 1.f, LSAM_ERR_BAD_ARG, "linear_ce: label smoothing %g outside [0, 1]", (double)smooth);
+    return LSAM_OK;
+}
+
+template <typename T> size_t ce_state_bytes(int M, int D) { return CePlan<T>(M, D, 1, false).state(nullptr, nullptr); }
+template <typename T> size_t ce_ws_bytes(int M, int D, int V, const void* w, long ldw, float smooth, int grads) {
+    const CePlan<T> pl(M, D, V, !rows_direct<T>(w, ldw, D));
+    const size_t n = grads ? pl.bwd(nullptr, nullptr, grads & 1, grads & 2, grads & 4) : pl.fwd(nullptr, nullptr, smooth != 0.f);
+    return n ? n : 256;   // without rows nothing is kept there, but the pointer is wanted
+}
+
+template <typename T>
+int launch_linear_ce_fwd(const void* x, long ldx, const void* w, long ldw, const float* bias, const long long* target, int M, int D, int V,
+                         long long ignore, float smooth, int reduction, float* loss, void* state, void* ws, size_t ws_bytes, hipStream_t s) {
+    LSAM_TRY(ce_check(M, D, V, reduction, smooth));
+    const CePlan<T> pl(M, D, V, !rows_direct<T>(w, ldw, D));
+    LSAM_REQUIRE((M == 0 || (x && target)) && w && state && ws && (loss || (M == 0 && reduction == LSAM_REDUCE_NONE)), LSAM_ERR_BAD_ARG,
+                 "linear_ce: null operand");
+    LSAM_REQUIRE(ldx >= D && ldw >= D && aligned16(state) && aligned16(ws), LSAM_ERR_BAD_ARG,
+                 "linear_ce: row strides %ld, %ld below %d columns, or a workspace off its 16-byte alignment", ldx, ldw, D);
+    CeState st;
+    typename CePlan<T>::Fwd f;
+    pl.state(static_cast<char*>(state), &st);
+    LSAM_REQUIRE(pl.fwd(static_cast<char*>(ws), &f, smooth != 0.f) <= ws_bytes, LSAM_ERR_WORKSPACE, "linear_ce: workspace too small");
+    ce_rows_kernel<<<1, 1024, 0, s>>>(target, M, V, ignore, st, reduction == LSAM_REDUCE_NONE ? loss : nullptr);
+    LSAM_LAUNCH_CHECK();
+    if (M > 0) {
+        LSAM_TRY(gather<T>(x, ldx, st.idx, st.n, M, D, pl.Dp, st.xc, s));
+        if (pl.pack_w) LSAM_TRY(gather<T>(w, ldw, nullptr, nullptr, V, D, pl.Dp, f.wp, s));
+        CeArgs a{};
+        a.A = pl.pack_w ? f.wp : w; a.lda = pl.pack_w ? pl.Dp : ldw;
+        a.B = st.xc; a.ldb = pl.Dp;
+        a.I = V; a.J = M; a.K = pl.Dp; a.n = st.n;
+        a.bias = bias; a.tgt = st.tgt; a.smooth_z = smooth; a.part = f.part; a.zt = f.zt; a.rows_cap = M; a.splits = 1;
+        LSAM_TRY((ce_gemm<T, true, true, STATS, 2, 4, 8, 4, 2>(a, s)));
+    }
+    const int blocks = M > 0 ? cdiv(M, 16) : 1;
+    if (M > 0 || reduction != LSAM_REDUCE_NONE) {
+        ce_loss_kernel<<<blocks, 1024, 0, s>>>(f.part, f.zt, pl.tiles_v, M, V, smooth, st, f.row_loss, loss, reduction);
+        LSAM_LAUNCH_CHECK();
+    }
+    if (blocks > 1 && reduction != LSAM_REDUCE_NONE) {
+        ce_sum_kernel<<<1, 1024, 0, s>>>(f.row_loss, st.n, loss, reduction);
+        LSAM_LAUNCH_CHECK();
+    }
+    return LSAM_OK;
+}
+
+template <typename T>
+int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float* gout, int M, int D, int V, float smooth, int reduction,
+                         const void* state, void* dx, long lddx, void* dw, long lddw, float* db, void* ws, size_t ws_bytes, hipStream_t s) {
+    LSAM_TRY(ce_check(M, D, V, reduction, smooth));
+    const CePlan<T> pl(M, D, V, !rows_direct<T>(w, ldw, D));
+    LSAM_REQUIRE(w && state && ws && (M == 0 || gout), LSAM_ERR_BAD_ARG, "linear_ce: null operand");
+    LSAM_REQUIRE(ldw >= D && (!dx || lddx >= D) && (!dw || lddw >= D) && aligned16(state) && aligned16(ws), LSAM_ERR_BAD_ARG,
+                 "linear_ce: a row stride below %d columns, or a workspace off its 16-byte alignment", D);
+    CeState st;
+    typename CePlan<T>::Bwd b;
+    pl.state(static_cast<char*>(const_cast<void*>(state)), &st);
+    LSAM_REQUIRE(pl.bwd(static_cast<char*>(ws), &b, dx != nullptr, dw != nullptr, db != nullptr) <= ws_bytes, LSAM_ERR_WORKSPACE,
+                 "linear_ce: workspace too small");
+    if (pl.pack_w) LSAM_TRY(gather<T>(w, ldw, nullptr, nullptr, V, D, pl.Dp, b.wp, s));
+    const char* W = pl.pack_w ? b.wp : static_cast<const char*>(w);
+    const long lw = pl.pack_w ? pl.Dp : ldw;
+    if (M > 0) {
+        ce_coef_kernel<<<cdiv(M, 256), 256, 0, s>>>(gout, reduction, st, b.coef, b.coef_s);
+        LSAM_LAUNCH_CHECK();
+    }
+    for (int v0 = 0, k = 0; v0 < V; v0 += pl.piece, ++k) {
+        const int nv = V - v0 < pl.piece ? V - v0 : pl.piece;
+        if (M > 0) {
+            CeArgs a{};
+            a.A = W + (size_t)v0 * lw * sizeof(T); a.lda = lw;
+            a.B = st.xc; a.ldb = pl.Dp;
+            a.I = nv; a.J = M; a.K = pl.Dp; a.n = st.n;
+            a.bias = bias ? bias + v0 : nullptr; a.tgt = st.tgt; a.i_base = v0;
+            a.base2 = st.base2; a.coef = b.coef; a.coef_s = b.coef_s; a.sm = smooth / (float)V; a.keep = 1.f - smooth;
+            a.dbp = db ? b.dbp + v0 : nullptr; a.dbp_ld = V;
+            a.out = b.dz; a.ldo = pl.piece; a.splits = 1;
+            LSAM_TRY((ce_gemm<T, true, true, DZ, 2, 4, 8, 4, 2>(a, s)));
+        }
+        if (dx && M > 0) {
+            CeArgs a{};
+            a.A = W + (size_t)v0 * lw * sizeof(T); a.lda = lw;
+            a.B = b.dz; a.ldb = pl.piece;
+            a.I = pl.Dp; a.J = M; a.K = nv; a.n = st.n;
+            a.out = b.dx; a.ldo = pl.Dp; a.split_stride = (long)M * pl.Dp; a.splits = pl.s_dx; a.accumulate = k > 0;
+            LSAM_TRY((ce_gemm<T, false, true, ACC, 2, 2, 8, 8, 1>(a, s)));
+        }
+        if (dw) {
+            const bool vec = D % 4 == 0 && lddw % 4 == 0 && aligned16(dw);
+            T* o = static_cast<T*>(dw) + (size_t)v0 * lddw;
+            CeArgs a{};
+            a.A = st.xc; a.lda = pl.Dp;
+            a.B = b.dz; a.ldb = pl.piece;
+            a.I = pl.Dp; a.J = nv; a.K = M; a.n = st.n; a.cols = D; a.vec = vec; a.splits = pl.s_dw;
+            if (pl.s_dw > 1) { a.out = b.dw; a.ldo = pl.Dp; a.split_stride = (long)pl.piece * pl.Dp; }
+            else { a.out = o; a.ldo = lddw; }
+            LSAM_TRY((ce_gemm<T, false, false, OUT, 2, 2, 8, 8, 1>(a, s)));
+            if (pl.s_dw > 1) {
+                const long blocks = ((long)nv * (pl.Dp / 4) + 255) / 256;
+                ce_dx_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(b.dw, a.split_stride, pl.s_dw, nullptr, nv, D, pl.Dp, vec, o, lddw);
+                LSAM_LAUNCH_CHECK();
+            }
+        }
+    }
+    if (dx && M > 0) {
+        const long blocks = ((long)M * (pl.Dp / 4) + 255) / 256;
+        ce_dx_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(b.dx, (long)M * pl.Dp, pl.s_dx, st.pos, M, D, pl.Dp,
+                                                                             D % 4 == 0 && lddx % 4 == 0 && aligned16(dx), static_cast<T*>(dx), lddx);
+        LSAM_LAUNCH_CHECK();
+    }
+    if (db) {
+        ce_db_kernel<<<cdiv(V, 256), 256, 0, s>>>(b.dbp, V, st.n, 256, V, db);
+        LSAM_LAUNCH_CHECK();
+    }
+    return LSAM_OK;
+}
+#define CE_INST(T)                                                                                                                          \
+    template size_t ce_state_bytes<T>(int, int);                                                                                           \
+    template size_t ce_ws_bytes<T>(int, int, int, const void*, long, float, int);                                                          \
+    template int launch_linear_ce_fwd<T>(const void*, long, const void*, long, const float*, const long long*, int, int, int, long long,   \
+                                         float, int, float*, void*, void*, size_t, hipStream_t);                                           \
+    template int launch_linear_ce_bwd<T>(const void*, long, const float*, const float*, int, int, int, float, int, const void*, void*,     \
+                                         long, void*, long, float*, void*, size_t, hipStream_t);
+CE_INST(float)
+CE_INST(bf16)
+}  // namespace lsam

@@ -242,3 +242,23 @@ class MaskLossSumsFn(torch.autograd.Function):
         alpha, gamma = ctx.cfg
         coef = g[..., :3].contiguous()
         return ops.mask_loss_bwd(logits, targets, coef, alpha, gamma).view(logits.shape), None, None, None
+
+
+class LinearCrossEntropyFn(torch.autograd.Function):
+    """loss_fns.linear_cross_entropy on rows: fp32 loss of x T [M, D], weight T [V, D], bias [V] or None, int64 target [M].
+    x itself is not kept: the forward's state holds the rows that count."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, target, ignore_index, label_smoothing, reduction):
+        loss, state = ops.linear_ce_fwd(x, weight, bias, target, ignore_index, label_smoothing, reduction)
+        ctx.save_for_backward(weight, bias, state)
+        ctx.cfg = (x.shape[0], label_smoothing, reduction)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        weight, bias, state = ctx.saved_tensors
+        M, label_smoothing, reduction = ctx.cfg
+        dx, dw, db = ops.linear_ce_bwd(g, state, weight, bias, M, label_smoothing, reduction, ctx.needs_input_grad[:3])
+        return dx, dw, db if db is None else db.to(bias.dtype), None, None, None, None

@@ -75,6 +75,36 @@ def iou_loss(inputs, targets, pred_ious, num_objects, loss_on_multimask=False, u
     return loss / num_objects if loss_on_multimask else loss.sum() / num_objects
 
 
+def linear_cross_entropy(inputs, weight, targets, bias=None, ignore_index: int = -100, label_smoothing: float = 0.0,
+                         reduction: str = "mean"):
+    """Softmax cross entropy of `inputs @ weight.T + bias` against class indices, as F.cross_entropy(F.linear(inputs, weight, bias),
+    targets, ...) defines it, without the scores ever in memory: forward and backward form them a tile, then a piece of the classes,
+    at a time (`lsam_linear_ce_fwd` / `_bwd`).
+
+    inputs [..., D] and weight [V, D]: both float32 or both bfloat16 (sums and statistics are fp32 either way); targets [...] integer;
+    bias [V] any float type: -inf takes a class out, finite values beyond +-1e9 (masks) count as that.  The loss is fp32: targets' shape under reduction="none" (0 where ignored), one value otherwise.
+    Rows whose target is `ignore_index` cost nothing and pass nothing on, whatever they hold.  A target outside [0, V) makes the loss
+    NaN (F.cross_entropy stops the process there); with no row left, "mean" is NaN and the gradients are zero."""
+    if not inputs.is_cuda:
+        raise LsamError("linear_cross_entropy runs on the MI355X only (no CPU or PyTorch fallback)")
+    if inputs.dim() < 1 or weight.dim() != 2 or inputs.shape[-1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise LsamError(f"linear_cross_entropy: inputs {tuple(inputs.shape)} do not match weight {tuple(weight.shape)}")
+    if inputs.dtype != weight.dtype or inputs.dtype not in (torch.float32, torch.bfloat16):
+        raise LsamError(f"linear_cross_entropy: inputs {inputs.dtype} and weight {weight.dtype} must both be float32 or both bfloat16")
+    if targets.shape != inputs.shape[:-1] or targets.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8, torch.int8):
+        raise LsamError(f"linear_cross_entropy: targets {tuple(targets.shape)} {targets.dtype} must be class indices of shape "
+                        f"{tuple(inputs.shape[:-1])}")
+    if bias is not None and (bias.shape != weight.shape[:1] or not bias.is_floating_point()):
+        raise LsamError(f"linear_cross_entropy: bias {tuple(bias.shape)} {bias.dtype} does not match {weight.shape[0]} classes")
+    if reduction not in ("none", "mean", "sum"):
+        raise ValueError(f"{reduction} is not a valid value for reduction")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"label_smoothing must be between 0.0 and 1.0, got {label_smoothing}")
+    loss = HA.LinearCrossEntropyFn.apply(inputs.reshape(-1, inputs.shape[-1]), weight, bias, targets.reshape(-1), int(ignore_index),
+                                         float(label_smoothing), reduction)
+    return loss.view(targets.shape) if reduction == "none" else loss
+
+
 class MultiStepMultiMasksAndIous(nn.Module):
     """loss_fns.py:132-313.  One `lsam_mask_loss_sums` pass per prediction step serves the focal, dice and IoU terms."""
 

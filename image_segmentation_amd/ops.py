@@ -765,3 +765,67 @@ def batched_outer(G: torch.Tensor, U: torch.Tensor) -> torch.Tensor:
     ws = torch.empty(lib().lsam_batched_outer_ws_floats(B, L, Cc), dtype=torch.float32, device=G.device)
     check(lib().lsam_batched_outer(dtype_code(U.dtype), ptr(G), ptr(U), ptr(out), ptr(ws), B, M, L, Cc, stream()))
     return out
+
+
+# ---- class loss over a large table (csrc/vocab_ce.hip) ------------------------------------------------------------------
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _same_device(*ts):
+    """The operands' one GPU: calls run there, on its current stream, whatever the current device is."""
+    _need_gpu(*ts)
+    devs = {t.device for t in ts if t is not None}
+    if len(devs) != 1:
+        raise _C.LsamError(f"operands on different devices: {sorted(map(str, devs))}")
+    return torch.cuda.device(devs.pop())
+
+
+def _unit_stride(t: torch.Tensor) -> torch.Tensor:
+    """2-D tensor whose rows are contiguous and do not overlap (a leading dimension is passed separately); else a copy."""
+    t = t.detach()
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+def _ld(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def linear_ce_fwd(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], target: torch.Tensor, ignore_index: int = -100,
+                  label_smoothing: float = 0.0, reduction: str = "mean"):
+    """(loss, state): softmax cross entropy of x [M, D] @ weight [V, D]^T + bias [V] against int64 target [M]; fp32 loss, [M] or 0-d.
+    `state` (uint8) is what linear_ce_bwd needs; it holds the selected rows of x, so x itself may change or go."""
+    with _same_device(x, weight, bias, target):
+        code = dtype_code(x.dtype)
+        x, weight, b = _unit_stride(x), _unit_stride(weight), _f32c(bias)
+        target = target.detach().to(torch.int64).contiguous()
+        (M, D), V = x.shape, weight.shape[0]
+        loss = torch.empty((M,) if reduction == "none" else (), dtype=torch.float32, device=x.device)
+        L, u8 = lib(), dict(dtype=torch.uint8, device=x.device)
+        state = torch.empty(L.lsam_linear_ce_state_bytes(code, M, D), **u8)
+        ws = torch.empty(L.lsam_linear_ce_ws_bytes(code, M, D, V, ptr(weight), _ld(weight), label_smoothing, 0), **u8)
+        check(L.lsam_linear_ce_fwd(code, ptr(x), _ld(x), ptr(weight), _ld(weight), ptr(b), ptr(target), M, D, V, ignore_index,
+                                   label_smoothing, REDUCTIONS[reduction], ptr(loss), ptr(state), ptr(ws), ws.numel(), stream()))
+    return loss, state
+
+
+def linear_ce_bwd(gout: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], M: int,
+                  label_smoothing: float = 0.0, reduction: str = "mean", want=(True, True, True)):
+    """(dx, dweight, dbias fp32) of linear_ce_fwd, None where not wanted; gout fp32 [M] or 0-d."""
+    with _same_device(gout, state, weight, bias):
+        code = dtype_code(weight.dtype)
+        weight, b, gout = _unit_stride(weight), _f32c(bias), _f32c(gout)
+        V, D = weight.shape
+        dx = torch.empty(M, D, dtype=weight.dtype, device=weight.device) if want[0] else None
+        dw = torch.empty(V, D, dtype=weight.dtype, device=weight.device) if want[1] else None
+        db = torch.empty(V, dtype=torch.float32, device=weight.device) if want[2] and bias is not None else None
+        L = lib()
+        flags = (dx is not None) + 2 * (dw is not None) + 4 * (db is not None)
+        if not flags:
+            return None, None, None
+        ws = torch.empty(L.lsam_linear_ce_ws_bytes(code, M, D, V, ptr(weight), _ld(weight), label_smoothing, flags), dtype=torch.uint8,
+                         device=weight.device)
+        check(L.lsam_linear_ce_bwd(code, ptr(weight), _ld(weight), ptr(b), ptr(gout), M, D, V, label_smoothing, REDUCTIONS[reduction],
+                                   ptr(state), ptr(dx), D, ptr(dw), D, ptr(db), ptr(ws), ws.numel(), stream()))
+    return dx, dw, db

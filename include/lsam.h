@@ -488,6 +488,27 @@ int lsam_hiera_backward_block(lsam_hiera_t* h, const float* grad_out, int batch,
                               float* const* host_lora_grads, void* arena, void* workspace, size_t workspace_bytes,
                               lsam_stream_t stream);
 
+/* ---- class loss over a large table: softmax cross entropy of z = x W^T + b, [M, V] scores never in memory ------------------------
+ * x T [M][ldx], w T [V][ldw] (D columns each), bias fp32 [V] or NULL, target int64 [M].  Rows whose target is `ignore` take no part;
+ * a target outside [0, V) makes its row's loss and gradient NaN (nothing is read out of range).
+ * A bias of -inf takes its class out; finite ones beyond +-1e9 count as that (x W^T itself has to stay within).
+ *   loss_m = (1 - smooth)(lse_m - z_mt) + smooth (lse_m - mean_v z_mv);  MEAN divides the sum by the rows that count (0 / 0 = NaN).
+ * loss fp32: [M] under LSAM_REDUCE_NONE (0 where ignored), one value otherwise.  `state` (lsam_linear_ce_state_bytes) is what the
+ * backward needs of the forward: row selection, statistics, and the selected rows of x.  `ws`: lsam_linear_ce_ws_bytes with grads = 0
+ * for the forward, else the sum of LSAM_CE_D{X,W,B} for the gradients wanted; the same w / ldw as in the call. */
+enum { LSAM_REDUCE_NONE = 0, LSAM_REDUCE_MEAN = 1, LSAM_REDUCE_SUM = 2 };
+enum { LSAM_CE_DX = 1, LSAM_CE_DW = 2, LSAM_CE_DB = 4 };
+size_t lsam_linear_ce_state_bytes(int dtype, int M, int D);
+size_t lsam_linear_ce_ws_bytes(int dtype, int M, int D, int V, const void* w, long ldw, float smooth, int grads);
+int lsam_linear_ce_fwd(int dtype, const void* x, long ldx, const void* w, long ldw, const float* bias, const long long* target, int M,
+                       int D, int V, long long ignore, float smooth, int reduction, float* loss, void* state, void* ws, size_t ws_bytes,
+                       lsam_stream_t stream);
+/* gout fp32: [M] under NONE, one value otherwise.  dx T [M][lddx] (zeros in ignored rows), dw T [V][lddw], db fp32 [V], each written
+ * whole; NULL where not wanted. */
+int lsam_linear_ce_bwd(int dtype, const void* w, long ldw, const float* bias, const float* gout, int M, int D, int V, float smooth,
+                       int reduction, const void* state, void* dx, long lddx, void* dw, long lddw, float* db, void* ws, size_t ws_bytes,
+                       lsam_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -161,6 +161,12 @@ def lib() -> C.CDLL:
         L.lsam_linear_ce_ws_bytes.argtypes = [i, i, i, i, vp, l, f, i]
         L.lsam_linear_ce_fwd.argtypes = [i, vp, l, vp, l, vp, vp, i, i, i, ll, f, i, vp, vp, vp, sz, vp]
         L.lsam_linear_ce_bwd.argtypes = [i, vp, l, vp, vp, i, i, i, f, i, vp, vp, l, vp, l, vp, vp, sz, vp]
+        L.lsam_group_norm_act_ws_bytes.restype = L.lsam_clip_grads_ws_bytes.restype = sz
+        L.lsam_group_norm_act_ws_bytes.argtypes = [i] * 5
+        L.lsam_group_norm_act_fwd.argtypes = [i, vp, l, l, vp, vp, i, i, i, i, f, i, vp, vp, vp, sz, vp]
+        L.lsam_group_norm_act_bwd.argtypes = [i, vp, l, l, vp, l, l, vp, vp, vp, i, i, i, i, i, vp, vp, vp, vp, sz, vp]
+        L.lsam_clip_grads_ws_bytes.argtypes = [vp, i]
+        L.lsam_clip_grads.argtypes = [vp, vp, vp, vp, i, C.c_double, i, C.c_double, vp, vp, sz, vp]
         L.lsam_prof_arm.argtypes = [i]
         L.lsam_prof_read.argtypes = [i, vp, vp, vp, vp]
         L.lsam_prof_bracket_cost.argtypes = [vp, i, vp]
@@ -210,5 +216,6 @@ EXPORTED = [
     "lsam_qkv_window4_attention_image_bytes", "lsam_qkv_window4_attention_pack", "lsam_qkv_window4_attention_fwd",
     "lsam_stream_linear_image_bytes", "lsam_stream_linear_pack", "lsam_stream_linear_fwd",
     "lsam_linear_ce_state_bytes", "lsam_linear_ce_ws_bytes", "lsam_linear_ce_fwd", "lsam_linear_ce_bwd",
+    "lsam_group_norm_act_ws_bytes", "lsam_group_norm_act_fwd", "lsam_group_norm_act_bwd", "lsam_clip_grads_ws_bytes", "lsam_clip_grads",
     "lsam_outer_reduce_static_max_ws", "lsam_outer_reduce_static_init", "lsam_outer_reduce_static",
 ]

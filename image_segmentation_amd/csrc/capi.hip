@@ -384,4 +384,35 @@ int lsam_linear_ce_bwd(int dtype, const void* w, long ldw, const float* bias, co
              launch_linear_ce_bwd<bf16>(w, ldw, bias, gout, M, D, V, smooth, reduction, state, dx, lddx, dw, lddw, db, ws, ws_bytes, s));
 }
 
+size_t lsam_group_norm_act_ws_bytes(int N, int P, int C, int G, int backward) {
+    return C > 0 && G > 0 ? gn_ws_bytes(N, P, C, G, backward) : 0;
+}
+int lsam_group_norm_act_fwd(int dtype, const void* x, long sx, long px, const float* gamma, const float* beta, int N, int P, int C, int G,
+                            float eps, int act, void* y, float* stats, void* ws, size_t ws_bytes, lsam_stream_t stream) {
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    DISPATCH(dtype, launch_group_norm_act_fwd<float>(x, sx, px, gamma, beta, N, P, C, G, eps, act, y, stats, ws, ws_bytes, s),
+             launch_group_norm_act_fwd<bf16>(x, sx, px, gamma, beta, N, P, C, G, eps, act, y, stats, ws, ws_bytes, s));
+}
+int lsam_group_norm_act_bwd(int dtype, const void* dy, long sy, long py, const void* x, long sx, long px, const float* gamma,
+                            const float* beta, const float* stats, int N, int P, int C, int G, int act, void* dx, float* dgamma,
+                            float* dbeta, void* ws, size_t ws_bytes, lsam_stream_t stream) {
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    DISPATCH(dtype,
+             launch_group_norm_act_bwd<float>(dy, sy, py, x, sx, px, gamma, beta, stats, N, P, C, G, act, dx, dgamma, dbeta, ws, ws_bytes, s),
+             launch_group_norm_act_bwd<bf16>(dy, sy, py, x, sx, px, gamma, beta, stats, N, P, C, G, act, dx, dgamma, dbeta, ws, ws_bytes, s));
+}
+
+size_t lsam_clip_grads_ws_bytes(const long long* host_n, int count) { return clip_ws_bytes(host_n, count); }
+int lsam_clip_grads(const unsigned long long* host_src, const unsigned long long* host_dst, const long long* host_n,
+                    const unsigned char* host_kind, int count, double max_norm, int inf, double scale, float* out, void* ws,
+                    size_t ws_bytes, lsam_stream_t stream) {
+    try {   // the list is laid out in host memory
+        return launch_clip_grads(host_src, host_dst, host_n, host_kind, count, max_norm, inf, scale, out, ws, ws_bytes,
+                                 static_cast<hipStream_t>(stream));
+    } catch (...) {
+        set_error("clip_grads: out of host memory");
+        return LSAM_ERR_BAD_ARG;
+    }
+}
+
 }  // extern "C"

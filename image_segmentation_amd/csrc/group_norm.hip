@@ -1,0 +1,502 @@
+// Group norm with an activation over channels-last maps, forward and backward.
+//
+//   xhat = (x - mean_ng) rstd_ng,  h = xhat gamma_c + beta_c,  y = act(h)          mean / variance over the P pixels x C/G channels
+//   dh = dy act'(h),  dgamma_c = sum_np dh xhat,  dbeta_c = sum_np dh,
+//   dx = rstd (gamma dh - (S1 + xhat S2) / m),  S1 = sum_group gamma dh,  S2 = sum_group gamma dh xhat,  m = P C/G
+//
+// Memory-bound both ways.  A workgroup walks a range of pixels with whole rows of channels: consecutive lanes take consecutive
+// 16-byte pieces of a row, a thread keeps to its channels, so what a channel needs stays in its registers and the sums over pixels
+// need no exchange until the range ends.  Sums over ranges are joined in a fixed order by the next kernel: same bits every time.
+#include "kernels.hpp"
+
+namespace lsam {
+namespace {
+constexpr int NT = 256, MAXC = 8192;
+
+// Thread layout over a row of C channels: `cw` threads side by side take V channels each, `rw` pixels at a time, in `blocks` column
+// blocks when a row is wider than the workgroup.
+struct Lay {
+    int cols, cw, rw, blocks;
+    __host__ __device__ Lay(int C, int V) {
+        cols = C / V;
+        blocks = (cols + NT - 1) / NT;
+        cw = (cols + blocks - 1) / blocks;
+        rw = NT / cw;
+    }
+};
+
+template <typename T, int V> __device__ __forceinline__ void load(const T* p, float (&v)[V]) {
+    if constexpr (V == 1) v[0] = to_f(*p);
+    else {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        T e[V];
+        __builtin_memcpy(e, &u, 16);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = to_f(e[j]);
+    }
+}
+template <typename T, int V> __device__ __forceinline__ void store(T* p, const float (&v)[V]) {
+    if constexpr (V == 1) *p = from_f<T>(v[0]);
+    else {
+        T e[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) e[j] = from_f<T>(v[j]);
+        uint4 u;
+        __builtin_memcpy(&u, e, 16);
+        *reinterpret_cast<uint4*>(p) = u;
+    }
+}
+
+__device__ __forceinline__ float sigmoid(float h) { return __builtin_amdgcn_rcpf(1.f + __expf(-h)); }
+// EXACT: erff, for fp32 results; else the rational form (|error| < 1.5e-7), whose exponential the derivative shares
+template <bool EXACT> __device__ __forceinline__ float act_fwd(int act, float h) {
+    if (act == LSAM_ACT_RELU) return h < 0.f ? 0.f : h;
+    if (act == LSAM_ACT_SILU) return h * sigmoid(h);
+    if (act == LSAM_ACT_GELU) return 0.5f * h * (1.f + (EXACT ? erff(h * 0.70710678118654752f) : erf_fast(h * 0.70710678118654752f)));
+    return h;
+}
+template <bool EXACT> __device__ __forceinline__ float act_slope(int act, float h) {
+    if (act == LSAM_ACT_RELU) return h <= 0.f ? 0.f : 1.f;
+    if (act == LSAM_ACT_SILU) {
+        const float q = sigmoid(h);
+        return q * fmaf(h, 1.f - q, 1.f);
+    }
+    if (act == LSAM_ACT_GELU) return gelu_grad_t<!EXACT>(h);
+    return 1.f;
+}
+
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+    return x;
+}
+
+// Mean and M2 = sum (x - mean)^2 of `k` pieces with counts n_i, means m_i, M2_i, one wave: mean first, then the spread around it.
+template <typename F> __device__ __forceinline__ void join(int k, int lane, F piece, float& mean, float& m2, float& count) {
+    float n = 0.f, s = 0.f;
+    for (int i = lane; i < k; i += 64) {
+        float c, m, q;
+        piece(i, c, m, q);
+        n += c;
+        s += c * m;
+    }
+    count = wave_sum(n);
+    mean = wave_sum(s) / count;
+    float v = 0.f;
+    for (int i = lane; i < k; i += 64) {
+        float c, m, q;
+        piece(i, c, m, q);
+        v += q + c * (m - mean) * (m - mean);
+    }
+    m2 = wave_sum(v);
+}
+
+struct GnArgs {
+    const void* x; long sx, px;    // sample and pixel strides (elements)
+    const void* dy; long sy, py;
+    const float *gamma, *beta;     // or null: 1, 0
+    int N, P, C, G, act, splits, rows;   // rows: pixels a split
+    float eps;
+    float* part;                   // fwd: [N][splits][G][2] (mean, M2); bwd: [N][splits][C][2] (sum dh, sum dh xhat)
+    float* stats;                  // [N][G][2] mean, rstd
+    float* chan;                   // bwd: [N][C][2] the sums over the splits
+    float* coef;                   // bwd: [N][G][2] S1 / m, S2 / m
+    void* out;                     // [N][P][C]
+    float *dgamma, *dbeta;
+};
+
+// per-range statistics.  A thread takes its first pixel as the pivot of its channels: sums of (x - pivot) and their squares cannot
+// cancel by more than the number of its pixels, however far the mean is from zero.
+template <typename T, int V>
+__global__ __launch_bounds__(NT) void gn_stats_kernel(const GnArgs p) {
+    extern __shared__ float sm[];              // mean[C], m2[C], then the threads' pieces
+    float* cm = sm;
+    float* cq = sm + p.C;
+    float* tm = sm + 2 * p.C;
+    float* tq = tm + NT * V;
+    const Lay l(p.C, V);
+    const int tid = threadIdx.x, tx = tid % l.cw, ty = tid / l.cw, lane = tid & 63;
+    const int n = blockIdx.x / p.splits, sp = blockIdx.x - n * p.splits;
+    const int p0 = sp * p.rows, p1 = min(p.P, p0 + p.rows), cnt = p1 - p0;
+    const T* x = static_cast<const T*>(p.x) + n * p.sx;
+    for (int b = 0; b < l.blocks; ++b) {
+        const int col = b * l.cw + tx;
+        const bool on = ty < l.rw && col < l.cols && p0 + ty < p1;
+        float k[V], s[V], q[V];
+        int mine = 0;
+        if (on) {
+            const T* xp = x + (long)(p0 + ty) * p.px + col * V;
+            load<T, V>(xp, k);
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[j] = q[j] = 0.f;
+            mine = (cnt - ty + l.rw - 1) / l.rw;
+            const long step = (long)l.rw * p.px;
+#pragma unroll 4
+            for (int i = 1; i < mine; ++i) {
+                float v[V];
+                load<T, V>(xp + i * step, v);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float d = v[j] - k[j];
+                    s[j] += d;
+                    q[j] = fmaf(d, d, q[j]);
+                }
+            }
+        }
+        if (b) __syncthreads();
+        if (ty < l.rw) {
+            const float inv = mine ? 1.f / (float)mine : 0.f;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                tm[(ty * l.cw + tx) * V + j] = on ? fmaf(s[j], inv, k[j]) : 0.f;
+                tq[(ty * l.cw + tx) * V + j] = on ? fmaxf(0.f, q[j] - s[j] * s[j] * inv) : 0.f;
+            }
+        }
+        __syncthreads();
+        for (int c = tid; c < l.cw * V && b * l.cw * V + c < p.C; c += NT) {
+            float sum = 0.f, spread = 0.f;
+            for (int r = 0; r < l.rw && r < cnt; ++r) sum += tm[r * l.cw * V + c] * (float)((cnt - r + l.rw - 1) / l.rw);
+            const float mean = sum / (float)cnt;
+            for (int r = 0; r < l.rw && r < cnt; ++r) {
+                const float d = tm[r * l.cw * V + c] - mean;
+                spread += tq[r * l.cw * V + c] + d * d * (float)((cnt - r + l.rw - 1) / l.rw);
+            }
+            cm[b * l.cw * V + c] = mean;
+            cq[b * l.cw * V + c] = spread;
+        }
+    }
+    __syncthreads();
+    const int cpg = p.C / p.G;
+    for (int g = tid >> 6; g < p.G; g += NT / 64) {
+        float mean, m2, count;
+        join(cpg, lane, [&](int i, float& c, float& m, float& q) { c = (float)cnt; m = cm[g * cpg + i]; q = cq[g * cpg + i]; }, mean, m2, count);
+        if (lane == 0) {
+            float* o = p.part + ((size_t)blockIdx.x * p.G + g) * 2;
+            o[0] = mean;
+            o[1] = m2;
+        }
+    }
+}
+
+// what a thread needs of its channels
+template <int V> struct Chan {
+    float mean[V], rstd[V], gamma[V], beta[V];
+    __device__ __forceinline__ void get(const GnArgs& p, const float* st, int c0) {
+        const int cpg = p.C / p.G;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int g = (c0 + j) / cpg;
+            mean[j] = st[2 * g];
+            rstd[j] = st[2 * g + 1];
+            gamma[j] = p.gamma ? p.gamma[c0 + j] : 1.f;
+            beta[j] = p.beta ? p.beta[c0 + j] : 0.f;
+        }
+    }
+};
+
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(NT) void gn_apply_kernel(const GnArgs p) {
+    extern __shared__ float sm[];   // [G][2]
+    const Lay l(p.C, V);
+    const int tid = threadIdx.x, tx = tid % l.cw, ty = tid / l.cw, lane = tid & 63;
+    const int n = blockIdx.x / p.splits, sp = blockIdx.x - n * p.splits;
+    const int p0 = sp * p.rows, p1 = min(p.P, p0 + p.rows), cpg = p.C / p.G;
+    for (int g = tid >> 6; g < p.G; g += NT / 64) {
+        float mean, m2, count;
+        join(p.splits, lane, [&](int i, float& c, float& m, float& q) {
+            const float* o = p.part + ((size_t)(n * p.splits + i) * p.G + g) * 2;
+            c = (float)(min(p.P, (i + 1) * p.rows) - i * p.rows) * (float)cpg;
+            m = o[0];
+            q = o[1];
+        }, mean, m2, count);
+        if (lane == 0) {
+            const float rstd = 1.f / sqrtf(m2 / count + p.eps);
+            sm[2 * g] = mean;
+            sm[2 * g + 1] = rstd;
+            if (sp == 0 && p.stats) {
+                p.stats[((size_t)n * p.G + g) * 2] = mean;
+                p.stats[((size_t)n * p.G + g) * 2 + 1] = rstd;
+            }
+        }
+    }
+    __syncthreads();
+    const T* x = static_cast<const T*>(p.x) + n * p.sx;
+    T* y = static_cast<T*>(p.out) + (size_t)n * p.P * p.C;
+    for (int b = 0; b < l.blocks; ++b) {
+        const int col = b * l.cw + tx;
+        if (ty >= l.rw || col >= l.cols) continue;
+        Chan<V> ch;
+        ch.get(p, sm, col * V);
+#pragma unroll
+        for (int j = 0; j < V; ++j) ch.gamma[j] *= ch.rstd[j];
+#pragma unroll 4
+        for (int i = p0 + ty; i < p1; i += l.rw) {
+            float v[V];
+            load<T, V>(x + (long)i * p.px + col * V, v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = act_fwd<sizeof(T) == 4>(ACT, fmaf(v[j] - ch.mean[j], ch.gamma[j], ch.beta[j]));
+            store<T, V>(y + (size_t)i * p.C + col * V, v);
+        }
+    }
+}
+
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(NT) void gn_bwd_sums_kernel(const GnArgs p) {
+    extern __shared__ float sm[];
+    const Lay l(p.C, V);
+    const int tid = threadIdx.x, tx = tid % l.cw, ty = tid / l.cw;
+    const int n = blockIdx.x / p.splits, sp = blockIdx.x - n * p.splits;
+    const int p0 = sp * p.rows, p1 = min(p.P, p0 + p.rows);
+    const T* x = static_cast<const T*>(p.x) + n * p.sx;
+    const T* dy = static_cast<const T*>(p.dy) + n * p.sy;
+    float *ta = sm, *tb = sm + NT * V;
+    for (int b = 0; b < l.blocks; ++b) {
+        const int col = b * l.cw + tx;
+        float a[V], c[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) a[j] = c[j] = 0.f;
+        if (ty < l.rw && col < l.cols) {
+            Chan<V> ch;
+            ch.get(p, p.stats + (size_t)n * p.G * 2, col * V);
+#pragma unroll 2
+            for (int i = p0 + ty; i < p1; i += l.rw) {
+                float v[V], d[V];
+                load<T, V>(x + (long)i * p.px + col * V, v);
+                load<T, V>(dy + (long)i * p.py + col * V, d);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float xh = (v[j] - ch.mean[j]) * ch.rstd[j];
+                    const float dh = d[j] * act_slope<sizeof(T) == 4>(ACT, fmaf(xh, ch.gamma[j], ch.beta[j]));
+                    a[j] += dh;
+                    c[j] = fmaf(dh, xh, c[j]);
+                }
+            }
+        }
+        if (b) __syncthreads();
+        if (ty < l.rw) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                ta[(ty * l.cw + tx) * V + j] = a[j];
+                tb[(ty * l.cw + tx) * V + j] = c[j];
+            }
+        }
+        __syncthreads();
+        for (int k = tid; k < l.cw * V && b * l.cw * V + k < p.C; k += NT) {
+            float s = 0.f, t = 0.f;
+            for (int r = 0; r < l.rw; ++r) {
+                s += ta[r * l.cw * V + k];
+                t += tb[r * l.cw * V + k];
+            }
+            float* o = p.part + ((size_t)blockIdx.x * p.C + b * l.cw * V + k) * 2;
+            o[0] = s;
+            o[1] = t;
+        }
+    }
+}
+
+// one workgroup a (sample, group): its channels' sums over the ranges, and the two group sums
+__global__ __launch_bounds__(NT) void gn_bwd_join_kernel(const GnArgs p) {
+    __shared__ float r1[NT / 64], r2[NT / 64];
+    const int n = blockIdx.x / p.G, g = blockIdx.x - n * p.G, cpg = p.C / p.G, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float s1 = 0.f, s2 = 0.f;
+    for (int c = wave; c < cpg; c += NT / 64) {   // a wave a channel, lanes over the ranges
+        const int ch = g * cpg + c;
+        float a = 0.f, b = 0.f;
+        for (int s = lane; s < p.splits; s += 64) {
+            const float* o = p.part + ((size_t)(n * p.splits + s) * p.C + ch) * 2;
+            a += o[0];
+            b += o[1];
+        }
+        a = wave_sum(a);
+        b = wave_sum(b);
+        if (lane == 0) {
+            p.chan[((size_t)n * p.C + ch) * 2] = a;
+            p.chan[((size_t)n * p.C + ch) * 2 + 1] = b;
+        }
+        const float gm = p.gamma ? p.gamma[ch] : 1.f;
+        s1 = fmaf(gm, a, s1);
+        s2 = fmaf(gm, b, s2);
+    }
+    if (lane == 0) { r1[wave] = s1; r2[wave] = s2; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float a = 0.f, b = 0.f;
+        for (int w = 0; w < NT / 64; ++w) { a += r1[w]; b += r2[w]; }
+        const float m = (float)p.P * (float)cpg;
+        p.coef[2 * blockIdx.x] = a / m;
+        p.coef[2 * blockIdx.x + 1] = b / m;
+    }
+}
+
+template <typename T, int V, int ACT>
+__global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(const GnArgs p) {
+    const int tid = threadIdx.x;
+    if ((int)blockIdx.x >= p.N * p.splits) {   // the workgroups behind the maps': dgamma, dbeta
+        const int c = ((int)blockIdx.x - p.N * p.splits) * NT + tid;
+        if (c < p.C) {
+            float a = 0.f, b = 0.f;
+            for (int n = 0; n < p.N; ++n) {
+                a += p.chan[((size_t)n * p.C + c) * 2];
+                b += p.chan[((size_t)n * p.C + c) * 2 + 1];
+            }
+            if (p.dbeta) p.dbeta[c] = a;
+            if (p.dgamma) p.dgamma[c] = b;
+        }
+        return;
+    }
+    const Lay l(p.C, V);
+    const int tx = tid % l.cw, ty = tid / l.cw, cpg = p.C / p.G;
+    const int n = blockIdx.x / p.splits, sp = blockIdx.x - n * p.splits;
+    const int p0 = sp * p.rows, p1 = min(p.P, p0 + p.rows);
+    const T* x = static_cast<const T*>(p.x) + n * p.sx;
+    const T* dy = static_cast<const T*>(p.dy) + n * p.sy;
+    T* dx = static_cast<T*>(p.out) + (size_t)n * p.P * p.C;
+    for (int b = 0; b < l.blocks; ++b) {
+        const int col = b * l.cw + tx;
+        if (ty >= l.rw || col >= l.cols) continue;
+        Chan<V> ch;
+        ch.get(p, p.stats + (size_t)n * p.G * 2, col * V);
+        float c1[V], c2[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float* o = p.coef + ((size_t)n * p.G + (col * V + j) / cpg) * 2;
+            c1[j] = o[0];
+            c2[j] = o[1];
+        }
+#pragma unroll 2
+        for (int i = p0 + ty; i < p1; i += l.rw) {
+            float v[V], d[V];
+            load<T, V>(x + (long)i * p.px + col * V, v);
+            load<T, V>(dy + (long)i * p.py + col * V, d);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float xh = (v[j] - ch.mean[j]) * ch.rstd[j];
+                const float dg = d[j] * act_slope<sizeof(T) == 4>(ACT, fmaf(xh, ch.gamma[j], ch.beta[j])) * ch.gamma[j];
+                v[j] = ch.rstd[j] * (dg - fmaf(xh, c2[j], c1[j]));
+            }
+            store<T, V>(dx + (size_t)i * p.C + col * V, v);
+        }
+    }
+}
+
+// pixels a range: enough ranges for four workgroups a compute unit, at least eight pixels a thread where there are that many
+void ranges(GnArgs& p, int V) {
+    const Lay l(p.C, V);
+    int s = (4 * 256 + p.N - 1) / p.N;
+    const int most = cdiv(p.P, l.rw * 8);
+    if (s > most) s = most;
+    if (s < 1) s = 1;
+    p.rows = cdiv(cdiv(p.P, s), l.rw) * l.rw;
+    p.splits = cdiv(p.P, p.rows);
+}
+int vec_of(int esz, const GnArgs& p, bool with_dy) {
+    const int V = 16 / esz;
+    const bool ok = p.C % V == 0 && p.px % V == 0 && p.sx % V == 0 && aligned16(p.x) && (!p.out || aligned16(p.out)) &&
+                    (!with_dy || (p.py % V == 0 && p.sy % V == 0 && aligned16(p.dy)));
+    return ok ? V : 1;
+}
+template <typename T, int V> int run_fwd(const GnArgs& p, hipStream_t s) {
+    gn_stats_kernel<T, V><<<p.N * p.splits, NT, (2 * p.C + 2 * NT * V) * sizeof(float), s>>>(p);
+    LSAM_LAUNCH_CHECK();
+    auto k = p.act == LSAM_ACT_RELU   ? gn_apply_kernel<T, V, LSAM_ACT_RELU>
+             : p.act == LSAM_ACT_SILU ? gn_apply_kernel<T, V, LSAM_ACT_SILU>
+             : p.act == LSAM_ACT_GELU ? gn_apply_kernel<T, V, LSAM_ACT_GELU>
+                                      : gn_apply_kernel<T, V, LSAM_ACT_NONE>;
+    k<<<p.N * p.splits, NT, 2 * p.G * sizeof(float), s>>>(p);
+    LSAM_LAUNCH_CHECK();
+    return LSAM_OK;
+}
+template <typename T, int V> int run_bwd(const GnArgs& p, hipStream_t s) {
+    auto k = p.act == LSAM_ACT_RELU   ? gn_bwd_sums_kernel<T, V, LSAM_ACT_RELU>
+             : p.act == LSAM_ACT_SILU ? gn_bwd_sums_kernel<T, V, LSAM_ACT_SILU>
+             : p.act == LSAM_ACT_GELU ? gn_bwd_sums_kernel<T, V, LSAM_ACT_GELU>
+                                      : gn_bwd_sums_kernel<T, V, LSAM_ACT_NONE>;
+    k<<<p.N * p.splits, NT, 2 * NT * V * sizeof(float), s>>>(p);
+    LSAM_LAUNCH_CHECK();
+    gn_bwd_join_kernel<<<p.N * p.G, NT, 0, s>>>(p);
+    LSAM_LAUNCH_CHECK();
+    auto a = p.act == LSAM_ACT_RELU   ? gn_bwd_apply_kernel<T, V, LSAM_ACT_RELU>
+             : p.act == LSAM_ACT_SILU ? gn_bwd_apply_kernel<T, V, LSAM_ACT_SILU>
+             : p.act == LSAM_ACT_GELU ? gn_bwd_apply_kernel<T, V, LSAM_ACT_GELU>
+                                      : gn_bwd_apply_kernel<T, V, LSAM_ACT_NONE>;
+    a<<<p.N * p.splits + cdiv(p.C, NT), NT, 0, s>>>(p);
+    LSAM_LAUNCH_CHECK();
+    return LSAM_OK;
+}
+
+int gn_check(int N, int P, int C, int G, int act, long sx, long px) {
+    LSAM_REQUIRE(N >= 0 && P >= 0 && C > 0 && G > 0 && C % G == 0, LSAM_ERR_BAD_ARG, "group_norm_act: %d samples, %d pixels, %d channels in %d groups", N, P,
+                 C, G);
+    LSAM_REQUIRE(C <= MAXC && (long)N * G < (1l << 24) && N < (1 << 20) && P < (1 << 30), LSAM_ERR_UNSUPPORTED,
+                 "group_norm_act: %d samples, %d pixels, %d channels, %d groups", N, P, C, G);
+    LSAM_REQUIRE(act >= LSAM_ACT_NONE && act <= LSAM_ACT_GELU, LSAM_ERR_BAD_ARG, "group_norm_act: activation %d", act);
+    LSAM_REQUIRE(px >= 0 && sx >= 0, LSAM_ERR_BAD_ARG, "group_norm_act: strides %ld, %ld", sx, px);
+    return LSAM_OK;
+}
+}  // namespace
+
+// the most that either layout needs
+size_t gn_ws_bytes(int N, int P, int C, int G, int backward) {
+    size_t most = 0;
+    for (int V : {1, 4, 8}) {
+        if (C % V) continue;
+        GnArgs p{};
+        p.N = N > 0 ? N : 1; p.P = P > 0 ? P : 1; p.C = C;
+        ranges(p, V);
+        const size_t n = backward ? ((size_t)p.N * p.splits * C * 2 + (size_t)p.N * C * 2 + (size_t)p.N * G * 2) * sizeof(float)
+                                  : (size_t)p.N * p.splits * G * 2 * sizeof(float);
+        if (n > most) most = n;
+    }
+    return most;
+}
+
+template <typename T>
+int launch_group_norm_act_fwd(const void* x, long sx, long px, const float* gamma, const float* beta, int N, int P, int C, int G, float eps, int act,
+                              void* y, float* stats, void* ws, size_t ws_bytes, hipStream_t s) {
+    LSAM_TRY(gn_check(N, P, C, G, act, sx, px));
+    if (N == 0 || P == 0) return LSAM_OK;
+    LSAM_REQUIRE(x && y && ws && aligned16(ws), LSAM_ERR_BAD_ARG, "group_norm_act: null operand or workspace off its 16-byte alignment");
+    LSAM_REQUIRE(ws_bytes >= gn_ws_bytes(N, P, C, G, 0), LSAM_ERR_WORKSPACE, "group_norm_act: workspace too small");
+    GnArgs p{};
+    p.x = x; p.sx = sx; p.px = px; p.gamma = gamma; p.beta = beta; p.N = N; p.P = P; p.C = C; p.G = G; p.act = act; p.eps = eps;
+    p.part = static_cast<float*>(ws); p.stats = stats; p.out = y;
+    const int V = vec_of(sizeof(T), p, false);
+    ranges(p, V);
+    return V > 1 ? run_fwd<T, 16 / sizeof(T)>(p, s) : run_fwd<T, 1>(p, s);
+}
+
+template <typename T>
+int launch_group_norm_act_bwd(const void* dy, long sy, long py, const void* x, long sx, long px, const float* gamma, const float* beta,
+                              const float* stats, int N, int P, int C, int G, int act, void* dx, float* dgamma, float* dbeta, void* ws,
+                              size_t ws_bytes, hipStream_t s) {
+    LSAM_TRY(gn_check(N, P, C, G, act, sx, px));
+    LSAM_TRY(gn_check(N, P, C, G, act, sy, py));
+    GnArgs p{};
+    p.N = N; p.P = P; p.C = C; p.G = G; p.act = act;
+    LSAM_REQUIRE(ws && aligned16(ws), LSAM_ERR_BAD_ARG, "group_norm_act: null workspace or off its 16-byte alignment");
+    LSAM_REQUIRE(ws_bytes >= gn_ws_bytes(N, P, C, G, 1), LSAM_ERR_WORKSPACE, "group_norm_act: workspace too small");
+    p.x = x; p.sx = sx; p.px = px; p.dy = dy; p.sy = sy; p.py = py; p.gamma = gamma; p.beta = beta; p.stats = const_cast<float*>(stats);
+    p.out = dx; p.dgamma = dgamma; p.dbeta = dbeta;
+    p.chan = static_cast<float*>(ws);
+    p.coef = p.chan + (size_t)(N > 0 ? N : 1) * C * 2;
+    p.part = p.coef + (size_t)(N > 0 ? N : 1) * G * 2;
+    if (N == 0 || P == 0) {   // nothing but zero sums: the workgroups behind no maps
+        p.N = 0;
+        p.splits = 1;
+        gn_bwd_apply_kernel<T, 1, LSAM_ACT_NONE><<<cdiv(C, NT), NT, 0, s>>>(p);
+        LSAM_LAUNCH_CHECK();
+        return LSAM_OK;
+    }
+    LSAM_REQUIRE(x && dy && dx && stats, LSAM_ERR_BAD_ARG, "group_norm_act: null operand");
+    const int V = vec_of(sizeof(T), p, true);
+    ranges(p, V);
+    return V > 1 ? run_bwd<T, 16 / sizeof(T)>(p, s) : run_bwd<T, 1>(p, s);
+}
+#define GN_INST(T)                                                                                                                              \
+    template int launch_group_norm_act_fwd<T>(const void*, long, long, const float*, const float*, int, int, int, int, float, int, void*,       \
+                                              float*, void*, size_t, hipStream_t);                                                             \
+    template int launch_group_norm_act_bwd<T>(const void*, long, long, const void*, long, long, const float*, const float*, const float*, int,  \
+                                              int, int, int, int, void*, float*, float*, void*, size_t, hipStream_t);
+GN_INST(float)
+GN_INST(bf16)
+}  // namespace lsam

@@ -247,4 +247,19 @@ template <typename T>
 int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float* gout, int M, int D, int V, float smooth, int reduction,
                          const void* state, void* dx, long lddx, void* dw, long lddw, float* db, void* ws, size_t ws_bytes, hipStream_t s);
 
+// group norm with an activation, channels last (group_norm.hip); strides in elements, y / dx contiguous [N][P][C]
+size_t gn_ws_bytes(int N, int P, int C, int G, int backward);
+template <typename T>
+int launch_group_norm_act_fwd(const void* x, long sx, long px, const float* gamma, const float* beta, int N, int P, int C, int G, float eps, int act,
+                              void* y, float* stats, void* ws, size_t ws_bytes, hipStream_t s);
+template <typename T>
+int launch_group_norm_act_bwd(const void* dy, long sy, long py, const void* x, long sx, long px, const float* gamma, const float* beta,
+                              const float* stats, int N, int P, int C, int G, int act, void* dx, float* dgamma, float* dbeta, void* ws,
+                              size_t ws_bytes, hipStream_t s);
+
+// global norm of a list of tensors and clipping by it (grad_clip.hip); the arrays are host memory, the addresses in them device
+size_t clip_ws_bytes(const long long* n, int count);
+int launch_clip_grads(const unsigned long long* src, const unsigned long long* dst, const long long* n, const unsigned char* kind, int count,
+                      double max_norm, int inf, double scale, float* out, void* ws, size_t ws_bytes, hipStream_t s);
+
 }  // namespace lsam

@@ -17,10 +17,62 @@ from inside the backward -- the mean over one rank is the identity, so results s
 without any process group (plain `python bench.py`) are the calls no-ops.  `stats` counts the collectives issued."""
 from __future__ import annotations
 
-from typing import Iterable, List, Optional
+from typing import Iterable, List, Optional, Sequence, Union
 
 import torch
 import torch.distributed as dist
+
+from . import ops
+
+
+@torch.no_grad()
+def clip_grads_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0, out: Optional[Sequence[torch.Tensor]] = None,
+                grad_scale: float = 1.0, error_if_nonfinite: bool = False) -> torch.Tensor:
+    """The global norm of `grad_scale * grads` (fp32, 0-d, on the device) and the gradients scaled by grad_scale * min(1, max_norm /
+    (norm + 1e-6)), in place or into `out`.
+
+    fp32 / bf16 tensors of any mix on one GPU; `out` may have other types than `grads` (bf16 gradients into fp32 buffers).  norm_type
+    2 or inf.  Squares are summed in fp64.  A norm that is not finite makes the factor what torch.nn.utils.clip_grad_norm_ makes it
+    (NaN, or 0 for an infinite one); error_if_nonfinite looks at the norm on the host first and raises, with nothing changed.
+    max_norm = inf: the norm alone.  Two tensors that share memory are refused."""
+    grads = list(grads)
+    inf_norm = float(norm_type) == float("inf")
+    if not inf_norm and float(norm_type) != 2.0:
+        raise ops._C.LsamError(f"clip_grads_: norm_type {norm_type}; 2 and inf are built")
+    max_norm, grad_scale = float(max_norm), float(grad_scale)
+    if not max_norm >= 0.0 or grad_scale != grad_scale:
+        raise ValueError(f"clip_grads_: max_norm {max_norm}, grad_scale {grad_scale}")
+    if not grads:
+        return torch.tensor(0.0)
+    into = grads if out is None else list(out)
+    if len(into) != len(grads) or any(a.shape != b.shape for a, b in (() if out is None else zip(into, grads))):
+        raise ops._C.LsamError("clip_grads_: out must hold one tensor of the same shape for each gradient")
+    if not all(map(torch.Tensor.is_contiguous, grads)):           # a gradient in another layout goes through a contiguous copy
+        src = [g.contiguous() for g in grads]
+        if out is None:
+            into = src
+    else:
+        src = grads
+    dst = into if into is src or all(map(torch.Tensor.is_contiguous, into)) else [t.contiguous() for t in into]
+    if error_if_nonfinite:
+        norm = ops.clip_grads(src, src, float("inf"), inf_norm)[0] * abs(grad_scale)
+        if not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so it cannot be clipped.")
+    norm = ops.clip_grads(src, dst, max_norm, inf_norm, grad_scale)[0]
+    target = grads if out is None else into
+    if dst is not target:
+        for t, d in zip(target, dst):
+            if t is not d:
+                t.copy_(d)
+    return norm
+
+
+def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """torch.nn.utils.clip_grad_norm_ on liblsam: clips the gradients of `parameters` in place by their global norm and returns it.
+    A parameter that is listed twice counts once."""
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(dict.fromkeys(parameters))
+    return clip_grads_([p.grad for p in params if p.grad is not None], max_norm, norm_type, error_if_nonfinite=error_if_nonfinite)
 
 
 class _Bucket:
@@ -122,10 +174,12 @@ class LoRAGradReducer:
         b.work = self._all_reduce(b.flat, True)
 
     @torch.no_grad()
-    def reduce(self):
-        """grads <- mean over ranks.  Missing grads count as zero (DDP semantics)."""
+    def reduce(self, max_norm: Optional[float] = None):
+        """grads <- mean over ranks.  Missing grads count as zero (DDP semantics).  With `max_norm` the mean is clipped to that global
+        norm as it is written (one pass with the division by the ranks: clip_grads_), and the norm before clipping is returned; every
+        rank clips the same sums, so the ranks stay alike without another exchange."""
         if not self.active():
-            return
+            return None if max_norm is None else clip_grad_norm_(self.params, max_norm)
         ws = self.world_size()
         for b in reversed(self.buckets):   # the order the backward produced (and launched) them
             if not b.filled:
@@ -139,6 +193,11 @@ class LoRAGradReducer:
                 b.flat.add_(inc)
             b.pending = []
             b.work, b.filled = None, False
+        if max_norm is not None:
+            for p in self.params:
+                if p.grad is None:
+                    p.grad = torch.empty_like(p)
+            return clip_grads_(self.views, max_norm, out=[p.grad for p in self.params], grad_scale=1.0 / ws)
         if ws > 1:
             self.flat.mul_(1.0 / ws)
         for p, v in zip(self.params, self.views):

@@ -262,3 +262,24 @@ class LinearCrossEntropyFn(torch.autograd.Function):
         M, label_smoothing, reduction = ctx.cfg
         dx, dw, db = ops.linear_ce_bwd(g, state, weight, bias, M, label_smoothing, reduction, ctx.needs_input_grad[:3])
         return dx, dw, db if db is None else db.to(bias.dtype), None, None, None, None
+
+
+class GroupNormActFn(torch.autograd.Function):
+    """act(group_norm(x)) of a channels-last T map, affine parameters trainable or not (norms.group_norm_act)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act):
+        ctx.act = act
+        if not any(ctx.needs_input_grad):
+            return ops.group_norm_act_fwd(x, groups, weight, bias, eps, act)
+        y, stats = ops.group_norm_act_fwd(x, groups, weight, bias, eps, act, want_stats=True)
+        ctx.save_for_backward(x, stats, weight, bias)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, stats, weight, bias = ctx.saved_tensors
+        dx, dw, db = ops.group_norm_act_bwd(g, x, stats, weight, bias, ctx.act)
+        need = ctx.needs_input_grad
+        return (dx if need[0] else None, dw.to(weight.dtype) if need[1] else None, db.to(bias.dtype) if need[2] else None, None, None, None)

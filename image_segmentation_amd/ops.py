@@ -6,7 +6,9 @@ go through here: `Hiera.forward` makes a single `lsam_hiera_forward` call.
 Everything requires CUDA(HIP) tensors; nothing here computes in PyTorch."""
 from __future__ import annotations
 
-from typing import Optional, Tuple
+import math
+from array import array
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -829,3 +831,114 @@ def linear_ce_bwd(gout: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
         check(L.lsam_linear_ce_bwd(code, ptr(weight), _ld(weight), ptr(b), ptr(gout), M, D, V, label_smoothing, REDUCTIONS[reduction],
                                    ptr(state), ptr(dx), D, ptr(dw), D, ptr(db), ptr(ws), ws.numel(), stream()))
     return dx, dw, db
+
+
+# ---- group norm with an activation, channels last (csrc/group_norm.hip) ----------------------------------------------------
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+def channels_last_rows(x: torch.Tensor) -> Optional[Tuple[int, int, int, int]]:
+    """(samples, pixels, sample stride, pixel stride) of [N, C, *spatial] whose channels are contiguous and whose pixels lie one
+    stride apart in row-major order (channels-last, also as a channel slice of a wider map); None if it is laid out otherwise."""
+    N, Cc = x.shape[:2]
+    if x.numel() == 0:                                         # nothing to lie anywhere
+        return N, math.prod(x.shape[2:]), 0, Cc
+    if Cc > 1 and x.stride(1) != 1:
+        return None
+    P, px = 1, None
+    for n, st in zip(reversed(x.shape[2:]), reversed(x.stride()[2:])):
+        if n == 1:
+            continue
+        if px is None:
+            px = st
+        elif st != px * P:
+            return None
+        P *= n
+    px = Cc if px is None else px
+    sx = x.stride(0) if N > 1 else P * px
+    return (N, P, sx, px) if (px >= Cc or P == 1) and (sx >= Cc or N == 1) else None
+
+
+def _channels_last_like(x: torch.Tensor) -> torch.Tensor:
+    """Empty tensor of x's shape and type, channels last without gaps."""
+    N, Cc = x.shape[:2]
+    return torch.empty((N, *x.shape[2:], Cc), dtype=x.dtype, device=x.device).movedim(-1, 1)
+
+
+def group_norm_act_fwd(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float = 1e-5,
+                       act: str = "none", want_stats: bool = False):
+    """act(group_norm(x)) for T [N, C, *spatial] laid out channels last, same type and layout; with want_stats also fp32
+    [N, groups, 2] (mean, 1 / std) for group_norm_act_bwd."""
+    with _same_device(x, weight, bias):
+        code = dtype_code(x.dtype)
+        x = x.detach()
+        lay = channels_last_rows(x)
+        if lay is None:
+            raise _C.LsamError(f"group_norm_act: shape {tuple(x.shape)} with strides {x.stride()} is not channels last "
+                               "(x.contiguous(memory_format=torch.channels_last))")
+        N, P, sx, px = lay
+        Cc, w, b = x.shape[1], _f32c(weight), _f32c(bias)
+        y = _channels_last_like(x)
+        stats = torch.empty(N, groups, 2, dtype=torch.float32, device=x.device) if want_stats else None
+        L = lib()
+        ws = torch.empty(L.lsam_group_norm_act_ws_bytes(N, P, Cc, groups, 0), dtype=torch.uint8, device=x.device)
+        check(L.lsam_group_norm_act_fwd(code, ptr(x), sx, px, ptr(w), ptr(b), N, P, Cc, groups, eps, ACTIVATIONS[act], ptr(y), ptr(stats),
+                                        ptr(ws), ws.numel(), stream()))
+    return (y, stats) if want_stats else y
+
+
+def group_norm_act_bwd(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
+                       act: str = "none"):
+    """(dx T channels last, dweight fp32, dbias fp32) of group_norm_act_fwd; dy of any layout (copied to channels last if it is not)."""
+    with _same_device(dy, x, stats, weight, bias):
+        x, dy = x.detach(), dy.detach().to(x.dtype)
+        lay_y = channels_last_rows(dy)
+        if lay_y is None:
+            dy = _channels_last_like(x).copy_(dy)
+            lay_y = channels_last_rows(dy)
+        N, P, sx, px = channels_last_rows(x)
+        Cc, G, w, b = x.shape[1], stats.shape[1], _f32c(weight), _f32c(bias)
+        dx = _channels_last_like(x)
+        dw, db = torch.empty(2, Cc, dtype=torch.float32, device=x.device)
+        L = lib()
+        ws = torch.empty(L.lsam_group_norm_act_ws_bytes(N, P, Cc, G, 1), dtype=torch.uint8, device=x.device)
+        check(L.lsam_group_norm_act_bwd(dtype_code(x.dtype), ptr(dy), lay_y[2], lay_y[3], ptr(x), sx, px, ptr(w), ptr(b), ptr(stats), N, P, Cc,
+                                        G, ACTIVATIONS[act], ptr(dx), ptr(dw), ptr(db), ptr(ws), ws.numel(), stream()))
+    return dx, dw, db
+
+
+# ---- global norm of a list of tensors, clipping (csrc/grad_clip.hip) ---------------------------------------------------------
+_PTR, _NUMEL, _DEV, _CONTIG = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous
+_KIND = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def clip_grads(src: Sequence[torch.Tensor], dst: Sequence[torch.Tensor], max_norm: float, inf_norm: bool = False, scale: float = 1.0):
+    """fp32 [2] (norm, factor): the global norm of `scale * src` and dst_i = factor * src_i with factor = scale * min(1, max_norm /
+    (norm + 1e-6)); contiguous fp32 / bf16 tensors on one GPU, dst may be src.  One pass over the list costs a few attribute reads a
+    tensor on the host, no device memory but the chunk sums."""
+    if not src:
+        raise _C.LsamError("clip_grads: no tensors")
+    devs = set(map(_DEV, src)) | set(map(_DEV, dst))
+    if len(devs) != 1 or -1 in devs:
+        raise _C.LsamError("clip_grads: the tensors must be on one MI355X (there is no CPU fallback)")
+    place = dst is src
+    n = array("q", map(_NUMEL, src))
+    try:
+        ks = bytes([_KIND[t.dtype] for t in src])
+        kinds = bytes([3 * k for k in ks]) if place else bytes([a + 2 * _KIND[b.dtype] for a, b in zip(ks, dst)])
+    except KeyError as e:
+        raise _C.LsamError(f"clip_grads: unsupported type {e.args[0]}; float32 and bfloat16 are") from None
+    if not (all(map(_CONTIG, src)) and (place or all(map(_CONTIG, dst)))):
+        raise _C.LsamError("clip_grads: the tensors must be contiguous")
+    if not place and (len(dst) != len(src) or array("q", map(_NUMEL, dst)) != n):
+        raise _C.LsamError("clip_grads: src and dst differ in number or size")
+    with torch.cuda.device(src[0].device):
+        sp = array("Q", map(_PTR, src))
+        dp = sp if place else array("Q", map(_PTR, dst))
+        L, na = lib(), n.buffer_info()[0]
+        out = torch.empty(2, dtype=torch.float32, device=src[0].device)
+        ws = torch.empty(L.lsam_clip_grads_ws_bytes(na, len(src)) // 8, dtype=torch.float64, device=src[0].device)
+        check(L.lsam_clip_grads(sp.buffer_info()[0], dp.buffer_info()[0], na, kinds, len(src), max_norm, int(inf_norm), scale, ptr(out), ptr(ws),
+                                ws.numel() * 8, stream()))
+    torch.autograd.graph.increment_version(dst)
+    return out

@@ -509,6 +509,30 @@ int lsam_linear_ce_bwd(int dtype, const void* w, long ldw, const float* bias, co
                        int reduction, const void* state, void* dx, long lddx, void* dw, long lddw, float* db, void* ws, size_t ws_bytes,
                        lsam_stream_t stream);
 
+/* ---- group norm with an activation, channels last ------------------------------------------------------------------------------
+ * x T [N] samples of P pixels of C channels: sample stride sx, pixel stride px (elements), channels contiguous; groups of C / G
+ * neighbouring channels.  y = act((x - mean) rstd gamma + beta), T, contiguous [N][P][C]; gamma / beta fp32 [C] or NULL (1, 0).
+ * stats fp32 [N][G][2] (mean, rstd) is what the backward needs, NULL where it is not wanted.  C <= 8192. */
+enum { LSAM_ACT_NONE = 0, LSAM_ACT_RELU = 1, LSAM_ACT_SILU = 2, LSAM_ACT_GELU = 3 };
+size_t lsam_group_norm_act_ws_bytes(int N, int P, int C, int G, int backward);
+int lsam_group_norm_act_fwd(int dtype, const void* x, long sx, long px, const float* gamma, const float* beta, int N, int P, int C, int G,
+                            float eps, int act, void* y, float* stats, void* ws, size_t ws_bytes, lsam_stream_t stream);
+/* dx T contiguous [N][P][C]; dgamma / dbeta fp32 [C], NULL where not wanted; overwritten. */
+int lsam_group_norm_act_bwd(int dtype, const void* dy, long sy, long py, const void* x, long sx, long px, const float* gamma,
+                            const float* beta, const float* stats, int N, int P, int C, int G, int act, void* dx, float* dgamma,
+                            float* dbeta, void* ws, size_t ws_bytes, lsam_stream_t stream);
+
+/* ---- global norm of a list of tensors, and clipping by it ------------------------------------------------------------------------
+ * total = |scale| * (sum g^2)^(1/2) over all tensors, or |scale| * max |g| with inf != 0;  c = min(1, max_norm / (total + 1e-6));
+ * dst = c * scale * src, each tensor contiguous; dst may be src.  out fp32 [2] (device) = total, c * scale.  With max_norm = INFINITY,
+ * scale = 1 and every dst = src nothing is written but `out`.
+ * host_*: host arrays of `count` entries: device addresses, element counts, and kinds (bit 0: src is bf16, bit 1: dst is bf16; else
+ * fp32); read before the call returns.  Tensors whose memory overlaps are refused where anything would be written. */
+size_t lsam_clip_grads_ws_bytes(const long long* host_n, int count);
+int lsam_clip_grads(const unsigned long long* host_src, const unsigned long long* host_dst, const long long* host_n,
+                    const unsigned char* host_kind, int count, double max_norm, int inf, double scale, float* out, void* ws,
+                    size_t ws_bytes, lsam_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,12 +20,12 @@ constexpr int ROW_BAD = -1;   // target outside [0, V): the row's loss and gradi
 // The product: Out[j][i] = sum_k A(i, k) B(j, k), i contiguous in Out.  An operand is stored "KC" ([i][k], k contiguous) or
 // transposed ([k][i]).  Tile IT x JT, k-tiles of 128 bytes, two LDS stages filled by LDS-DMA.
 // ---------------------------------------------------------------------------------------------------------------------
-enum Mode { STATS, DZ, ACC, OUT };
+enum Mode { STATS, DZ, ACC, OUT, PART };   // PART: OUT in fp32
 
 struct CeArgs {
     const void* A; long lda;   // elements
     const void* B; long ldb;
-    int I, J, K;               // limits; J (STATS, DZ, ACC) or K (OUT) is further limited by *n
+    int I, J, K;               // limits; J (STATS, DZ, ACC) or K (OUT, PART) is further limited by *n
     const int* n;              // number of rows that count (device)
     // STATS / DZ
     const float* bias;         // [I] or null
@@ -42,10 +42,9 @@ struct CeArgs {
     long dbp_ld;
     int rows_cap;
     // outputs
-    void* out; long ldo;       // DZ: T; ACC: fp32; OUT: T, or fp32 partials when splits > 1
+    void* out; long ldo;       // DZ, OUT: T; ACC, PART: fp32
     long split_stride;         // elements between the splits' outputs
     int splits, accumulate;
-    int cols, vec;             // OUT: columns to write; whether 4 at a time may be stored at once
 };
 
 template <typename T> struct Ce;
@@ -64,28 +63,29 @@ template <> struct Ce<float> {
 
 // One operand's tile in LDS.  KC: R rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7).  Transposed: 128 / sizeof(T) rows of
 // R * sizeof(T) bytes; bf16 is read with the transposing LDS load (16 lanes take 4 k-rows x 16 columns), whose 8 rows of a half
-// wave must fall on different banks: 32-byte column pairs p of row k at p ^ h(k); fp32 is read one dword a lane, 64-byte column
-// groups at group ^ ((k >> 2) & 3).
+// wave must fall on different banks: 32-byte column pair p of row k at p ^ h(k), h = k's bits 0, 1, 3; fp32 is read one dword a lane,
+// 64-byte column group at group ^ bit 2 of k.
+// DMA instruction q (of NI a wave) fills 1 KB; from one q to the next a lane's source moves by a fixed number of rows, and its chunk
+// within the row stays, so one offset and one first k describe them all.  Rows of a KC tile behind the limit lie behind the
+// descriptor's last byte and read zeros; every other chunk that must not be read gets an offset that does.
 template <typename T, bool KC, int R, int NW> struct Tile {
     static constexpr int ES = sizeof(T), EPC = 16 / ES, KE = 128 / ES, RB = R * ES;
-    static constexpr int NI = R * 128 / 1024 / NW;   // DMA instructions a wave and stage
-    static_assert(R * 128 % (1024 * NW) == 0, "whole DMA instructions");
-    unsigned vo[NI];   // byte offsets of this lane's chunks in the k-tile's slab; 0xFFFFFFFF reads zeros
-    short ke[NI];      // first k of the chunk
+    static constexpr int NI = R * 128 / 1024 / NW;          // DMA instructions a wave and stage
+    static constexpr int ROWS = KC ? NW * 8 : NW * 1024 / RB;   // rows from one of them to the next
+    static_assert(R * 128 % (1024 * NW) == 0 && (KC || (NW * 1024 % RB == 0 && ROWS % (ES == 2 ? 16 : 8) == 0)), "a lane's chunk stays");
+    unsigned vo;   // byte offset of this lane's first chunk in the k-tile's slab
+    int ke;        // its first k; past every k-tile where the column does not exist
     __device__ __forceinline__ void init(int wave, int lane, long ld, int r0, int lim) {
-#pragma unroll
-        for (int q = 0; q < NI; ++q) {
-            const int b = (wave + NW * q) * 1024 + lane * 16;
-            if constexpr (KC) {
-                const int row = b >> 7, c = ((b >> 4) & 7) ^ (row & 7);
-                vo[q] = r0 + row < lim ? (unsigned)((long)row * ld * ES + c * 16) : 0xFFFFFFFFu;
-                ke[q] = (short)(c * EPC);
-            } else {
-                const int k = b / RB, pos = (b % RB) >> 4;
-                const int c = ES == 2 ? pos ^ (2 * ((k & 3) | (((k >> 3) & 1) << 2))) : pos ^ (4 * ((k >> 2) & 3));
-                vo[q] = r0 + c * EPC < lim ? (unsigned)((long)k * ld * ES + c * 16) : 0xFFFFFFFFu;
-                ke[q] = (short)k;
-            }
+        const int b = wave * 1024 + lane * 16;
+        if constexpr (KC) {
+            const int row = b >> 7, c = ((b >> 4) & 7) ^ (row & 7);
+            vo = (unsigned)((long)row * ld * ES + c * 16);
+            ke = c * EPC;
+        } else {
+            const int k = b / RB, pos = (b % RB) >> 4;
+            const int c = ES == 2 ? pos ^ (2 * ((k & 3) | (((k >> 3) & 1) << 2))) : pos ^ (4 * ((k >> 2) & 1));
+            vo = (unsigned)((long)k * ld * ES + c * 16);
+            ke = r0 + c * EPC < lim ? k : 1 << 20;
         }
     }
     // k-tile slab: KC advances 128 bytes along the rows, transposed KE rows
@@ -93,45 +93,29 @@ template <typename T, bool KC, int R, int NW> struct Tile {
         const char* p = static_cast<const char*>(base);
         return KC ? p + ((long)r0 * ld + k0) * ES : p + (k0 * ld + r0) * ES;
     }
-    __device__ __forceinline__ void issue(const char* slab_p, char* dst, int wave, int left) const {
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(slab_p), 0, 0x7FFFFFFF, 0x00020000);
-        if (left >= KE) {
-#pragma unroll
-            for (int q = 0; q < NI; ++q)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_p)(dst + (wave + NW * q) * 1024), 16, vo[q], 0, 0, 0);
-        } else {
-#pragma unroll
-            for (int q = 0; q < NI; ++q)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_p)(dst + (wave + NW * q) * 1024), 16,
-                                                         ke[q] < left ? vo[q] : 0xFFFFFFFFu, 0, 0, 0);
-        }
+    // DMA instruction q of a k-tile of which `left` k-columns exist
+    __device__ __forceinline__ void issue(const char* slab_p, char* dst, int wave, int left, int q, long ld, int rows) const {
+        const int bytes = KC ? rows * (int)ld * ES : 0x7FFFFFFF;
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(slab_p), 0, bytes, 0x00020000);
+        const bool ok = ke < left - (KC ? 0 : q * ROWS);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_p)(dst + (wave + NW * q) * 1024), 16,
+                                                 ok ? vo + (unsigned)(q * ROWS * ES) * (unsigned)ld : 0xFFFFFFFFu, 0, 0, 0);
     }
-    // fragments of NT 16-wide tiles starting at tile t0, k-step ks (0, 1)
-    template <int NT> static __device__ __forceinline__ void read(const char* s, int t0, int ks, int g, int lr, uint4 (&f)[NT]) {
-        if constexpr (KC) {
-            const char* p = s + (t0 * 16 + lr) * 128 + (((ks * 4 + g) ^ (lr & 7)) << 4);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) f[t] = *reinterpret_cast<const uint4*>(p + t * 2048);
-        } else if constexpr (ES == 2) {
+    // the fragment of 16-wide tile t, k-step ks (0, 1): lane (g, lr) holds column 16 t + lr, its share of the step's k
+    static __device__ __forceinline__ uint4 read(const char* s, int t, int ks, int g, int lr) {
+        if constexpr (KC) return *reinterpret_cast<const uint4*>(s + (t * 16 + lr) * 128 + (((ks * 4 + g) ^ (lr & 7)) << 4));
+        else if constexpr (ES == 2) {
             using s4 = __attribute__((ext_vector_type(4))) short;
             using s4p = __attribute__((address_space(3))) s4*;
             const int h = (lr >> 2) | ((g & 1) << 2);
-            const char* p = s + (ks * 32 + 8 * g + (lr >> 2)) * RB + (lr & 3) * 8;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const char* a = p + (((t0 + t) ^ h) << 5);
-                const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)a), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)(a + 4 * RB));
-                const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, hi);
-                f[t] = make_uint4(x.x, x.y, y.x, y.y);
-            }
+            const char* a = s + (ks * 32 + 8 * g + (lr >> 2)) * RB + (lr & 3) * 8 + ((t ^ h) << 5);
+            const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)a), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)(a + 4 * RB));
+            const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, hi);
+            return make_uint4(x.x, x.y, y.x, y.y);
         } else {
-            const char* p = s + (ks * 16 + 4 * g) * RB + lr * 4;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const char* a = p + (((t0 + t) ^ g) << 6);
-                f[t] = make_uint4(*reinterpret_cast<const unsigned*>(a), *reinterpret_cast<const unsigned*>(a + RB),
-                                  *reinterpret_cast<const unsigned*>(a + 2 * RB), *reinterpret_cast<const unsigned*>(a + 3 * RB));
-            }
+            const char* a = s + (ks * 16 + 4 * g) * RB + lr * 4 + ((t ^ (g & 1)) << 6);
+            return make_uint4(*reinterpret_cast<const unsigned*>(a), *reinterpret_cast<const unsigned*>(a + RB),
+                              *reinterpret_cast<const unsigned*>(a + 2 * RB), *reinterpret_cast<const unsigned*>(a + 3 * RB));
         }
     }
 };
@@ -149,15 +133,20 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void ce_gemm_kernel(const CeArgs
 #if defined(__HIP_DEVICE_COMPILE__)   // the host pass needs the launch stub only, and cannot form the LDS builtins
     constexpr int NW = WI * WJ, IT = WI * TI * 16, JT = WJ * TJ * 16;
     constexpr int KE = 128 / (int)sizeof(T);
+    constexpr bool OPQ = !AKC && !BKC;
     using TA = Tile<T, AKC, IT, NW>;
     using TB = Tile<T, BKC, JT, NW>;
-    __shared__ __attribute__((aligned(1024))) char st0[(IT + JT) * 128];
-    __shared__ __attribute__((aligned(1024))) char st1[(IT + JT) * 128];
+    // two stages of either operand, each a variable of its own: what the compiler can tell apart it does not make a read wait for
+    __shared__ __attribute__((aligned(1024))) char sa0[IT * 128];
+    __shared__ __attribute__((aligned(1024))) char sa1[IT * 128];
+    __shared__ __attribute__((aligned(1024))) char sb0[JT * 128];
+    __shared__ __attribute__((aligned(1024))) char sb1[JT * 128];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wi = wave % WI, wj = wave / WI, g = lane >> 4, lr = lane & 15;
-    const int n = *p.n;
-    const int J = MODE == OUT ? p.J : min(p.J, n), K = MODE == OUT ? min(p.K, n) : p.K;
+    const int n = __builtin_amdgcn_readfirstlane(*p.n);   // in a scalar register, like all that the tile loop counts by
+    constexpr bool ROWS_K = MODE == OUT || MODE == PART;
+    const int J = ROWS_K ? p.J : min(p.J, n), K = ROWS_K ? min(p.K, n) : p.K;
 
     // tile order: runs of 8 j-tiles against one i-tile, so the workgroups that an XCD holds at a time share operands in its L2
     const int tiles_i = (p.I + IT - 1) / IT, tiles_j = (p.J + JT - 1) / JT;
@@ -184,49 +173,70 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void ce_gemm_kernel(const CeArgs
         TB tb;
         ta.init(wave, lane, p.lda, i0, p.I);
         tb.init(wave, lane, p.ldb, j0, J);
-        auto issue = [&](int kt, char* s) {
-            const int left = K - kt * KE;
-            ta.issue(TA::slab(p.A, p.lda, i0, (long)kt * KE), s, wave, left);
-            tb.issue(TB::slab(p.B, p.ldb, j0, (long)kt * KE), s + IT * 128, wave, left);
+        constexpr int NP = TA::NI + TB::NI;
+        auto issue = [&](int kt, char* sa, char* sb, int q) {   // DMA instruction q; a k-tile behind the last fetches nothing
+            const int left = kt < kt1 ? K - kt * KE : 0;
+            if (q < TA::NI) ta.issue(TA::slab(p.A, p.lda, i0, (long)kt * KE), sa, wave, left, q, p.lda, min(IT, p.I - i0));
+            else tb.issue(TB::slab(p.B, p.ldb, j0, (long)kt * KE), sb, wave, left, q - TA::NI, p.ldb, min(JT, J - j0));
         };
-        auto mma = [&](const uint4 (&a)[TI], const uint4 (&b)[TJ]) {
+        int lr_k = lr, g_k = g;
+        auto rd_a = [&](const char* s, int x, int ks) { return TA::read(s, wi * TI + x, ks, g_k, lr_k); };
+        auto rd_b = [&](const char* s, int y, int ks) { return TB::read(s, wj * TJ + y, ks, g_k, lr_k); };
+        // A k-step is TI rows of TJ MFMAs.  Behind row x its A fragment is replaced by the next step's (needed TI rows later), the next
+        // step's B fragments arrive in a second set during the first rows.  In the second step of a k-tile, behind row 0 -- by then every
+        // read of this tile has landed -- the workgroup meets: the other stage is complete, this one is free for the tile after next,
+        // whose DMA instructions go out between the rows.
+        uint4 a[TI], b0[TJ], b1[TJ];
+        auto step = [&](const char* na, const char* nb, int ks, uint4 (&bc)[TJ], uint4 (&bn)[TJ], bool meet, int kt, char* fa, char* fb) {
+            // two transposed operands: their addresses are worked out here; held across the loop they spill (4096^3: 816 against 1100 TF/s)
+            if (OPQ) asm volatile("" : "+v"(lr_k), "+v"(g_k));
 #pragma unroll
-            for (int x = 0; x < TI; ++x)
+            for (int x = 0; x < TI; ++x) {
 #pragma unroll
-                for (int y = 0; y < TJ; ++y) Ce<T>::mma(a[x], b[y], acc[x][y]);
-        };
-        uint4 a0[TI], b0[TJ], a1[TI], b1[TJ];
-        auto read = [&](const char* s, int ks, uint4 (&a)[TI], uint4 (&b)[TJ]) {
-            TA::template read<TI>(s, wi * TI, ks, g, lr, a);
-            TB::template read<TJ>(s + IT * 128, wj * TJ, ks, g, lr, b);
-        };
-        // k-tile q:  read ks1(q) | MFMA ks0(q) | own DMA(q+1) landed, own reads of q done, barrier | read ks0(q+1), issue DMA(q+2) | MFMA ks1(q)
-        auto step = [&](int kt, char* cur, char* nxt) {
-            read(cur, 1, a1, b1);
-            mma(a0, b0);
-            if (kt + 1 < kt1) {
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
-                read(nxt, 0, a0, b0);
-                if (kt + 2 < kt1) issue(kt + 2, cur);
+                for (int y = 0; y < TJ; ++y) Ce<T>::mma(a[x], bc[y], acc[x][y]);
+                if (meet && x == 0) {
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
+                }
+                a[x] = rd_a(na, x, ks);
+#pragma unroll
+                for (int y = 0; y < TJ; ++y)
+                    if (y / 2 == x) bn[y] = rd_b(nb, y, ks);
+                if (meet) {
+#pragma unroll
+                    for (int q = 0; q < NP; ++q)
+                        if (q * TI / NP == x) issue(kt, fa, fb, q);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            mma(a1, b1);
         };
-        issue(kt0, st0);
-        if (kt0 + 1 < kt1) issue(kt0 + 1, st1);
+#pragma unroll
+        for (int q = 0; q < NP; ++q) issue(kt0, sa0, sb0, q);
+#pragma unroll
+        for (int q = 0; q < NP; ++q) issue(kt0 + 1, sa1, sb1, q);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        read(st0, 0, a0, b0);
+#pragma unroll
+        for (int x = 0; x < TI; ++x) a[x] = rd_a(sa0, x, 0);
+#pragma unroll
+        for (int y = 0; y < TJ; ++y) b0[y] = rd_b(sb0, y, 0);
         for (int kt = kt0; kt < kt1; kt += 2) {
-            step(kt, st0, st1);
-            if (kt + 1 < kt1) step(kt + 1, st1, st0);
+            step(sa0, sb0, 1, b0, b1, false, 0, nullptr, nullptr);
+            step(sa1, sb1, 0, b1, b0, true, kt + 2, sa0, sb0);
+            if (kt + 1 >= kt1) break;
+            step(sa1, sb1, 1, b0, b1, false, 0, nullptr, nullptr);
+            step(sa0, sb0, 0, b1, b0, true, kt + 3, sa1, sb1);
         }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing may land in this workgroup's LDS after it
     }
 
+    // opaque copies: nothing of an epilogue's addresses is worked out ahead of the k-loop, where every register is taken
+    int lr_e = lr, g_e = g;
+    asm volatile("" : "+v"(lr_e), "+v"(g_e));
     // ---- epilogues: lane (g, lr), tile (x, y), register r holds Out[j = j0 + (wj TJ + y) 16 + lr][i = i0 + (wi TI + x) 16 + 4 g + r]
-    const int ib = i0 + wi * TI * 16 + 4 * g, jb = j0 + wj * TJ * 16 + lr;
+    const int ib = i0 + wi * TI * 16 + 4 * g_e, jb = j0 + wj * TJ * 16 + lr_e;
     if constexpr (MODE == STATS || MODE == DZ) {
         __shared__ float red[(MODE == STATS ? WI * 3 * JT : WJ * IT)];
 #pragma unroll
@@ -274,8 +284,8 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void ce_gemm_kernel(const CeArgs
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[x][y][r], LOG2E, -sub));
                 s = group4_sum(s);
-                if (g == 0) {
-                    const int c = (wj * TJ + y) * 16 + lr;
+                if (g_e == 0) {
+                    const int c = (wj * TJ + y) * 16 + lr_e;
                     red[(wi * 3 + 0) * JT + c] = base;
                     red[(wi * 3 + 1) * JT + c] = s;
                     red[(wi * 3 + 2) * JT + c] = zs;
@@ -319,11 +329,11 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void ce_gemm_kernel(const CeArgs
                     }
                 if constexpr (sizeof(T) == 2) {
 #pragma unroll
-                    for (int x = 0; x < TI; x += 2) store_bf16_tile_pair(rowp + 16 * x, g, acc[x][y], acc[x + 1][y], ok);
+                    for (int x = 0; x < TI; x += 2) store_bf16_tile_pair(rowp + 16 * x, g_e, acc[x][y], acc[x + 1][y], ok);
                 } else {
                     if (ok) {
 #pragma unroll
-                        for (int x = 0; x < TI; ++x) store4(rowp + 16 * x + 4 * g, acc[x][y]);
+                        for (int x = 0; x < TI; ++x) store4(rowp + 16 * x + 4 * g_e, acc[x][y]);
                     }
                 }
             }
@@ -336,7 +346,7 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void ce_gemm_kernel(const CeArgs
 #pragma unroll
                         for (int y = 0; y < TJ; ++y) s += acc[x][y][r];
                         s = row16_sum(s);
-                        if (lr == 0) red[wj * IT + (wi * TI + x) * 16 + 4 * g + r] = s;
+                        if (lr_e == 0) red[wj * IT + (wi * TI + x) * 16 + 4 * g_e + r] = s;
                     }
                 __syncthreads();
                 for (int c = tid; c < IT; c += 64 * NW) {
@@ -348,28 +358,24 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void ce_gemm_kernel(const CeArgs
             }
         }
     } else {
-        const bool f32out = MODE == ACC || p.splits > 1;
 #pragma unroll
         for (int y = 0; y < TJ; ++y) {
             const int j = jb + 16 * y;
-            if (j >= J) continue;
+            if constexpr (MODE == OUT && sizeof(T) == 2) {   // every lane takes part in the exchange of a tile pair
+                T* rowp = static_cast<T*>(p.out) + (size_t)min(j, J - 1) * p.ldo + i0 + wi * TI * 16;
 #pragma unroll
-            for (int x = 0; x < TI; ++x) {
-                const int i = ib + 16 * x;
-                if (i >= (f32out ? p.I : p.cols)) continue;
-                if (f32out) {   // workspace: I padded to whole chunks, rows 16-byte aligned
+                for (int x = 0; x < TI; x += 2)
+                    store_bf16_tile_pair(rowp + 16 * x, g_e, acc[x][y], acc[x + 1][y], j < J && i0 + (wi * TI + x) * 16 + 8 * g_e < p.I);
+            } else {
+                if (j >= J) continue;
+#pragma unroll
+                for (int x = 0; x < TI; ++x) {
+                    const int i = ib + 16 * x;
+                    if (i >= p.I) continue;
                     float* o = static_cast<float*>(p.out) + split * p.split_stride + (size_t)j * p.ldo + i;
                     f32x4 v = acc[x][y];
                     if (MODE == ACC && p.accumulate) v += load4(o);
                     store4(o, v);
-                } else {
-                    T* o = static_cast<T*>(p.out) + (size_t)j * p.ldo + i;
-                    if (p.vec) store4(o, acc[x][y]);
-                    else {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (i + r < p.cols) o[r] = from_f<T>(acc[x][y][r]);
-                    }
                 }
             }
         }
@@ -593,6 +599,7 @@ template <typename T> struct CePlan {
         const size_t col = (size_t)M * sizeof(T) * TILE;
         size_t pt = DZ_CAP / (col ? col : 1);
         if (pt < 1) pt = 1;
+        if (pt > 1024) pt = 1024;   // byte offsets within a tile's rows stay within 31 bits
         if (pt > (size_t)tiles_v) pt = tiles_v;
         pieces = cdiv(tiles_v, (int)pt);
         piece = cdiv(tiles_v, pieces) * TILE;
@@ -604,8 +611,10 @@ template <typename T> struct CePlan {
             return s < most ? (s > 0 ? s : 1) : most;
         };
         s_dx = splits(tiles_m * tiles_d, cdiv(piece, kt));
-        s_dw = splits(piece / TILE * tiles_d, cdiv(M, kt));
+        s_dw = splits(piece / TILE * tiles_d, cdiv(M > 0 ? M : 1, kt));
     }
+    // partial sums, or rows of dW that do not take four columns at a time: through fp32 and the joining kernel
+    bool dw_f32() const { return s_dw > 1 || D % EPC; }
     size_t state(char* base, CeState* st) const {
         Carve c{base};
         CeState s;
@@ -639,7 +648,7 @@ template <typename T> struct CePlan {
         w.coef = c.take<float>(M);
         w.coef_s = c.take<float>(M);
         w.dx = c.take<float>(want_dx ? (size_t)s_dx * M * Dp : 0);
-        w.dw = c.take<float>(want_dw && s_dw > 1 ? (size_t)s_dw * piece * Dp : 0);
+        w.dw = c.take<float>(want_dw && dw_f32() ? (size_t)s_dw * piece * Dp : 0);
         w.dbp = c.take<float>(want_db ? (size_t)tiles_m * V : 0);
         if (f) *f = w;
         return c.used;
@@ -730,6 +739,8 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
     LSAM_REQUIRE(w && state && ws && (M == 0 || gout), LSAM_ERR_BAD_ARG, "linear_ce: null operand");
     LSAM_REQUIRE(ldw >= D && (!dx || lddx >= D) && (!dw || lddw >= D) && aligned16(state) && aligned16(ws), LSAM_ERR_BAD_ARG,
                  "linear_ce: a row stride below %d columns, or a workspace off its 16-byte alignment", D);
+    LSAM_REQUIRE((!dx || (aligned16(dx) && (lddx % 8 == 0 || D % 8))) && (!dw || (aligned16(dw) && (lddw % 8 == 0 || D % 8))), LSAM_ERR_BAD_ARG,
+                 "linear_ce: gradients off their 16-byte alignment");
     CeState st;
     typename CePlan<T>::Bwd b;
     pl.state(static_cast<char*>(const_cast<void*>(state)), &st);
@@ -761,21 +772,23 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
             a.B = b.dz; a.ldb = pl.piece;
             a.I = pl.Dp; a.J = M; a.K = nv; a.n = st.n;
             a.out = b.dx; a.ldo = pl.Dp; a.split_stride = (long)M * pl.Dp; a.splits = pl.s_dx; a.accumulate = k > 0;
-            LSAM_TRY((ce_gemm<T, false, true, ACC, 2, 2, 8, 8, 1>(a, s)));
+            LSAM_TRY((ce_gemm<T, false, true, ACC, 4, 2, 4, 8, 2>(a, s)));
         }
         if (dw) {
-            const bool vec = D % 4 == 0 && lddw % 4 == 0 && aligned16(dw);
             T* o = static_cast<T*>(dw) + (size_t)v0 * lddw;
             CeArgs a{};
             a.A = st.xc; a.lda = pl.Dp;
             a.B = b.dz; a.ldb = pl.piece;
-            a.I = pl.Dp; a.J = nv; a.K = M; a.n = st.n; a.cols = D; a.vec = vec; a.splits = pl.s_dw;
-            if (pl.s_dw > 1) { a.out = b.dw; a.ldo = pl.Dp; a.split_stride = (long)pl.piece * pl.Dp; }
-            else { a.out = o; a.ldo = lddw; }
-            LSAM_TRY((ce_gemm<T, false, false, OUT, 2, 2, 8, 8, 1>(a, s)));
-            if (pl.s_dw > 1) {
+            a.I = pl.Dp; a.J = nv; a.K = M; a.n = st.n; a.splits = pl.s_dw;
+            if (!pl.dw_f32()) {
+                a.out = o; a.ldo = lddw;
+                LSAM_TRY((ce_gemm<T, false, false, OUT, 2, 4, 8, 4, 2>(a, s)));
+            } else {
+                a.out = b.dw; a.ldo = pl.Dp; a.split_stride = (long)pl.piece * pl.Dp;
+                LSAM_TRY((ce_gemm<T, false, false, PART, 2, 4, 8, 4, 2>(a, s)));
                 const long blocks = ((long)nv * (pl.Dp / 4) + 255) / 256;
-                ce_dx_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(b.dw, a.split_stride, pl.s_dw, nullptr, nv, D, pl.Dp, vec, o, lddw);
+                ce_dx_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(b.dw, a.split_stride, pl.s_dw, nullptr, nv, D, pl.Dp,
+                                                                                     D % 4 == 0, o, lddw);
                 LSAM_LAUNCH_CHECK();
             }
         }
@@ -783,7 +796,7 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
     if (dx && M > 0) {
         const long blocks = ((long)M * (pl.Dp / 4) + 255) / 256;
         ce_dx_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(b.dx, (long)M * pl.Dp, pl.s_dx, st.pos, M, D, pl.Dp,
-                                                                             D % 4 == 0 && lddx % 4 == 0 && aligned16(dx), static_cast<T*>(dx), lddx);
+                                                                             D % 4 == 0, static_cast<T*>(dx), lddx);
         LSAM_LAUNCH_CHECK();
     }
     if (db) {

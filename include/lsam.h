@@ -504,7 +504,7 @@ int lsam_linear_ce_fwd(int dtype, const void* x, long ldx, const void* w, long l
                        int D, int V, long long ignore, float smooth, int reduction, float* loss, void* state, void* ws, size_t ws_bytes,
                        lsam_stream_t stream);
 /* gout fp32: [M] under NONE, one value otherwise.  dx T [M][lddx] (zeros in ignored rows), dw T [V][lddw], db fp32 [V], each written
- * whole; NULL where not wanted. */
+ * whole; NULL where not wanted; dx and dw 16-byte aligned, their row strides multiples of 8 where D is one. */
 int lsam_linear_ce_bwd(int dtype, const void* w, long ldw, const float* bias, const float* gout, int M, int D, int V, float smooth,
                        int reduction, const void* state, void* dx, long lddx, void* dw, long lddw, float* db, void* ws, size_t ws_bytes,
                        lsam_stream_t stream);

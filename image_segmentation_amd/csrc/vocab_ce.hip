@@ -37,7 +37,8 @@ struct CeArgs {
     const float* base2;        // DZ: the row's base, and its coefficient c and c / (sum of exponentials)
     const float* coef;
     const float* coef_s;
-    float sm, keep;            // DZ: e / V, 1 - e
+    float sm, keep;            // DZ: the subtrahends of every class and of the target, in units of the row's coefficient
+    const float* factor;       // OUT: what the product is multiplied with
     float* dbp;                // DZ: [tiles_j][I_cap] partial column sums or null
     long dbp_ld;
     int rows_cap;
@@ -74,18 +75,20 @@ template <typename T, bool KC, int R, int NW> struct Tile {
     static constexpr int ROWS = KC ? NW * 8 : NW * 1024 / RB;   // rows from one of them to the next
     static_assert(R * 128 % (1024 * NW) == 0 && (KC || (NW * 1024 % RB == 0 && ROWS % (ES == 2 ? 16 : 8) == 0)), "a lane's chunk stays");
     unsigned vo;   // byte offset of this lane's first chunk in the k-tile's slab
-    int ke;        // its first k; past every k-tile where the column does not exist
-    __device__ __forceinline__ void init(int wave, int lane, long ld, int r0, int lim) {
+    int ke, col;   // its first k; transposed: its first column in the tile
+    __device__ __forceinline__ void init(int wave, int lane, long ld) {
         const int b = wave * 1024 + lane * 16;
         if constexpr (KC) {
             const int row = b >> 7, c = ((b >> 4) & 7) ^ (row & 7);
             vo = (unsigned)((long)row * ld * ES + c * 16);
             ke = c * EPC;
+            col = 0;
         } else {
             const int k = b / RB, pos = (b % RB) >> 4;
             const int c = ES == 2 ? pos ^ (2 * ((k & 3) | (((k >> 3) & 1) << 2))) : pos ^ (4 * ((k >> 2) & 1));
             vo = (unsigned)((long)k * ld * ES + c * 16);
-            ke = r0 + c * EPC < lim ? k : 1 << 20;
+            ke = k;
+            col = c * EPC;
         }
     }
     // k-tile slab: KC advances 128 bytes along the rows, transposed KE rows
@@ -93,11 +96,14 @@ template <typename T, bool KC, int R, int NW> struct Tile {
         const char* p = static_cast<const char*>(base);
         return KC ? p + ((long)r0 * ld + k0) * ES : p + (k0 * ld + r0) * ES;
     }
-    // DMA instruction q of a k-tile of which `left` k-columns exist
+    static __device__ __forceinline__ long step(long ld) { return KC ? 128 : KE * ld * ES; }
+    // DMA instruction q of a k-tile of which `left` k and `rows` rows (columns, transposed) exist
     __device__ __forceinline__ void issue(const char* slab_p, char* dst, int wave, int left, int q, long ld, int rows) const {
         const int bytes = KC ? rows * (int)ld * ES : 0x7FFFFFFF;
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(slab_p), 0, bytes, 0x00020000);
-        const bool ok = ke < left - (KC ? 0 : q * ROWS);
+        unsigned vo = this->vo;
+        asm volatile("" : "+v"(vo));   // the NI offsets are not held across the loop
+        const bool ok = KC ? ke < left : ke < left - q * ROWS && col < rows;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_p)(dst + (wave + NW * q) * 1024), 16,
                                                  ok ? vo + (unsigned)(q * ROWS * ES) * (unsigned)ld : 0xFFFFFFFFu, 0, 0, 0);
     }
@@ -128,12 +134,17 @@ __device__ __forceinline__ float row16_sum(float x) {   // over the 16 lanes tha
     return x;
 }
 
-template <typename T, bool AKC, bool BKC, int MODE, int WI, int WJ, int TI, int TJ, int OCC>
-__global__ __launch_bounds__(64 * WI * WJ, OCC) void ce_gemm_kernel(const CeArgs p) {
+// The scores' products (short k, long epilogue) are persistent: a workgroup takes every gridDim-th tile, and the DMA runs two k-tiles
+// ahead across the border of two tiles, so that the next tile's operands arrive under this one's epilogue.  Lane (g, lr) of wave (wi, wj) ends up with Out[j][i] at
+// j = j0 + (wj TJ + y) 16 + lr, i = i0 + (wi TI + x) 16 + 4 g + r in register r of accumulator (x, y).
+template <typename T, bool AKC, bool BKC, int MODE, int WI, int WJ, int TI, int TJ>
+__global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p) {
 #if defined(__HIP_DEVICE_COMPILE__)   // the host pass needs the launch stub only, and cannot form the LDS builtins
     constexpr int NW = WI * WJ, IT = WI * TI * 16, JT = WJ * TJ * 16;
     constexpr int KE = 128 / (int)sizeof(T);
-    constexpr bool OPQ = !AKC && !BKC;
+    constexpr bool OPQ = !AKC && !BKC, ROWS_K = MODE == OUT || MODE == PART, SCORES = MODE == STATS || MODE == DZ;
+    constexpr bool MORE = SCORES;   // more than one tile a workgroup
+    static_assert(64 * NW >= IT && 64 * NW >= JT, "a thread a column and a row of the tile");
     using TA = Tile<T, AKC, IT, NW>;
     using TB = Tile<T, BKC, JT, NW>;
     // two stages of either operand, each a variable of its own: what the compiler can tell apart it does not make a read wait for
@@ -145,244 +156,335 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void ce_gemm_kernel(const CeArgs
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wi = wave % WI, wj = wave / WI, g = lane >> 4, lr = lane & 15;
     const int n = __builtin_amdgcn_readfirstlane(*p.n);   // in a scalar register, like all that the tile loop counts by
-    constexpr bool ROWS_K = MODE == OUT || MODE == PART;
     const int J = ROWS_K ? p.J : min(p.J, n), K = ROWS_K ? min(p.K, n) : p.K;
+    const int tiles_i = (p.I + IT - 1) / IT, tiles_j = (J + JT - 1) / JT, tiles = tiles_i * tiles_j * p.splits;
+    const int kt_all = (K + KE - 1) / KE, per_split = (kt_all + p.splits - 1) / p.splits;
 
-    // tile order: runs of 8 j-tiles against one i-tile, so the workgroups that an XCD holds at a time share operands in its L2
-    const int tiles_i = (p.I + IT - 1) / IT, tiles_j = (p.J + JT - 1) / JT;
+    // Tile order: runs of 8 j-tiles against one i-tile.  An XCD's workgroups take neighbours, which share operands in its L2.
+    struct At { int i0, j0, it, jt, split; };
+    auto at = [&](int id) __attribute__((always_inline)) {
+        At t;
+        int ti = tiles_i, tj = tiles_j;
+        asm volatile("" : "+s"(ti), "+s"(tj));   // the divisions' reciprocals are not kept in registers across the k-loop
+        t.split = id / (ti * tj);
+        id -= t.split * ti * tj;
+        const int per = 8 * ti, grp = id / per, in = id - grp * per, gj = min(8, tj - grp * 8);
+        t.it = in / gj;
+        t.jt = grp * 8 + in - t.it * gj;
+        t.i0 = t.it * IT;
+        t.j0 = t.jt * JT;
+        return t;
+    };
+    // k-tiles of a tile: an even number, so that every tile begins in the same stage; those behind its share of k read zeros
+    const int kts = max(2, (min(per_split, kt_all) + 1) & ~1);
     int id = xcd_remap(blockIdx.x, gridDim.x);
-    const int split = id / (tiles_i * tiles_j);
-    id -= split * tiles_i * tiles_j;
-    const int per = 8 * tiles_i, grp = id / per, in = id - grp * per, gj = min(8, tiles_j - grp * 8);
-    const int jt = grp * 8 + in % gj, it = in / gj;
-    const int i0 = it * IT, j0 = jt * JT;
-    if (j0 >= J) return;
-
-    const int kt_all = (K + KE - 1) / KE;
-    const int per_split = (kt_all + p.splits - 1) / p.splits;
-    const int kt0 = min(split * per_split, kt_all), kt1 = min(kt0 + per_split, kt_all);
+    if (id >= tiles) return;
+    TA ta;
+    TB tb;
+    ta.init(wave, lane, p.lda);
+    tb.init(wave, lane, p.ldb);
+    constexpr int NP = TA::NI + TB::NI;
+    // Where the DMA is: the next k-tile to fetch, `fin` k-tiles into a tile.  It runs on into the workgroup's next tile.
+    struct Slab { const char *pa, *pb; int left, ra, rb; };   // first slabs; k left; rows (columns) of the tile that exist
+    Slab f, fnext;
+    int fin = 0;
+    auto enter = [&](int id) __attribute__((always_inline)) {
+        Slab f;
+        const At t = at(id);
+        const int kt0 = min(t.split * per_split, kt_all);
+        f.pa = TA::slab(p.A, p.lda, t.i0, (long)kt0 * KE);
+        f.pb = TB::slab(p.B, p.ldb, t.j0, (long)kt0 * KE);
+        f.left = min(K, (kt0 + per_split) * KE) - kt0 * KE;
+        f.ra = min(IT, p.I - t.i0);
+        f.rb = min(JT, J - t.j0);
+        return f;
+    };
+    auto advance = [&] __attribute__((always_inline)) {
+        f.pa += TA::step(p.lda);
+        f.pb += TB::step(p.ldb);
+        f.left -= KE;
+        if constexpr (MORE) {   // by masks: a branch in the k-loop splits the blocks that its registers are planned over, and they spill
+            const long m = -(long)(++fin == kts);
+            auto sel = [&](auto a, auto b) { return (decltype(a))(((long)b & m) | ((long)a & ~m)); };
+            f.pa = sel(f.pa, fnext.pa);
+            f.pb = sel(f.pb, fnext.pb);
+            f.left = sel(f.left, fnext.left);
+            f.ra = sel(f.ra, fnext.ra);
+            f.rb = sel(f.rb, fnext.rb);
+            fin &= ~(int)m;
+        }
+    };
+    // the DMA, two k-tiles ahead, leaves tile r for r + 1 while r is multiplied, and r + 1 for r + 2 where a tile is two k-tiles
+    auto follow = [&](int id) __attribute__((always_inline)) {
+        const bool more = id < tiles;
+        fnext = enter(more ? id : 0);
+        fnext.left = more ? fnext.left : 0;   // no such tile: nothing is fetched
+    };
+    f = enter(id);
+    follow(id + gridDim.x);
+    auto issue = [&](const Slab& t, char* sa, char* sb, int q) __attribute__((always_inline)) {   // DMA instruction q
+        if (q < TA::NI) ta.issue(t.pa, sa, wave, t.left, q, p.lda, t.ra);
+        else tb.issue(t.pb, sb, wave, t.left, q - TA::NI, p.ldb, t.rb);
+    };
+    int lr_k = lr, g_k = g;
+    auto rd_a = [&](const char* s, int x, int ks) __attribute__((always_inline)) { return TA::read(s, wi * TI + x, ks, g_k, lr_k); };
+    auto rd_b = [&](const char* s, int y, int ks) __attribute__((always_inline)) { return TB::read(s, wj * TJ + y, ks, g_k, lr_k); };
 
     f32x4 acc[TI][TJ];
-#pragma unroll
-    for (int a = 0; a < TI; ++a)
-#pragma unroll
-        for (int b = 0; b < TJ; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    if (kt0 < kt1) {
-        TA ta;
-        TB tb;
-        ta.init(wave, lane, p.lda, i0, p.I);
-        tb.init(wave, lane, p.ldb, j0, J);
-        constexpr int NP = TA::NI + TB::NI;
-        auto issue = [&](int kt, char* sa, char* sb, int q) {   // DMA instruction q; a k-tile behind the last fetches nothing
-            const int left = kt < kt1 ? K - kt * KE : 0;
-            if (q < TA::NI) ta.issue(TA::slab(p.A, p.lda, i0, (long)kt * KE), sa, wave, left, q, p.lda, min(IT, p.I - i0));
-            else tb.issue(TB::slab(p.B, p.ldb, j0, (long)kt * KE), sb, wave, left, q - TA::NI, p.ldb, min(JT, J - j0));
-        };
-        int lr_k = lr, g_k = g;
-        auto rd_a = [&](const char* s, int x, int ks) { return TA::read(s, wi * TI + x, ks, g_k, lr_k); };
-        auto rd_b = [&](const char* s, int y, int ks) { return TB::read(s, wj * TJ + y, ks, g_k, lr_k); };
-        // A k-step is TI rows of TJ MFMAs.  Behind row x its A fragment is replaced by the next step's (needed TI rows later), the next
-        // step's B fragments arrive in a second set during the first rows.  In the second step of a k-tile, behind row 0 -- by then every
-        // read of this tile has landed -- the workgroup meets: the other stage is complete, this one is free for the tile after next,
-        // whose DMA instructions go out between the rows.
-        uint4 a[TI], b0[TJ], b1[TJ];
-        auto step = [&](const char* na, const char* nb, int ks, uint4 (&bc)[TJ], uint4 (&bn)[TJ], bool meet, int kt, char* fa, char* fb) {
-            // two transposed operands: their addresses are worked out here; held across the loop they spill (4096^3: 816 against 1100 TF/s)
-            if (OPQ) asm volatile("" : "+v"(lr_k), "+v"(g_k));
-#pragma unroll
-            for (int x = 0; x < TI; ++x) {
-#pragma unroll
-                for (int y = 0; y < TJ; ++y) Ce<T>::mma(a[x], bc[y], acc[x][y]);
-                if (meet && x == 0) {
-                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-                    __builtin_amdgcn_s_barrier();
-                    asm volatile("" ::: "memory");
-                }
-                a[x] = rd_a(na, x, ks);
-#pragma unroll
-                for (int y = 0; y < TJ; ++y)
-                    if (y / 2 == x) bn[y] = rd_b(nb, y, ks);
-                if (meet) {
-#pragma unroll
-                    for (int q = 0; q < NP; ++q)
-                        if (q * TI / NP == x) issue(kt, fa, fb, q);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        };
-#pragma unroll
-        for (int q = 0; q < NP; ++q) issue(kt0, sa0, sb0, q);
-#pragma unroll
-        for (int q = 0; q < NP; ++q) issue(kt0 + 1, sa1, sb1, q);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-#pragma unroll
-        for (int x = 0; x < TI; ++x) a[x] = rd_a(sa0, x, 0);
-#pragma unroll
-        for (int y = 0; y < TJ; ++y) b0[y] = rd_b(sb0, y, 0);
-        for (int kt = kt0; kt < kt1; kt += 2) {
-            step(sa0, sb0, 1, b0, b1, false, 0, nullptr, nullptr);
-            step(sa1, sb1, 0, b1, b0, true, kt + 2, sa0, sb0);
-            if (kt + 1 >= kt1) break;
-            step(sa1, sb1, 1, b0, b1, false, 0, nullptr, nullptr);
-            step(sa0, sb0, 0, b1, b0, true, kt + 3, sa1, sb1);
-        }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing may land in this workgroup's LDS after it
-    }
-
-    // opaque copies: nothing of an epilogue's addresses is worked out ahead of the k-loop, where every register is taken
-    int lr_e = lr, g_e = g;
-    asm volatile("" : "+v"(lr_e), "+v"(g_e));
-    // ---- epilogues: lane (g, lr), tile (x, y), register r holds Out[j = j0 + (wj TJ + y) 16 + lr][i = i0 + (wi TI + x) 16 + 4 g + r]
-    const int ib = i0 + wi * TI * 16 + 4 * g_e, jb = j0 + wj * TJ * 16 + lr_e;
-    if constexpr (MODE == STATS || MODE == DZ) {
-        __shared__ float red[(MODE == STATS ? WI * 3 * JT : WJ * IT)];
+    // A k-step is TI rows of TJ MFMAs.  Behind row x its A fragment is replaced by the next step's (needed TI rows later), the next
+    // step's B fragments arrive in a second set during the first rows.  In the second step of a k-tile, behind row 0 -- by then every
+    // read of this tile has landed -- the workgroup meets: the other stage is complete, this one is free for the k-tile after next,
+    // whose DMA instructions go out between the rows.
+    uint4 a[TI], b0[TJ], b1[TJ];
+    auto step = [&](const char* na, const char* nb, int ks, uint4 (&bc)[TJ], uint4 (&bn)[TJ], bool meet, char* fa, char* fb) __attribute__((always_inline)) {
+        // two transposed operands: their addresses are worked out here; held across the loop they spill (4096^3: 816 against 1100 TF/s)
+        if (OPQ) asm volatile("" : "+v"(lr_k), "+v"(g_k));
 #pragma unroll
         for (int x = 0; x < TI; ++x) {
-            const int i = ib + 16 * x;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float b = p.bias && i + r < p.I ? p.bias[i + r] : 0.f;
-                // a class masked with the type's lowest value: a base of its size would not be a whole number's step away from its
-                // scores; -inf and NaN stay what they are
-                if (fabsf(b) > 1e9f && fabsf(b) != INFINITY) b = copysignf(1e9f, b);
+            for (int y = 0; y < TJ; ++y) Ce<T>::mma(a[x], bc[y], acc[x][y]);
+            if (meet && x == 0) {
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+            }
+            __builtin_amdgcn_sched_barrier(0);   // the replaced fragment's registers are taken over, not doubled
+            a[x] = rd_a(na, x, ks);
 #pragma unroll
-                for (int y = 0; y < TJ; ++y) acc[x][y][r] = i + r < p.I ? acc[x][y][r] + b : -INFINITY;
+            for (int y = 0; y < TJ; ++y)
+                if (y / 2 == x) bn[y] = rd_b(nb, y, ks);
+            if (meet) {
+#pragma unroll
+                for (int q = 0; q < NP; ++q)
+                    if (q * TI / NP == x) issue(f, fa, fb, q);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (meet) advance();
+    };
+    auto meet_lds = [&] {   // LDS writes of the epilogue only: the DMA in flight is not waited for
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+
+#pragma unroll
+    for (int q = 0; q < NP; ++q) issue(f, sa0, sb0, q);
+    advance();
+#pragma unroll
+    for (int q = 0; q < NP; ++q) issue(f, sa1, sb1, q);
+    advance();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    auto first = [&](const char* na, const char* nb) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < TI; ++x) a[x] = rd_a(na, x, 0);
+#pragma unroll
+        for (int y = 0; y < TJ; ++y) b0[y] = rd_b(nb, y, 0);
+    };
+    first(sa0, sb0);
+    for (;; id += gridDim.x) {
+        if (MORE) follow(id + (kts == 2 ? 2 : 1) * (int)gridDim.x);
+#pragma unroll
+        for (int x = 0; x < TI; ++x)
+#pragma unroll
+            for (int y = 0; y < TJ; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const At cur = at(id);
+        // a thread's column and row of the tile: what the epilogue needs of them, on its way while the products are formed
+        float col_b = 0.f, row_base = 0.f, row_w = 0.f, row_s = 0.f;
+        int row_t = ROW_BAD;
+        if constexpr (SCORES) {
+            const int i = cur.i0 + tid, m = cur.j0 + tid;
+            if (tid < IT) col_b = i < p.I ? (p.bias ? p.bias[i] : 0.f) : -INFINITY;   // classes that do not exist: masked
+            if (tid < JT && m < J) {
+                row_t = p.tgt[m] - p.i_base;
+                if constexpr (MODE == DZ) {
+                    row_base = p.base2[m];
+                    row_w = p.coef[m];
+                    row_s = p.coef_s[m];
+                }
             }
         }
-        if constexpr (MODE == STATS) {
+        for (int kt = 0; kt < kts; kt += 2) {
+            step(sa0, sb0, 1, b0, b1, false, nullptr, nullptr);
+            step(sa1, sb1, 0, b1, b0, true, sa0, sb0);
+            step(sa1, sb1, 1, b0, b1, false, nullptr, nullptr);
+            step(sa0, sb0, 0, b1, b0, true, sa1, sb1);
+        }
+
+        // opaque copies: nothing of an epilogue's addresses is worked out ahead of the k-loop, where every register is taken
+        int lr_e = lr, g_e = g, tid_e = tid;
+        asm volatile("" : "+v"(lr_e), "+v"(g_e), "+v"(tid_e));
+        const int i0 = cur.i0, j0 = cur.j0, ib = i0 + wi * TI * 16 + 4 * g_e, jb = j0 + wj * TJ * 16 + lr_e;
+        if constexpr (SCORES) {
+            __shared__ float col[IT], rbase[JT], rw[JT], rs[JT];
+            __shared__ int rt[JT];
+            __shared__ float red[MODE == STATS ? WI * 3 * JT : WJ * IT];
+            // a class masked with the type's lowest value: a base of its size would not be a whole number's step away from its
+            // scores; -inf and NaN stay what they are
+            if (fabsf(col_b) > 1e9f && fabsf(col_b) != INFINITY) col_b = copysignf(1e9f, col_b);
+            if (tid_e < IT) col[tid_e] = col_b;
+            if (tid_e < JT) {
+                rt[tid_e] = row_t;
+                if constexpr (MODE == DZ) {
+                    rbase[tid_e] = j0 + tid_e < J ? row_base : 3e38f;   // rows that do not exist: exponentials 0
+                    rw[tid_e] = row_w;
+                    rs[tid_e] = row_s;
+                }
+            }
+            meet_lds();
 #pragma unroll
-            for (int y = 0; y < TJ; ++y) {
-                const int m = jb + 16 * y;
-                const int t = m < J ? p.tgt[m] - p.i_base : ROW_BAD;
-                float mx = -INFINITY, zs = 0.f;
+            for (int x = 0; x < TI; ++x) {
+                const f32x4 b = *reinterpret_cast<const f32x4*>(col + (wi * TI + x) * 16 + 4 * g_e);
 #pragma unroll
-                for (int x = 0; x < TI; ++x)
+                for (int y = 0; y < TJ; ++y) acc[x][y] += b;
+            }
+            if constexpr (MODE == STATS) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float z = acc[x][y][r];
-                        mx = fmaxf(mx, z);
-                        if (ib + 16 * x + r == t) p.zt[m] = z;
-                    }
-                if (p.smooth_z != 0.f) {
+                for (int y = 0; y < TJ; ++y) {
+                    const int t = rt[(wj * TJ + y) * 16 + lr_e] - ib;   // the target's place among this lane's classes
+                    float mx = -INFINITY, zs = 0.f;
 #pragma unroll
                     for (int x = 0; x < TI; ++x)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) zs += ib + 16 * x + r < p.I ? acc[x][y][r] : 0.f;
-                    zs = group4_sum(zs);
-                }
-                // exponentials are taken as 2^(z log2e - base) with a whole-number base: one fused multiply-add an element, and bases
-                // of different tiles differ by exact powers of two.  (Scores beyond 1e9 would need z - max in a step of its own.)
-                mx = group4_max(mx);
-                const float base = __builtin_ceilf(mx * LOG2E);
-                const float sub = base == -INFINITY ? 0.f : base;   // every class of the tile at -inf: its exponentials are 0
-                float s = 0.f;
+                        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[x][y][r]);
+                    if (__any(t >= 0 && t < TI * 16)) {
 #pragma unroll
-                for (int x = 0; x < TI; ++x)
+                        for (int x = 0; x < TI; ++x)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[x][y][r], LOG2E, -sub));
-                s = group4_sum(s);
-                if (g_e == 0) {
-                    const int c = (wj * TJ + y) * 16 + lr_e;
-                    red[(wi * 3 + 0) * JT + c] = base;
-                    red[(wi * 3 + 1) * JT + c] = s;
-                    red[(wi * 3 + 2) * JT + c] = zs;
-                }
-            }
-            __syncthreads();
-            for (int c = tid; c < JT; c += 64 * NW) {
-                if (j0 + c >= J) continue;
-                float mx = red[c], s = 0.f, zs = 0.f;
-#pragma unroll
-                for (int w = 1; w < WI; ++w) mx = fmaxf(mx, red[w * 3 * JT + c]);
-#pragma unroll
-                for (int w = 0; w < WI; ++w) {
-                    const float mw = red[w * 3 * JT + c];
-                    s += red[(w * 3 + 1) * JT + c] * (mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mw - mx));
-                    zs += red[(w * 3 + 2) * JT + c];
-                }
-                const size_t o = (size_t)it * p.rows_cap + j0 + c, plane = (size_t)tiles_i * p.rows_cap;
-                p.part[o] = mx;
-                p.part[plane + o] = s;
-                if (p.smooth_z != 0.f) p.part[2 * plane + o] = zs;
-            }
-        } else {
-            T* out = static_cast<T*>(p.out);
-#pragma unroll
-            for (int y = 0; y < TJ; ++y) {
-                const int m = jb + 16 * y;
-                const bool ok = m < J;
-                const float base = ok ? p.base2[m] : 0.f, c = ok ? p.coef[m] : 0.f, cs = ok ? p.coef_s[m] : 0.f;
-                const float low = -c * p.sm, hit = c * p.keep;
-                const int t = ok ? p.tgt[m] - p.i_base : ROW_BAD;
-                T* rowp = out + (size_t)(ok ? m : 0) * p.ldo + i0 + wi * TI * 16;
-#pragma unroll
-                for (int x = 0; x < TI; ++x)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int i = ib + 16 * x + r;
-                        float q = fmaf(__builtin_amdgcn_exp2f(fmaf(acc[x][y][r], LOG2E, -base)), cs, low);
-                        if (i == t) q -= hit;
-                        acc[x][y][r] = ok && i < p.I ? q : 0.f;
+                            for (int r = 0; r < 4; ++r)
+                                if (16 * x + r == t) p.zt[jb + 16 * y] = acc[x][y][r];
                     }
-                if constexpr (sizeof(T) == 2) {
+                    if (p.smooth_z != 0.f) {
+                        if (i0 + IT > p.I) {
 #pragma unroll
-                    for (int x = 0; x < TI; x += 2) store_bf16_tile_pair(rowp + 16 * x, g_e, acc[x][y], acc[x + 1][y], ok);
-                } else {
-                    if (ok) {
+                            for (int x = 0; x < TI; ++x)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) zs += ib + 16 * x + r < p.I ? acc[x][y][r] : 0.f;
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < TI; ++x)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) zs += acc[x][y][r];
+                        }
+                        zs = group4_sum(zs);
+                    }
+                    // exponentials are taken as 2^(z log2e - base) with a whole-number base: one fused multiply-add an element, and
+                    // bases of different tiles differ by exact powers of two.  (Scores beyond 1e9 would need z - max in a step of its own.)
+                    mx = group4_max(mx);
+                    const float base = __builtin_ceilf(mx * LOG2E);
+                    const float sub = base == -INFINITY ? 0.f : base;   // every class of the tile at -inf: its exponentials are 0
+                    float s = 0.f;
+#pragma unroll
+                    for (int x = 0; x < TI; ++x)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[x][y][r], LOG2E, -sub));
+                    s = group4_sum(s);
+                    if (g_e == 0) {
+                        const int c = (wj * TJ + y) * 16 + lr_e;
+                        red[(wi * 3 + 0) * JT + c] = base;
+                        red[(wi * 3 + 1) * JT + c] = s;
+                        red[(wi * 3 + 2) * JT + c] = zs;
+                    }
+                }
+                meet_lds();
+                if (tid_e < JT && j0 + tid_e < J) {
+                    const int c = tid_e;
+                    float mx = red[c], s = 0.f, zs = 0.f;
+#pragma unroll
+                    for (int w = 1; w < WI; ++w) mx = fmaxf(mx, red[w * 3 * JT + c]);
+#pragma unroll
+                    for (int w = 0; w < WI; ++w) {
+                        const float mw = red[w * 3 * JT + c];
+                        s += red[(w * 3 + 1) * JT + c] * (mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mw - mx));
+                        zs += red[(w * 3 + 2) * JT + c];
+                    }
+                    const size_t o = (size_t)cur.it * p.rows_cap + j0 + c, plane = (size_t)tiles_i * p.rows_cap;
+                    p.part[o] = mx;
+                    p.part[plane + o] = s;
+                    if (p.smooth_z != 0.f) p.part[2 * plane + o] = zs;
+                }
+            } else {
+                T* out = static_cast<T*>(p.out);
+#pragma unroll
+                for (int y = 0; y < TJ; ++y) {
+                    const int c = (wj * TJ + y) * 16 + lr_e, m = j0 + c;
+                    const bool ok = m < J;
+                    const float base = rbase[c], w = rw[c], cs = rs[c], low = -w * p.sm;
+                    const int t = rt[c] - ib;
+#pragma unroll
+                    for (int x = 0; x < TI; ++x)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[x][y][r] = fmaf(__builtin_amdgcn_exp2f(fmaf(acc[x][y][r], LOG2E, -base)), cs, low);
+                    if (__any(t >= 0 && t < TI * 16)) {
+#pragma unroll
+                        for (int x = 0; x < TI; ++x)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) acc[x][y][r] -= 16 * x + r == t ? w * p.keep : 0.f;
+                    }
+                    T* rowp = out + (size_t)(ok ? m : 0) * p.ldo + i0 + wi * TI * 16;
+                    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                        for (int x = 0; x < TI; x += 2) store_bf16_tile_pair(rowp + 16 * x, g_e, acc[x][y], acc[x + 1][y], ok);
+                    } else if (ok) {
 #pragma unroll
                         for (int x = 0; x < TI; ++x) store4(rowp + 16 * x + 4 * g_e, acc[x][y]);
                     }
                 }
-            }
-            if (p.dbp) {
+                if (p.dbp) {
 #pragma unroll
-                for (int x = 0; x < TI; ++x)
+                    for (int x = 0; x < TI; ++x)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
+                        for (int r = 0; r < 4; ++r) {
+                            float s = 0.f;
+#pragma unroll
+                            for (int y = 0; y < TJ; ++y) s += acc[x][y][r];
+                            s = row16_sum(s);
+                            if (lr_e == 0) red[wj * IT + (wi * TI + x) * 16 + 4 * g_e + r] = s;
+                        }
+                    meet_lds();
+                    if (tid_e < IT && i0 + tid_e < p.I) {
                         float s = 0.f;
 #pragma unroll
-                        for (int y = 0; y < TJ; ++y) s += acc[x][y][r];
-                        s = row16_sum(s);
-                        if (lr_e == 0) red[wj * IT + (wi * TI + x) * 16 + 4 * g_e + r] = s;
+                        for (int w = 0; w < WJ; ++w) s += red[w * IT + tid_e];
+                        p.dbp[(size_t)cur.jt * p.dbp_ld + i0 + tid_e] = s;
                     }
-                __syncthreads();
-                for (int c = tid; c < IT; c += 64 * NW) {
-                    float s = 0.f;
+                }
+            }
+        } else {
+            const float f = MODE == OUT ? *p.factor : 1.f;
 #pragma unroll
-                    for (int w = 0; w < WJ; ++w) s += red[w * IT + c];
-                    if (i0 + c < p.I) p.dbp[(size_t)jt * p.dbp_ld + i0 + c] = s;
+            for (int y = 0; y < TJ; ++y) {
+                const int j = jb + 16 * y;
+                if constexpr (MODE == OUT && sizeof(T) == 2) {   // every lane takes part in the exchange of a tile pair
+                    T* rowp = static_cast<T*>(p.out) + (size_t)min(j, J - 1) * p.ldo + i0 + wi * TI * 16;
+#pragma unroll
+                    for (int x = 0; x < TI; x += 2)
+                        store_bf16_tile_pair(rowp + 16 * x, g_e, acc[x][y] * f, acc[x + 1][y] * f, j < J && i0 + (wi * TI + x) * 16 + 8 * g_e < p.I);
+                } else {
+                    if (j >= J) continue;
+#pragma unroll
+                    for (int x = 0; x < TI; ++x) {
+                        const int i = ib + 16 * x;
+                        if (i >= p.I) continue;
+                        float* o = static_cast<float*>(p.out) + cur.split * p.split_stride + (size_t)j * p.ldo + i;
+                        f32x4 v = acc[x][y] * f;
+                        if (MODE == ACC && p.accumulate) v += load4(o);
+                        store4(o, v);
+                    }
                 }
             }
         }
-    } else {
-#pragma unroll
-        for (int y = 0; y < TJ; ++y) {
-            const int j = jb + 16 * y;
-            if constexpr (MODE == OUT && sizeof(T) == 2) {   // every lane takes part in the exchange of a tile pair
-                T* rowp = static_cast<T*>(p.out) + (size_t)min(j, J - 1) * p.ldo + i0 + wi * TI * 16;
-#pragma unroll
-                for (int x = 0; x < TI; x += 2)
-                    store_bf16_tile_pair(rowp + 16 * x, g_e, acc[x][y], acc[x + 1][y], j < J && i0 + (wi * TI + x) * 16 + 8 * g_e < p.I);
-            } else {
-                if (j >= J) continue;
-#pragma unroll
-                for (int x = 0; x < TI; ++x) {
-                    const int i = ib + 16 * x;
-                    if (i >= p.I) continue;
-                    float* o = static_cast<float*>(p.out) + split * p.split_stride + (size_t)j * p.ldo + i;
-                    f32x4 v = acc[x][y];
-                    if (MODE == ACC && p.accumulate) v += load4(o);
-                    store4(o, v);
-                }
-            }
-        }
+        if (!MORE || id + (int)gridDim.x >= tiles) break;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        first(sa0, sb0);   // read here: held through the epilogue they cost 48 registers
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing may land in this workgroup's LDS after it
 #endif
 }
-
 // ---------------------------------------------------------------------------------------------------------------------
 // Row selection: the rows whose target is not ignored, in order.  One workgroup; 8 rows a thread and step.
 // ---------------------------------------------------------------------------------------------------------------------
@@ -529,28 +631,35 @@ __global__ __launch_bounds__(1024) void ce_sum_kernel(const float* __restrict__ 
     if (threadIdx.x == 0) loss[0] = (float)(reduction == LSAM_REDUCE_MEAN ? part[0] / (double)n : part[0]);
 }
 
-__global__ __launch_bounds__(256) void ce_coef_kernel(const float* __restrict__ gout, int reduction, CeState st, float* __restrict__ coef,
-                                                      float* __restrict__ coef_s) {
+// dz is held in T in units of `factor`, one number for all rows, chosen so that what dominates it -- the target's entry of a row that
+// is not learned yet -- is exactly -1 under MEAN and SUM: (1 - e) gout / n.  Rounded to bf16 at its own size that entry would be off by
+// the same fraction in every row, and that fraction would come through the sums whole.  The factor is applied to the fp32 sums.
+__global__ __launch_bounds__(256) void ce_coef_kernel(const float* __restrict__ gout, int reduction, float unit, CeState st, float* __restrict__ coef,
+                                                      float* __restrict__ coef_s, float* __restrict__ factor) {
     const int r = blockIdx.x * 256 + threadIdx.x, n = *st.n;
+    if (r == 0)   // without rows every sum is 0 and stays it, whatever 1 / n is
+        *factor = n == 0 ? 0.f : reduction == LSAM_REDUCE_NONE ? unit : reduction == LSAM_REDUCE_MEAN ? gout[0] * unit / (float)n : gout[0] * unit;
     if (r >= n) return;
-    float c = reduction == LSAM_REDUCE_NONE ? gout[st.idx[r]] : gout[0];
-    if (reduction == LSAM_REDUCE_MEAN) c = c / (float)n;
+    float c = reduction == LSAM_REDUCE_NONE ? gout[st.idx[r]] : 1.f;
     if (st.tgt[r] == ROW_BAD) c = NAN;
     coef[r] = c;
-    coef_s[r] = c / st.sum[r];
+    coef_s[r] = c / (unit * st.sum[r]);
 }
 
-// dx[m] = sum of the splits' rows, or zeros where the row was ignored
+// dx[m] = factor * (sum of the splits' rows), or zeros where the row was ignored
 template <typename T>
 __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ acc, long stride, int splits, const int* __restrict__ pos, int M, int D,
-                                                    int Dp, int vec, T* __restrict__ dx, long lddx) {
+                                                    int Dp, int vec, const float* __restrict__ factor,
+                                                    T* __restrict__ dx, long lddx) {
     const int cpr = Dp / 4;
+    const float f = *factor;
     for (long id = (long)blockIdx.x * 256 + threadIdx.x; id < (long)M * cpr; id += (long)gridDim.x * 256) {
         const int m = (int)(id / cpr), c = (int)(id - (long)m * cpr) * 4, r = pos ? pos[m] : m;
         if (c >= D) continue;
         f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
         if (r >= 0)
             for (int s = 0; s < splits; ++s) v += load4(acc + s * stride + (size_t)r * Dp + c);
+        if (r >= 0) v *= f;
         T* o = dx + (size_t)m * lddx + c;
         if (vec) store4(o, v);
         else {
@@ -562,12 +671,12 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ ac
 }
 
 __global__ __launch_bounds__(256) void ce_db_kernel(const float* __restrict__ dbp, long ld, const int* __restrict__ np, int rows_tile, int V,
-                                                    float* __restrict__ db) {
+                                                    const float* __restrict__ factor, float* __restrict__ db) {
     const int v = blockIdx.x * 256 + threadIdx.x, tiles = (*np + rows_tile - 1) / rows_tile;
     if (v >= V) return;
     float s = 0.f;
     for (int t = 0; t < tiles; ++t) s += dbp[(size_t)t * ld + v];
-    db[v] = s;
+    db[v] = tiles ? s * *factor : 0.f;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -639,12 +748,13 @@ template <typename T> struct CePlan {
         if (f) *f = w;
         return c.used;
     }
-    struct Bwd { char *wp, *dz; float *coef, *coef_s, *dx, *dw, *dbp; };
+    struct Bwd { char *wp, *dz; float *factor, *coef, *coef_s, *dx, *dw, *dbp; };
     size_t bwd(char* base, Bwd* f, bool want_dx, bool want_dw, bool want_db) const {
         Carve c{base};
         Bwd w;
         w.wp = c.take<char>(pack_w ? (size_t)V * Dp * sizeof(T) : 0);
         w.dz = c.take<char>((size_t)M * piece * sizeof(T));
+        w.factor = c.take<float>(1);
         w.coef = c.take<float>(M);
         w.coef_s = c.take<float>(M);
         w.dx = c.take<float>(want_dx ? (size_t)s_dx * M * Dp : 0);
@@ -655,10 +765,10 @@ template <typename T> struct CePlan {
     }
 };
 
-template <typename T, bool AKC, bool BKC, int MODE, int WI, int WJ, int TI, int TJ, int OCC> int ce_gemm(const CeArgs& a, hipStream_t s) {
+template <typename T, bool AKC, bool BKC, int MODE, int WI, int WJ, int TI, int TJ> int ce_gemm(const CeArgs& a, hipStream_t s) {
     constexpr int IT = WI * TI * 16, JT = WJ * TJ * 16;
-    const int tiles = cdiv(a.I, IT) * cdiv(a.J, JT) * a.splits;
-    ce_gemm_kernel<T, AKC, BKC, MODE, WI, WJ, TI, TJ, OCC><<<tiles, 64 * WI * WJ, 0, s>>>(a);
+    const long tiles = (long)cdiv(a.I, IT) * cdiv(a.J, JT) * a.splits;
+    ce_gemm_kernel<T, AKC, BKC, MODE, WI, WJ, TI, TJ><<<(int)(tiles < CU || !(MODE == STATS || MODE == DZ) ? tiles : CU), 64 * WI * WJ, 0, s>>>(a);
     LSAM_LAUNCH_CHECK();
     return LSAM_OK;
 }
@@ -717,7 +827,7 @@ int launch_linear_ce_fwd(const void* x, long ldx, const void* w, long ldw, const
         a.B = st.xc; a.ldb = pl.Dp;
         a.I = V; a.J = M; a.K = pl.Dp; a.n = st.n;
         a.bias = bias; a.tgt = st.tgt; a.smooth_z = smooth; a.part = f.part; a.zt = f.zt; a.rows_cap = M; a.splits = 1;
-        LSAM_TRY((ce_gemm<T, true, true, STATS, 2, 4, 8, 4, 2>(a, s)));
+        LSAM_TRY((ce_gemm<T, true, true, STATS, 2, 4, 8, 4>(a, s)));
     }
     const int blocks = M > 0 ? cdiv(M, 16) : 1;
     if (M > 0 || reduction != LSAM_REDUCE_NONE) {
@@ -749,10 +859,9 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
     if (pl.pack_w) LSAM_TRY(gather<T>(w, ldw, nullptr, nullptr, V, D, pl.Dp, b.wp, s));
     const char* W = pl.pack_w ? b.wp : static_cast<const char*>(w);
     const long lw = pl.pack_w ? pl.Dp : ldw;
-    if (M > 0) {
-        ce_coef_kernel<<<cdiv(M, 256), 256, 0, s>>>(gout, reduction, st, b.coef, b.coef_s);
-        LSAM_LAUNCH_CHECK();
-    }
+    const float keep = 1.f - smooth, unit = keep > 0.f ? keep : 1.f;
+    ce_coef_kernel<<<cdiv(M > 0 ? M : 1, 256), 256, 0, s>>>(gout, reduction, unit, st, b.coef, b.coef_s, b.factor);
+    LSAM_LAUNCH_CHECK();
     for (int v0 = 0, k = 0; v0 < V; v0 += pl.piece, ++k) {
         const int nv = V - v0 < pl.piece ? V - v0 : pl.piece;
         if (M > 0) {
@@ -761,10 +870,10 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
             a.B = st.xc; a.ldb = pl.Dp;
             a.I = nv; a.J = M; a.K = pl.Dp; a.n = st.n;
             a.bias = bias ? bias + v0 : nullptr; a.tgt = st.tgt; a.i_base = v0;
-            a.base2 = st.base2; a.coef = b.coef; a.coef_s = b.coef_s; a.sm = smooth / (float)V; a.keep = 1.f - smooth;
+            a.base2 = st.base2; a.coef = b.coef; a.coef_s = b.coef_s; a.sm = smooth / ((float)V * unit); a.keep = keep / unit;
             a.dbp = db ? b.dbp + v0 : nullptr; a.dbp_ld = V;
             a.out = b.dz; a.ldo = pl.piece; a.splits = 1;
-            LSAM_TRY((ce_gemm<T, true, true, DZ, 2, 4, 8, 4, 2>(a, s)));
+            LSAM_TRY((ce_gemm<T, true, true, DZ, 2, 4, 8, 4>(a, s)));
         }
         if (dx && M > 0) {
             CeArgs a{};
@@ -772,7 +881,7 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
             a.B = b.dz; a.ldb = pl.piece;
             a.I = pl.Dp; a.J = M; a.K = nv; a.n = st.n;
             a.out = b.dx; a.ldo = pl.Dp; a.split_stride = (long)M * pl.Dp; a.splits = pl.s_dx; a.accumulate = k > 0;
-            LSAM_TRY((ce_gemm<T, false, true, ACC, 4, 2, 4, 8, 2>(a, s)));
+            LSAM_TRY((ce_gemm<T, false, true, ACC, 4, 2, 4, 8>(a, s)));
         }
         if (dw) {
             T* o = static_cast<T*>(dw) + (size_t)v0 * lddw;
@@ -781,14 +890,14 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
             a.B = b.dz; a.ldb = pl.piece;
             a.I = pl.Dp; a.J = nv; a.K = M; a.n = st.n; a.splits = pl.s_dw;
             if (!pl.dw_f32()) {
-                a.out = o; a.ldo = lddw;
-                LSAM_TRY((ce_gemm<T, false, false, OUT, 2, 4, 8, 4, 2>(a, s)));
+                a.out = o; a.ldo = lddw; a.factor = b.factor;
+                LSAM_TRY((ce_gemm<T, false, false, OUT, 2, 4, 8, 4>(a, s)));
             } else {
                 a.out = b.dw; a.ldo = pl.Dp; a.split_stride = (long)pl.piece * pl.Dp;
-                LSAM_TRY((ce_gemm<T, false, false, PART, 2, 4, 8, 4, 2>(a, s)));
+                LSAM_TRY((ce_gemm<T, false, false, PART, 2, 4, 8, 4>(a, s)));
                 const long blocks = ((long)nv * (pl.Dp / 4) + 255) / 256;
                 ce_dx_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(b.dw, a.split_stride, pl.s_dw, nullptr, nv, D, pl.Dp,
-                                                                                     D % 4 == 0, o, lddw);
+                                                                                     D % 4 == 0, b.factor, o, lddw);
                 LSAM_LAUNCH_CHECK();
             }
         }
@@ -796,11 +905,11 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
     if (dx && M > 0) {
         const long blocks = ((long)M * (pl.Dp / 4) + 255) / 256;
         ce_dx_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(b.dx, (long)M * pl.Dp, pl.s_dx, st.pos, M, D, pl.Dp,
-                                                                             D % 4 == 0, static_cast<T*>(dx), lddx);
+                                                                             D % 4 == 0, b.factor, static_cast<T*>(dx), lddx);
         LSAM_LAUNCH_CHECK();
     }
     if (db) {
-        ce_db_kernel<<<cdiv(V, 256), 256, 0, s>>>(b.dbp, V, st.n, 256, V, db);
+        ce_db_kernel<<<cdiv(V, 256), 256, 0, s>>>(b.dbp, V, st.n, 256, V, b.factor, db);
         LSAM_LAUNCH_CHECK();
     }
     return LSAM_OK;

@@ -682,7 +682,9 @@ __global__ __launch_bounds__(256) void ce_db_kernel(const float* __restrict__ db
 // ---------------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr size_t DZ_CAP = (size_t)256 << 20;   // a piece's dz is kept within the last-level cache (256 MB)
+// A piece's dz.  16384 x 256 x 32000 in all: 1560 us with 256 MB (what the last-level cache holds), 1475 with 512, 1337 with 1024: fewer
+// passes over the fp32 sums of dx weigh more than where dz is read from.
+constexpr size_t DZ_CAP = (size_t)1 << 30;
 constexpr int CU = 256;
 
 struct Carve {
@@ -695,35 +697,60 @@ struct Carve {
     }
 };
 
+// Tiles of 256 x 256 (8 waves of 128 x 64 or 64 x 128, one workgroup a CU) or 128 x 128 (64 x 32, two a CU).  The large one feeds the
+// bf16 matrix pipes from LDS at close to their rate; the small one balances where the large leaves CUs idle.  fp32 takes the small one
+// always: its matrix instructions are 16 times slower, LDS keeps up either way.
+// Rounds of tiles, a small one costed at a quarter of a large one and half as much again.
+inline bool small_tiles(bool fp32, long big, long small) { return fp32 || (big + CU - 1) / CU * 4 > ((small + CU - 1) / CU * 3 + 1) / 2; }
+
 template <typename T> struct CePlan {
-    static constexpr int EPC = 16 / (int)sizeof(T), TILE = 256;
-    int M, D, V, Dp, tiles_v, tiles_m, tiles_d;
-    bool pack_w;
-    int piece, pieces, s_dx, s_dw;
+    static constexpr int EPC = 16 / (int)sizeof(T);
+    static constexpr bool FP32 = sizeof(T) == 4;
+    int M, D, V, Dp, tile, tiles_v, tiles_m;   // tile: of the scores
+    bool pack_w, dx_small, dw_small;
+    int piece, s_dx, s_dw;
     CePlan(int M_, int D_, int V_, bool pack) : M(M_), D(D_), V(V_), pack_w(pack) {
         Dp = (D + EPC - 1) / EPC * EPC;
-        tiles_v = cdiv(V, TILE);
-        tiles_m = M > 0 ? cdiv(M, TILE) : 1;
-        tiles_d = cdiv(Dp, TILE);
-        const size_t col = (size_t)M * sizeof(T) * TILE;
-        size_t pt = DZ_CAP / (col ? col : 1);
+        const int m = M > 0 ? M : 1;
+        tile = small_tiles(FP32, (long)cdiv(V, 256) * cdiv(m, 256), (long)cdiv(V, 128) * cdiv(m, 128)) ? 128 : 256;
+        tiles_v = cdiv(V, tile);
+        tiles_m = cdiv(m, tile);
+        const size_t col = (size_t)m * sizeof(T) * 256;
+        size_t pt = DZ_CAP / col;
         if (pt < 1) pt = 1;
         if (pt > 1024) pt = 1024;   // byte offsets within a tile's rows stay within 31 bits
-        if (pt > (size_t)tiles_v) pt = tiles_v;
-        pieces = cdiv(tiles_v, (int)pt);
-        piece = cdiv(tiles_v, pieces) * TILE;
-        pieces = cdiv(V, piece);
-        const int kt = 128 / (int)sizeof(T);
-        auto splits = [&](int tiles, int ksteps) {
-            int s = tiles >= CU ? 1 : CU / tiles;
-            const int most = ksteps / 4 > 0 ? ksteps / 4 : 1;   // at least four k-tiles a split
-            return s < most ? (s > 0 ? s : 1) : most;
+        const int vt = cdiv(V, 256);
+        if (pt > (size_t)vt) pt = vt;
+        piece = (int)pt * 256;
+        auto pick = [&](int rows, int k, bool& small, int& cuts) {
+            const long big = (long)cdiv(rows, 256) * cdiv(Dp, 256), lit = (long)cdiv(rows, 128) * cdiv(Dp, 128);
+            const int sb = splits(big, k, false), sl = splits(lit, k, true);
+            small = small_tiles(FP32, big * sb, lit * sl);
+            // compare the work of a CU: rounds of tiles times their share of k
+            if (!FP32) small = (double)((big * sb + CU - 1) / CU) * 4 / sb > 1.5 * (double)((lit * sl + CU - 1) / CU) / sl;
+            cuts = small ? sl : sb;
         };
-        s_dx = splits(tiles_m * tiles_d, cdiv(piece, kt));
-        s_dw = splits(piece / TILE * tiles_d, cdiv(M > 0 ? M : 1, kt));
+        pick(m, piece, dx_small, s_dx);
+        pick(piece, m, dw_small, s_dw);
+    }
+    int splits(long tiles, int k, bool small) const {   // cuts of k that keep the CUs busy, at least four k-tiles each
+        const int slots = small ? 2 * CU : CU, most = k * (int)sizeof(T) / 512 > 0 ? k * (int)sizeof(T) / 512 : 1;
+        const long s = tiles >= slots ? 1 : slots / tiles;
+        return (int)(s < most ? s : most);
+    }
+    // Several rounds of the weight gradient's large tiles with the last one less than half full: the classes of that one go apart, their
+    // k cut (8192 x 896 x 50257: 788 tiles on 256 CUs).  How many of nv classes do.
+    int rest(int nv) const {
+        const int td = cdiv(Dp, 256), vt = cdiv(nv, 256), over = vt * td % CU;
+        if (dw_small || dw_f32() || vt * td <= CU || over == 0 || over >= CU / 2) return 0;
+        const int rt = cdiv(over, td);
+        return splits((long)rt * td, M, false) > 1 ? nv - (vt - rt) * 256 : 0;
     }
     // partial sums, or rows of dW that do not take four columns at a time: through fp32 and the joining kernel
     bool dw_f32() const { return s_dw > 1 || D % EPC; }
+    size_t dw_floats() const {   // the rest's tiles times cuts: at most CU of 65536
+        return dw_f32() ? (size_t)s_dw * piece * Dp : piece / 256 * cdiv(Dp, 256) > CU ? (size_t)CU * 65536 : 0;
+    }
     size_t state(char* base, CeState* st) const {
         Carve c{base};
         CeState s;
@@ -758,19 +785,30 @@ template <typename T> struct CePlan {
         w.coef = c.take<float>(M);
         w.coef_s = c.take<float>(M);
         w.dx = c.take<float>(want_dx ? (size_t)s_dx * M * Dp : 0);
-        w.dw = c.take<float>(want_dw && dw_f32() ? (size_t)s_dw * piece * Dp : 0);
+        w.dw = c.take<float>(want_dw ? dw_floats() : 0);
         w.dbp = c.take<float>(want_db ? (size_t)tiles_m * V : 0);
         if (f) *f = w;
         return c.used;
     }
 };
 
-template <typename T, bool AKC, bool BKC, int MODE, int WI, int WJ, int TI, int TJ> int ce_gemm(const CeArgs& a, hipStream_t s) {
+template <typename T, bool AKC, bool BKC, int MODE, int WI, int WJ, int TI, int TJ> int ce_gemm_run(const CeArgs& a, int a_cu, hipStream_t s) {
     constexpr int IT = WI * TI * 16, JT = WJ * TJ * 16;
-    const long tiles = (long)cdiv(a.I, IT) * cdiv(a.J, JT) * a.splits;
-    ce_gemm_kernel<T, AKC, BKC, MODE, WI, WJ, TI, TJ><<<(int)(tiles < CU || !(MODE == STATS || MODE == DZ) ? tiles : CU), 64 * WI * WJ, 0, s>>>(a);
+    const long tiles = (long)cdiv(a.I, IT) * cdiv(a.J, JT) * a.splits, most = (long)CU * a_cu;
+    ce_gemm_kernel<T, AKC, BKC, MODE, WI, WJ, TI, TJ><<<(int)(tiles < most || !(MODE == STATS || MODE == DZ) ? tiles : most), 64 * WI * WJ, 0, s>>>(a);
     LSAM_LAUNCH_CHECK();
     return LSAM_OK;
+}
+// wave grids of the large tile: as many fragments of the operand that is cheaper to read.  4096^3: A transposed 64 x 128 waves 1333 TF/s
+// against 1177 with 128 x 64; both transposed 1205 against 1103 the other way round
+template <typename T, bool AKC, bool BKC, int MODE> int ce_gemm(const CeArgs& a, bool small, hipStream_t s) {
+    if constexpr (sizeof(T) == 2) {
+        if (!small) {
+            if constexpr (!AKC && BKC) return ce_gemm_run<T, AKC, BKC, MODE, 4, 2, 4, 8>(a, 1, s);
+            else return ce_gemm_run<T, AKC, BKC, MODE, 2, 4, 8, 4>(a, 1, s);
+        }
+    }
+    return ce_gemm_run<T, AKC, BKC, MODE, 2, 4, 4, 2>(a, 2, s);
 }
 
 template <typename T> bool rows_direct(const void* p, long ld, int D) {   // rows that 16-byte chunks can be fetched from in place
@@ -791,7 +829,7 @@ template <typename T> int gather(const void* src, long ld, const int* idx, const
 int ce_check(int M, int D, int V, int reduction, float smooth) {
     LSAM_REQUIRE(M >= 0 && D > 0 && V > 0, LSAM_ERR_BAD_ARG, "linear_ce: %d rows, %d columns, %d classes", M, D, V);
     LSAM_REQUIRE(M <= (1 << 28) && V <= (1 << 28) && D <= (1 << 18), LSAM_ERR_UNSUPPORTED, "linear_ce: %d rows, %d columns, %d classes", M, D, V);
-    LSAM_REQUIRE(((long)M / 256 + 1) * ((long)V / 256 + 1) < (1l << 30), LSAM_ERR_UNSUPPORTED, "linear_ce: %d rows x %d classes", M, V);
+    LSAM_REQUIRE(((long)M / 128 + 1) * ((long)V / 128 + 1) < (1l << 30), LSAM_ERR_UNSUPPORTED, "linear_ce: %d rows x %d classes", M, V);
     LSAM_REQUIRE(reduction >= 0 && reduction <= 2, LSAM_ERR_BAD_ARG, "linear_ce: reduction %d", reduction);
     LSAM_REQUIRE(smooth >= 0.f && smooth <= 1.f, LSAM_ERR_BAD_ARG, "linear_ce: label smoothing %g outside [0, 1]", (double)smooth);
     return LSAM_OK;
@@ -827,7 +865,7 @@ int launch_linear_ce_fwd(const void* x, long ldx, const void* w, long ldw, const
         a.B = st.xc; a.ldb = pl.Dp;
         a.I = V; a.J = M; a.K = pl.Dp; a.n = st.n;
         a.bias = bias; a.tgt = st.tgt; a.smooth_z = smooth; a.part = f.part; a.zt = f.zt; a.rows_cap = M; a.splits = 1;
-        LSAM_TRY((ce_gemm<T, true, true, STATS, 2, 4, 8, 4>(a, s)));
+        LSAM_TRY((ce_gemm<T, true, true, STATS>(a, pl.tile == 128, s)));
     }
     const int blocks = M > 0 ? cdiv(M, 16) : 1;
     if (M > 0 || reduction != LSAM_REDUCE_NONE) {
@@ -873,7 +911,7 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
             a.base2 = st.base2; a.coef = b.coef; a.coef_s = b.coef_s; a.sm = smooth / ((float)V * unit); a.keep = keep / unit;
             a.dbp = db ? b.dbp + v0 : nullptr; a.dbp_ld = V;
             a.out = b.dz; a.ldo = pl.piece; a.splits = 1;
-            LSAM_TRY((ce_gemm<T, true, true, DZ, 2, 4, 8, 4>(a, s)));
+            LSAM_TRY((ce_gemm<T, true, true, DZ>(a, pl.tile == 128, s)));
         }
         if (dx && M > 0) {
             CeArgs a{};
@@ -881,25 +919,31 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
             a.B = b.dz; a.ldb = pl.piece;
             a.I = pl.Dp; a.J = M; a.K = nv; a.n = st.n;
             a.out = b.dx; a.ldo = pl.Dp; a.split_stride = (long)M * pl.Dp; a.splits = pl.s_dx; a.accumulate = k > 0;
-            LSAM_TRY((ce_gemm<T, false, true, ACC, 4, 2, 4, 8>(a, s)));
+            LSAM_TRY((ce_gemm<T, false, true, ACC>(a, pl.dx_small, s)));
         }
         if (dw) {
-            T* o = static_cast<T*>(dw) + (size_t)v0 * lddw;
-            CeArgs a{};
-            a.A = st.xc; a.lda = pl.Dp;
-            a.B = b.dz; a.ldb = pl.piece;
-            a.I = pl.Dp; a.J = nv; a.K = M; a.n = st.n; a.splits = pl.s_dw;
-            if (!pl.dw_f32()) {
-                a.out = o; a.ldo = lddw; a.factor = b.factor;
-                LSAM_TRY((ce_gemm<T, false, false, OUT, 2, 4, 8, 4>(a, s)));
-            } else {
-                a.out = b.dw; a.ldo = pl.Dp; a.split_stride = (long)pl.piece * pl.Dp;
-                LSAM_TRY((ce_gemm<T, false, false, PART, 2, 4, 8, 4>(a, s)));
-                const long blocks = ((long)nv * (pl.Dp / 4) + 255) / 256;
-                ce_dx_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(b.dw, a.split_stride, pl.s_dw, nullptr, nv, D, pl.Dp,
-                                                                                     D % 4 == 0, b.factor, o, lddw);
+            // classes c0 .. c0 + nc of the piece; through fp32 where k is cut or T rows do not take four columns at a time
+            auto weight_grad = [&](int c0, int nc, bool f32, int cuts) -> int {
+                T* o = static_cast<T*>(dw) + (size_t)(v0 + c0) * lddw;
+                CeArgs a{};
+                a.A = st.xc; a.lda = pl.Dp;
+                a.B = b.dz + (size_t)c0 * sizeof(T); a.ldb = pl.piece;
+                a.I = pl.Dp; a.J = nc; a.K = M; a.n = st.n; a.splits = cuts;
+                if (!f32) {
+                    a.out = o; a.ldo = lddw; a.factor = b.factor;
+                    return ce_gemm<T, false, false, OUT>(a, pl.dw_small, s);
+                }
+                a.out = b.dw; a.ldo = pl.Dp; a.split_stride = (long)nc * pl.Dp;
+                LSAM_TRY((ce_gemm<T, false, false, PART>(a, pl.dw_small, s)));
+                const long blocks = ((long)nc * (pl.Dp / 4) + 255) / 256;
+                ce_dx_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(b.dw, a.split_stride, cuts, nullptr, nc, D, pl.Dp, D % 4 == 0,
+                                                                                     b.factor, o, lddw);
                 LSAM_LAUNCH_CHECK();
-            }
+                return LSAM_OK;
+            };
+            const int rest = pl.rest(nv);
+            LSAM_TRY(weight_grad(0, nv - rest, pl.dw_f32(), pl.s_dw));
+            if (rest) LSAM_TRY(weight_grad(nv - rest, rest, true, pl.splits((long)cdiv(rest, 256) * cdiv(pl.Dp, 256), M, false)));
         }
     }
     if (dx && M > 0) {
@@ -909,7 +953,7 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
         LSAM_LAUNCH_CHECK();
     }
     if (db) {
-        ce_db_kernel<<<cdiv(V, 256), 256, 0, s>>>(b.dbp, V, st.n, 256, V, b.factor, db);
+        ce_db_kernel<<<cdiv(V, 256), 256, 0, s>>>(b.dbp, V, st.n, pl.tile, V, b.factor, db);
         LSAM_LAUNCH_CHECK();
     }
     return LSAM_OK;

@@ -88,10 +88,22 @@ def test_matches_float64(M, D, V, dtype, bias, smoothing, reduction):
     check(x, w, t, b, g, smoothing, reduction)
 
 
+# large tiles (bf16): one and several tiles a workgroup, one to four k-tiles, an odd number of them, rows and classes that end inside a
+# tile, a weight gradient whose last tiles go apart
+LARGE = [(4096, 16, 4096), (4000, 100, 8200), (5001, 448, 8192), (3900, 200, 8300), (1100, 256, 67300), (300, 896, 66000)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M, D, V", LARGE)
+def test_large_tiles(M, D, V, dtype):
+    x, w, t, b, g = make(M, D, V, dtype, M % 2 == 0, M + D + V)
+    check(x, w, t, b, g, 0.1 if D == 100 else 0.0, "none" if D == 200 else "mean")
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_several_pieces_of_the_classes(dtype):
-    # 36,000 x 8,000 gradients of scores are over a piece's 256 MB in either type: the products accumulate over pieces
-    x, w, t, b, g = make(36000, 16, 8000, dtype, True, 5)
+    # gradients of the scores over a piece's 1 GiB in either type: the products accumulate over pieces
+    x, w, t, b, g = make(36000, 16, 15990 if dtype == torch.bfloat16 else 8000, dtype, True, 5)
     check(x, w, t, b, g, 0.1, "mean")
 
 

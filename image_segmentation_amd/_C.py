@@ -187,6 +187,11 @@ def stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def stream_of(device_index: int) -> int:
+    """Handle of the device's current stream, without the Stream object that current_stream() builds (a few us a call)."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
 def dtype_code(dt: torch.dtype) -> int:
     if dt == torch.float32:
         return F32

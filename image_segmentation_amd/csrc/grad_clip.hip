@@ -241,7 +241,8 @@ int launch_clip_grads(const unsigned long long* src, const unsigned long long* d
         w.reserve(count);
         for (int i = 0; i < count; ++i)
             if (n[i]) w.push_back({dst[i], dst[i] + (unsigned long long)n[i] * (kind[i] & 2 ? 2 : 4), i});
-        std::sort(w.begin(), w.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
+        const auto below = [](const Span& a, const Span& b) { return a.lo < b.lo; };
+        if (!std::is_sorted(w.begin(), w.end(), below)) std::sort(w.begin(), w.end(), below);
         for (size_t k = 1; k < w.size(); ++k)
             LSAM_REQUIRE(w[k].lo >= w[k - 1].hi, LSAM_ERR_BAD_ARG, "clip_grads: tensors %d and %d share memory", w[k - 1].i, w[k].i);
         for (int i = 0; i < count; ++i) {

@@ -44,24 +44,22 @@ def clip_grads_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float
         raise ValueError(f"clip_grads_: max_norm {max_norm}, grad_scale {grad_scale}")
     if not grads:
         return torch.tensor(0.0)
-    into = grads if out is None else list(out)
-    if len(into) != len(grads) or any(a.shape != b.shape for a, b in (() if out is None else zip(into, grads))):
-        raise ops._C.LsamError("clip_grads_: out must hold one tensor of the same shape for each gradient")
-    if not all(map(torch.Tensor.is_contiguous, grads)):           # a gradient in another layout goes through a contiguous copy
-        src = [g.contiguous() for g in grads]
-        if out is None:
-            into = src
+    if out is None:
+        into = grads
     else:
-        src = grads
-    dst = into if into is src or all(map(torch.Tensor.is_contiguous, into)) else [t.contiguous() for t in into]
+        into = list(out)
+        if list(map(torch.Tensor.size, into)) != list(map(torch.Tensor.size, grads)):
+            raise ops._C.LsamError("clip_grads_: out must hold one tensor of the same shape for each gradient")
+    dense = torch.Tensor.is_contiguous
+    src = grads if all(map(dense, grads)) else [g.contiguous() for g in grads]   # another layout goes through a contiguous copy
+    dst = src if out is None else into if all(map(dense, into)) else [t.contiguous() for t in into]
     if error_if_nonfinite:
-        norm = ops.clip_grads(src, src, float("inf"), inf_norm)[0] * abs(grad_scale)
+        norm = ops._clip_grads(src, src, float("inf"), inf_norm, 1.0)[0] * abs(grad_scale)
         if not bool(torch.isfinite(norm)):
             raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so it cannot be clipped.")
-    norm = ops.clip_grads(src, dst, max_norm, inf_norm, grad_scale)[0]
-    target = grads if out is None else into
-    if dst is not target:
-        for t, d in zip(target, dst):
+    norm = ops._clip_grads(src, dst, max_norm, inf_norm, grad_scale)[0]
+    if dst is not into:
+        for t, d in zip(into, dst):
             if t is not d:
                 t.copy_(d)
     return norm

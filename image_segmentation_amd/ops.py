@@ -6,6 +6,7 @@ go through here: `Hiera.forward` makes a single `lsam_hiera_forward` call.
 Everything requires CUDA(HIP) tensors; nothing here computes in PyTorch."""
 from __future__ import annotations
 
+import contextlib
 import math
 from array import array
 from typing import Optional, Sequence, Tuple
@@ -13,7 +14,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _C
-from ._C import check, dtype_code, lib, ptr, stream
+from ._C import check, dtype_code, lib, ptr, stream, stream_of
 
 
 def _need_gpu(*ts):
@@ -773,13 +774,19 @@ def batched_outer(G: torch.Tensor, U: torch.Tensor) -> torch.Tensor:
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
-def _same_device(*ts):
-    """The operands' one GPU: calls run there, on its current stream, whatever the current device is."""
-    _need_gpu(*ts)
-    devs = {t.device for t in ts if t is not None}
-    if len(devs) != 1:
-        raise _C.LsamError(f"operands on different devices: {sorted(map(str, devs))}")
-    return torch.cuda.device(devs.pop())
+_HERE = contextlib.nullcontext()
+
+
+def _on_device(*ts):
+    """(index, context) of the operands' one GPU: calls run there, on its current stream, whatever the current device is."""
+    d = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != d:
+            _need_gpu(*ts)
+            raise _C.LsamError(f"operands on different devices: {sorted({str(t.device) for t in ts if t is not None})}")
+    if d < 0:
+        _need_gpu(*ts)
+    return d, _HERE if torch.cuda.current_device() == d else torch.cuda.device(d)
 
 
 def _unit_stride(t: torch.Tensor) -> torch.Tensor:
@@ -798,7 +805,8 @@ def linear_ce_fwd(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
                   label_smoothing: float = 0.0, reduction: str = "mean"):
     """(loss, state): softmax cross entropy of x [M, D] @ weight [V, D]^T + bias [V] against int64 target [M]; fp32 loss, [M] or 0-d.
     `state` (uint8) is what linear_ce_bwd needs; it holds the selected rows of x, so x itself may change or go."""
-    with _same_device(x, weight, bias, target):
+    dev, on = _on_device(x, weight, bias, target)
+    with on:
         code = dtype_code(x.dtype)
         x, weight, b = _unit_stride(x), _unit_stride(weight), _f32c(bias)
         target = target.detach().to(torch.int64).contiguous()
@@ -808,14 +816,15 @@ def linear_ce_fwd(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
         state = torch.empty(L.lsam_linear_ce_state_bytes(code, M, D), **u8)
         ws = torch.empty(L.lsam_linear_ce_ws_bytes(code, M, D, V, ptr(weight), _ld(weight), label_smoothing, 0), **u8)
         check(L.lsam_linear_ce_fwd(code, ptr(x), _ld(x), ptr(weight), _ld(weight), ptr(b), ptr(target), M, D, V, ignore_index,
-                                   label_smoothing, REDUCTIONS[reduction], ptr(loss), ptr(state), ptr(ws), ws.numel(), stream()))
+                                   label_smoothing, REDUCTIONS[reduction], ptr(loss), ptr(state), ptr(ws), ws.numel(), stream_of(dev)))
     return loss, state
 
 
 def linear_ce_bwd(gout: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], M: int,
                   label_smoothing: float = 0.0, reduction: str = "mean", want=(True, True, True)):
     """(dx, dweight, dbias fp32) of linear_ce_fwd, None where not wanted; gout fp32 [M] or 0-d."""
-    with _same_device(gout, state, weight, bias):
+    dev, on = _on_device(gout, state, weight, bias)
+    with on:
         code = dtype_code(weight.dtype)
         weight, b, gout = _unit_stride(weight), _f32c(bias), _f32c(gout)
         V, D = weight.shape
@@ -829,7 +838,7 @@ def linear_ce_bwd(gout: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
         ws = torch.empty(L.lsam_linear_ce_ws_bytes(code, M, D, V, ptr(weight), _ld(weight), label_smoothing, flags), dtype=torch.uint8,
                          device=weight.device)
         check(L.lsam_linear_ce_bwd(code, ptr(weight), _ld(weight), ptr(b), ptr(gout), M, D, V, label_smoothing, REDUCTIONS[reduction],
-                                   ptr(state), ptr(dx), D, ptr(dw), D, ptr(db), ptr(ws), ws.numel(), stream()))
+                                   ptr(state), ptr(dx), D, ptr(dw), D, ptr(db), ptr(ws), ws.numel(), stream_of(dev)))
     return dx, dw, db
 
 
@@ -840,27 +849,31 @@ ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 def channels_last_rows(x: torch.Tensor) -> Optional[Tuple[int, int, int, int]]:
     """(samples, pixels, sample stride, pixel stride) of [N, C, *spatial] whose channels are contiguous and whose pixels lie one
     stride apart in row-major order (channels-last, also as a channel slice of a wider map); None if it is laid out otherwise."""
-    N, Cc = x.shape[:2]
+    shape, strides = x.shape, x.stride()
+    N, Cc = shape[:2]
     if x.numel() == 0:                                         # nothing to lie anywhere
-        return N, math.prod(x.shape[2:]), 0, Cc
-    if Cc > 1 and x.stride(1) != 1:
+        return N, math.prod(shape[2:]), 0, Cc
+    if Cc > 1 and strides[1] != 1:
         return None
     P, px = 1, None
-    for n, st in zip(reversed(x.shape[2:]), reversed(x.stride()[2:])):
+    for a in range(len(shape) - 1, 1, -1):
+        n = shape[a]
         if n == 1:
             continue
         if px is None:
-            px = st
-        elif st != px * P:
+            px = strides[a]
+        elif strides[a] != px * P:
             return None
         P *= n
     px = Cc if px is None else px
-    sx = x.stride(0) if N > 1 else P * px
+    sx = strides[0] if N > 1 else P * px
     return (N, P, sx, px) if (px >= Cc or P == 1) and (sx >= Cc or N == 1) else None
 
 
-def _channels_last_like(x: torch.Tensor) -> torch.Tensor:
+def _channels_last_like(x: torch.Tensor, lay=None) -> torch.Tensor:
     """Empty tensor of x's shape and type, channels last without gaps."""
+    if lay is not None and lay[3] == x.shape[1] and lay[2] == lay[1] * lay[3] and x.dim() > 2:
+        return torch.empty_like(x)                             # keeps the order of a dense tensor's axes
     N, Cc = x.shape[:2]
     return torch.empty((N, *x.shape[2:], Cc), dtype=x.dtype, device=x.device).movedim(-1, 1)
 
@@ -869,76 +882,92 @@ def group_norm_act_fwd(x: torch.Tensor, groups: int, weight: Optional[torch.Tens
                        act: str = "none", want_stats: bool = False):
     """act(group_norm(x)) for T [N, C, *spatial] laid out channels last, same type and layout; with want_stats also fp32
     [N, groups, 2] (mean, 1 / std) for group_norm_act_bwd."""
-    with _same_device(x, weight, bias):
-        code = dtype_code(x.dtype)
+    dev, on = _on_device(x, weight, bias)
+    with on:
         x = x.detach()
         lay = channels_last_rows(x)
         if lay is None:
             raise _C.LsamError(f"group_norm_act: shape {tuple(x.shape)} with strides {x.stride()} is not channels last "
                                "(x.contiguous(memory_format=torch.channels_last))")
         N, P, sx, px = lay
-        Cc, w, b = x.shape[1], _f32c(weight), _f32c(bias)
-        y = _channels_last_like(x)
-        stats = torch.empty(N, groups, 2, dtype=torch.float32, device=x.device) if want_stats else None
-        L = lib()
-        ws = torch.empty(L.lsam_group_norm_act_ws_bytes(N, P, Cc, groups, 0), dtype=torch.uint8, device=x.device)
-        check(L.lsam_group_norm_act_fwd(code, ptr(x), sx, px, ptr(w), ptr(b), N, P, Cc, groups, eps, ACTIVATIONS[act], ptr(y), ptr(stats),
-                                        ptr(ws), ws.numel(), stream()))
+        Cc, w, b, L = x.shape[1], _f32c(weight), _f32c(bias), lib()
+        y = _channels_last_like(x, lay)
+        stats = torch.empty((N, groups, 2), dtype=torch.float32, device=x.device) if want_stats else None
+        nws = L.lsam_group_norm_act_ws_bytes(N, P, Cc, groups, 0)
+        ws = torch.empty(nws, dtype=torch.uint8, device=x.device)
+        check(L.lsam_group_norm_act_fwd(dtype_code(x.dtype), x.data_ptr(), sx, px, ptr(w), ptr(b), N, P, Cc, groups, eps, ACTIVATIONS[act],
+                                        y.data_ptr(), ptr(stats), ws.data_ptr(), nws, stream_of(dev)))
     return (y, stats) if want_stats else y
 
 
 def group_norm_act_bwd(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
                        act: str = "none"):
     """(dx T channels last, dweight fp32, dbias fp32) of group_norm_act_fwd; dy of any layout (copied to channels last if it is not)."""
-    with _same_device(dy, x, stats, weight, bias):
-        x, dy = x.detach(), dy.detach().to(x.dtype)
-        lay_y = channels_last_rows(dy)
+    dev, on = _on_device(dy, x, stats, weight, bias)
+    with on:
+        x, dy = x.detach(), dy.detach()
+        lay = channels_last_rows(x)
+        if dy.dtype != x.dtype:
+            dy = dy.to(x.dtype)
+        lay_y = lay if dy.stride() == x.stride() else channels_last_rows(dy)
         if lay_y is None:
             dy = _channels_last_like(x).copy_(dy)
             lay_y = channels_last_rows(dy)
-        N, P, sx, px = channels_last_rows(x)
-        Cc, G, w, b = x.shape[1], stats.shape[1], _f32c(weight), _f32c(bias)
-        dx = _channels_last_like(x)
-        dw, db = torch.empty(2, Cc, dtype=torch.float32, device=x.device)
-        L = lib()
-        ws = torch.empty(L.lsam_group_norm_act_ws_bytes(N, P, Cc, G, 1), dtype=torch.uint8, device=x.device)
-        check(L.lsam_group_norm_act_bwd(dtype_code(x.dtype), ptr(dy), lay_y[2], lay_y[3], ptr(x), sx, px, ptr(w), ptr(b), ptr(stats), N, P, Cc,
-                                        G, ACTIVATIONS[act], ptr(dx), ptr(dw), ptr(db), ptr(ws), ws.numel(), stream()))
+        N, P, sx, px = lay
+        Cc, G, w, b, L = x.shape[1], stats.shape[1], _f32c(weight), _f32c(bias), lib()
+        dx = _channels_last_like(x, lay)
+        dw, db = torch.empty((2, Cc), dtype=torch.float32, device=x.device).unbind()
+        nws = L.lsam_group_norm_act_ws_bytes(N, P, Cc, G, 1)
+        ws = torch.empty(nws, dtype=torch.uint8, device=x.device)
+        check(L.lsam_group_norm_act_bwd(dtype_code(x.dtype), dy.data_ptr(), lay_y[2], lay_y[3], x.data_ptr(), sx, px, ptr(w), ptr(b),
+                                        stats.data_ptr(), N, P, Cc, G, ACTIVATIONS[act], dx.data_ptr(), dw.data_ptr(), db.data_ptr(),
+                                        ws.data_ptr(), nws, stream_of(dev)))
     return dx, dw, db
 
 
 # ---- global norm of a list of tensors, clipping (csrc/grad_clip.hip) ---------------------------------------------------------
-_PTR, _NUMEL, _DEV, _CONTIG = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous
+_PTR, _NUMEL, _DEV, _CONTIG, _SIZE = (torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous,
+                                      torch.Tensor.size)
 _KIND = {torch.float32: 0, torch.bfloat16: 1}
 
 
 def clip_grads(src: Sequence[torch.Tensor], dst: Sequence[torch.Tensor], max_norm: float, inf_norm: bool = False, scale: float = 1.0):
     """fp32 [2] (norm, factor): the global norm of `scale * src` and dst_i = factor * src_i with factor = scale * min(1, max_norm /
-    (norm + 1e-6)); contiguous fp32 / bf16 tensors on one GPU, dst may be src.  One pass over the list costs a few attribute reads a
-    tensor on the host, no device memory but the chunk sums."""
+    (norm + 1e-6)); contiguous fp32 / bf16 tensors on one GPU, dst may be src."""
+    if not (all(map(_CONTIG, src)) and (dst is src or all(map(_CONTIG, dst)))):
+        raise _C.LsamError("clip_grads: the tensors must be contiguous")
+    if dst is not src and list(map(_SIZE, src)) != list(map(_SIZE, dst)):
+        raise _C.LsamError("clip_grads: src and dst differ in number or shape")
+    return _clip_grads(src, dst, max_norm, inf_norm, scale)
+
+
+def _clip_grads(src, dst, max_norm, inf_norm, scale):
+    """clip_grads for lists whose layout and shapes are known to fit.  The host's part is a few attribute reads a tensor; with hundreds
+    of tensors it is as long as the kernels, so it reads nothing twice."""
     if not src:
         raise _C.LsamError("clip_grads: no tensors")
-    devs = set(map(_DEV, src)) | set(map(_DEV, dst))
+    place = dst is src
+    devs = set(map(_DEV, src))
+    if not place:
+        devs.update(map(_DEV, dst))
     if len(devs) != 1 or -1 in devs:
         raise _C.LsamError("clip_grads: the tensors must be on one MI355X (there is no CPU fallback)")
-    place = dst is src
     n = array("q", map(_NUMEL, src))
     try:
-        ks = bytes([_KIND[t.dtype] for t in src])
+        ks = [_KIND[t.dtype] for t in src]
         kinds = bytes([3 * k for k in ks]) if place else bytes([a + 2 * _KIND[b.dtype] for a, b in zip(ks, dst)])
     except KeyError as e:
         raise _C.LsamError(f"clip_grads: unsupported type {e.args[0]}; float32 and bfloat16 are") from None
-    if not (all(map(_CONTIG, src)) and (place or all(map(_CONTIG, dst)))):
-        raise _C.LsamError("clip_grads: the tensors must be contiguous")
-    if not place and (len(dst) != len(src) or array("q", map(_NUMEL, dst)) != n):
-        raise _C.LsamError("clip_grads: src and dst differ in number or size")
-    with torch.cuda.device(src[0].device):
+    dev, device = devs.pop(), src[0].device
+    with _HERE if torch.cuda.current_device() == dev else torch.cuda.device(dev):
         sp = array("Q", map(_PTR, src))
         dp = sp if place else array("Q", map(_PTR, dst))
         L, na = lib(), n.buffer_info()[0]
-        out = torch.empty(2, dtype=torch.float32, device=src[0].device)
-        ws = torch.empty(L.lsam_clip_grads_ws_bytes(na, len(src)) // 8, dtype=torch.float64, device=src[0].device)
-        check(L.lsam_clip_grads(sp.buffer_info()[0], dp.buffer_info()[0], na, kinds, len(src), max_norm, int(inf_norm), scale, ptr(out), ptr(ws),
-                                ws.numel() * 8, stream()))
-    torch.autograd.graph.increment_version(dst)
+        out = torch.empty(2, dtype=torch.float32, device=device)
+        nws = L.lsam_clip_grads_ws_bytes(na, len(src))
+        ws = torch.empty(nws, dtype=torch.uint8, device=device)
+        check(L.lsam_clip_grads(sp.buffer_info()[0], dp.buffer_info()[0], na, kinds, len(src), max_norm, int(inf_norm), scale, out.data_ptr(),
+                                ws.data_ptr(), nws, stream_of(dev)))
+    if not place or scale != 1.0 or max_norm != math.inf:
+        torch.autograd.graph.increment_version(dst)
     return out

@@ -3,7 +3,8 @@
 //
 // Memory-bound: one read for the norm, then a read and a write where anything changes (in place with c = 1 the second pass ends at
 // once).  The list travels by value in the kernels' arguments, so a call needs no device table and can be captured; tensors are cut
-// into chunks and a workgroup takes one chunk.  Squares are summed in fp64 (free beside the loads): neither 1e-30 nor 1e30 leaves the
+// into chunks and a workgroup takes one chunk.  Squares are summed in fp64 (free beside the loads: 136 us for
+// 212 M bf16 values against 133 in fp32): neither 1e-30 nor 1e30 leaves the
 // range, and the norm does not depend on how the list is cut beyond the last bit of an fp64 sum.  Chunk sums are joined in a fixed
 // order: same bits every time.
 #include <algorithm>
@@ -181,10 +182,11 @@ __global__ __launch_bounds__(NT) void clip_scale_kernel(const Table t, const dou
 
 constexpr long ENTRY = 1l << 30;   // elements an entry of the table may have
 
-// elements a chunk: about 2048 workgroups, 2 Ki to 32 Ki elements
+// elements a chunk: about 2048 workgroups, 2 Ki to 16 Ki elements.  212 M bf16 values into fp32: both passes 396 us with 16 Ki, 431 with
+// 32 Ki, 470 with 64 Ki
 int chunk_of(long total) {
     int c = 2048;
-    while (c < 32768 && total / c > 2048) c *= 2;
+    while (c < 16384 && total / c > 2048) c *= 2;
     return c;
 }
 long chunks_of(const long long* n, int count, int chunk) {

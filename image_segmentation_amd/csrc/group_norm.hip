@@ -48,11 +48,27 @@ template <typename T, int V> __device__ __forceinline__ void store(T* p, const f
 }
 
 __device__ __forceinline__ float sigmoid(float h) { return __builtin_amdgcn_rcpf(1.f + __expf(-h)); }
-// EXACT: erff, for fp32 results; else the rational form (|error| < 1.5e-7), whose exponential the derivative shares
+// Phi(h), the normal distribution's, and e = exp(-h^2 / 2) by the way.  EXACT: erff, for fp32 results; else Abramowitz & Stegun 7.1.26
+// (|error| < 1.5e-7), a polynomial in t = 1 / (1 + p |x|), x = h / sqrt 2, times that same exponential: half the instructions, and a map's
+// pass with GELU is bound by them.
+template <bool EXACT> __device__ __forceinline__ float phi(float h, float& e) {
+    e = __builtin_amdgcn_exp2f(h * h * -0.72134752044448170f);
+    if constexpr (EXACT) return 0.5f * (1.f + erff(h * 0.70710678118654752f));
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.23164189f, fabsf(h), 1.f));
+    float y = fmaf(0.5307027145f, t, -0.7265760135f);   // half of 7.1.26's coefficients
+    y = fmaf(y, t, 0.7107068705f);
+    y = fmaf(y, t, -0.142248368f);
+    y = fmaf(y, t, 0.127414796f);
+    y = y * t * e;
+    return h < 0.f ? y : 1.f - y;
+}
 template <bool EXACT> __device__ __forceinline__ float act_fwd(int act, float h) {
     if (act == LSAM_ACT_RELU) return h < 0.f ? 0.f : h;
     if (act == LSAM_ACT_SILU) return h * sigmoid(h);
-    if (act == LSAM_ACT_GELU) return 0.5f * h * (1.f + (EXACT ? erff(h * 0.70710678118654752f) : erf_fast(h * 0.70710678118654752f)));
+    if (act == LSAM_ACT_GELU) {
+        float e;
+        return h * phi<EXACT>(h, e);
+    }
     return h;
 }
 template <bool EXACT> __device__ __forceinline__ float act_slope(int act, float h) {
@@ -61,7 +77,11 @@ template <bool EXACT> __device__ __forceinline__ float act_slope(int act, float 
         const float q = sigmoid(h);
         return q * fmaf(h, 1.f - q, 1.f);
     }
-    if (act == LSAM_ACT_GELU) return gelu_grad_t<!EXACT>(h);
+    if (act == LSAM_ACT_GELU) {
+        float e;
+        const float f = phi<EXACT>(h, e);
+        return fmaf(0.39894228040143268f * h, e, f);
+    }
     return 1.f;
 }
 
@@ -97,10 +117,10 @@ struct GnArgs {
     const float *gamma, *beta;     // or null: 1, 0
     int N, P, C, G, act, splits, rows;   // rows: pixels a split
     float eps;
-    float* part;                   // fwd: [N][splits][G][2] (mean, M2); bwd: [N][splits][C][2] (sum dh, sum dh xhat)
+    float* part;                   // fwd: [N][splits][G][2] (mean, M2); bwd: [N][splits][C][2] (sum dh, sum dh (x - mean))
     float* stats;                  // [N][G][2] mean, rstd
-    float* chan;                   // bwd: [N][C][2] the sums over the splits
-    float* coef;                   // bwd: [N][G][2] S1 / m, S2 / m
+    float* chan;                   // bwd: [N][C][2] the sums over the splits, the second one times rstd: sum dh xhat
+    float* coef;                   // bwd: [N][G][2] rstd S1 / m, rstd^2 S2 / m
     void* out;                     // [N][P][C]
     float *dgamma, *dbeta;
 };
@@ -167,28 +187,66 @@ __global__ __launch_bounds__(NT) void gn_stats_kernel(const GnArgs p) {
     }
     __syncthreads();
     const int cpg = p.C / p.G;
-    for (int g = tid >> 6; g < p.G; g += NT / 64) {
-        float mean, m2, count;
-        join(cpg, lane, [&](int i, float& c, float& m, float& q) { c = (float)cnt; m = cm[g * cpg + i]; q = cq[g * cpg + i]; }, mean, m2, count);
-        if (lane == 0) {
+    auto put = [&](int g, float mean, float m2) {
+        if (p.splits == 1) {   // the whole sample: done
+            p.stats[((size_t)n * p.G + g) * 2] = mean;
+            p.stats[((size_t)n * p.G + g) * 2 + 1] = 1.f / sqrtf(m2 / ((float)cnt * (float)cpg) + p.eps);
+        } else {
             float* o = p.part + ((size_t)blockIdx.x * p.G + g) * 2;
             o[0] = mean;
             o[1] = m2;
         }
+    };
+    if (cpg <= 32) {   // a thread a group; a wave a group, one after another, costs more than the range's loads (16 x 64 x 64 x 256: 19 us)
+        for (int g = tid; g < p.G; g += NT) {
+            float mean = 0.f, m2 = 0.f;
+            for (int c = 0; c < cpg; ++c) mean += cm[g * cpg + c];
+            mean /= (float)cpg;
+            for (int c = 0; c < cpg; ++c) {
+                const float d = cm[g * cpg + c] - mean;
+                m2 += fmaf((float)cnt * d, d, cq[g * cpg + c]);
+            }
+            put(g, mean, m2);
+        }
+    } else {
+        for (int g = tid >> 6; g < p.G; g += NT / 64) {
+            float mean, m2, count;
+            join(cpg, lane, [&](int i, float& c, float& m, float& q) { c = (float)cnt; m = cm[g * cpg + i]; q = cq[g * cpg + i]; }, mean, m2, count);
+            if (lane == 0) put(g, mean, m2);
+        }
     }
 }
 
-// what a thread needs of its channels
+// a wave a (sample, group): joins its ranges
+__global__ __launch_bounds__(NT) void gn_join_kernel(const GnArgs p) {
+    const int id = blockIdx.x * (NT / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (id >= p.N * p.G) return;
+    const int n = id / p.G, g = id - n * p.G;
+    const float cpg = (float)(p.C / p.G);
+    float mean, m2, count;
+    join(p.splits, lane, [&](int i, float& c, float& m, float& q) {
+        const float* o = p.part + ((size_t)(n * p.splits + i) * p.G + g) * 2;
+        c = (float)(min(p.P, (i + 1) * p.rows) - i * p.rows) * cpg;
+        m = o[0];
+        q = o[1];
+    }, mean, m2, count);
+    if (lane == 0) {
+        p.stats[2 * (size_t)id] = mean;
+        p.stats[2 * (size_t)id + 1] = 1.f / sqrtf(m2 / count + p.eps);
+    }
+}
+
+// what a thread needs of its channels: h = (x - mean) slope + beta, slope = rstd gamma
 template <int V> struct Chan {
-    float mean[V], rstd[V], gamma[V], beta[V];
-    __device__ __forceinline__ void get(const GnArgs& p, const float* st, int c0) {
+    float mean[V], slope[V], beta[V];
+    __device__ __forceinline__ void get(const GnArgs& p, int n, int c0) {
+        const float* st = p.stats + (size_t)n * p.G * 2;
         const int cpg = p.C / p.G;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int g = (c0 + j) / cpg;
             mean[j] = st[2 * g];
-            rstd[j] = st[2 * g + 1];
-            gamma[j] = p.gamma ? p.gamma[c0 + j] : 1.f;
+            slope[j] = st[2 * g + 1] * (p.gamma ? p.gamma[c0 + j] : 1.f);
             beta[j] = p.beta ? p.beta[c0 + j] : 0.f;
         }
     }
@@ -196,45 +254,23 @@ template <int V> struct Chan {
 
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(NT) void gn_apply_kernel(const GnArgs p) {
-    extern __shared__ float sm[];   // [G][2]
     const Lay l(p.C, V);
-    const int tid = threadIdx.x, tx = tid % l.cw, ty = tid / l.cw, lane = tid & 63;
+    const int tid = threadIdx.x, tx = tid % l.cw, ty = tid / l.cw;
     const int n = blockIdx.x / p.splits, sp = blockIdx.x - n * p.splits;
-    const int p0 = sp * p.rows, p1 = min(p.P, p0 + p.rows), cpg = p.C / p.G;
-    for (int g = tid >> 6; g < p.G; g += NT / 64) {
-        float mean, m2, count;
-        join(p.splits, lane, [&](int i, float& c, float& m, float& q) {
-            const float* o = p.part + ((size_t)(n * p.splits + i) * p.G + g) * 2;
-            c = (float)(min(p.P, (i + 1) * p.rows) - i * p.rows) * (float)cpg;
-            m = o[0];
-            q = o[1];
-        }, mean, m2, count);
-        if (lane == 0) {
-            const float rstd = 1.f / sqrtf(m2 / count + p.eps);
-            sm[2 * g] = mean;
-            sm[2 * g + 1] = rstd;
-            if (sp == 0 && p.stats) {
-                p.stats[((size_t)n * p.G + g) * 2] = mean;
-                p.stats[((size_t)n * p.G + g) * 2 + 1] = rstd;
-            }
-        }
-    }
-    __syncthreads();
+    const int p0 = sp * p.rows, p1 = min(p.P, p0 + p.rows);
     const T* x = static_cast<const T*>(p.x) + n * p.sx;
     T* y = static_cast<T*>(p.out) + (size_t)n * p.P * p.C;
     for (int b = 0; b < l.blocks; ++b) {
         const int col = b * l.cw + tx;
         if (ty >= l.rw || col >= l.cols) continue;
         Chan<V> ch;
-        ch.get(p, sm, col * V);
-#pragma unroll
-        for (int j = 0; j < V; ++j) ch.gamma[j] *= ch.rstd[j];
+        ch.get(p, n, col * V);
 #pragma unroll 4
         for (int i = p0 + ty; i < p1; i += l.rw) {
             float v[V];
             load<T, V>(x + (long)i * p.px + col * V, v);
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = act_fwd<sizeof(T) == 4>(ACT, fmaf(v[j] - ch.mean[j], ch.gamma[j], ch.beta[j]));
+            for (int j = 0; j < V; ++j) v[j] = act_fwd<sizeof(T) == 4>(ACT, fmaf(v[j] - ch.mean[j], ch.slope[j], ch.beta[j]));
             store<T, V>(y + (size_t)i * p.C + col * V, v);
         }
     }
@@ -257,7 +293,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_sums_kernel(const GnArgs p) {
         for (int j = 0; j < V; ++j) a[j] = c[j] = 0.f;
         if (ty < l.rw && col < l.cols) {
             Chan<V> ch;
-            ch.get(p, p.stats + (size_t)n * p.G * 2, col * V);
+            ch.get(p, n, col * V);
 #pragma unroll 2
             for (int i = p0 + ty; i < p1; i += l.rw) {
                 float v[V], d[V];
@@ -265,10 +301,10 @@ __global__ __launch_bounds__(NT) void gn_bwd_sums_kernel(const GnArgs p) {
                 load<T, V>(dy + (long)i * p.py + col * V, d);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const float xh = (v[j] - ch.mean[j]) * ch.rstd[j];
-                    const float dh = d[j] * act_slope<sizeof(T) == 4>(ACT, fmaf(xh, ch.gamma[j], ch.beta[j]));
+                    const float u = v[j] - ch.mean[j];
+                    const float dh = d[j] * act_slope<sizeof(T) == 4>(ACT, fmaf(u, ch.slope[j], ch.beta[j]));
                     a[j] += dh;
-                    c[j] = fmaf(dh, xh, c[j]);
+                    c[j] = fmaf(dh, u, c[j]);
                 }
             }
         }
@@ -298,6 +334,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_sums_kernel(const GnArgs p) {
 __global__ __launch_bounds__(NT) void gn_bwd_join_kernel(const GnArgs p) {
     __shared__ float r1[NT / 64], r2[NT / 64];
     const int n = blockIdx.x / p.G, g = blockIdx.x - n * p.G, cpg = p.C / p.G, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const float rstd = p.stats[2 * (size_t)blockIdx.x + 1];
     float s1 = 0.f, s2 = 0.f;
     for (int c = wave; c < cpg; c += NT / 64) {   // a wave a channel, lanes over the ranges
         const int ch = g * cpg + c;
@@ -308,7 +345,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_join_kernel(const GnArgs p) {
             b += o[1];
         }
         a = wave_sum(a);
-        b = wave_sum(b);
+        b = wave_sum(b) * rstd;
         if (lane == 0) {
             p.chan[((size_t)n * p.C + ch) * 2] = a;
             p.chan[((size_t)n * p.C + ch) * 2 + 1] = b;
@@ -323,8 +360,8 @@ __global__ __launch_bounds__(NT) void gn_bwd_join_kernel(const GnArgs p) {
         float a = 0.f, b = 0.f;
         for (int w = 0; w < NT / 64; ++w) { a += r1[w]; b += r2[w]; }
         const float m = (float)p.P * (float)cpg;
-        p.coef[2 * blockIdx.x] = a / m;
-        p.coef[2 * blockIdx.x + 1] = b / m;
+        p.coef[2 * (size_t)blockIdx.x] = rstd * a / m;
+        p.coef[2 * (size_t)blockIdx.x + 1] = rstd * rstd * b / m;
     }
 }
 
@@ -355,7 +392,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(const GnArgs p) {
         const int col = b * l.cw + tx;
         if (ty >= l.rw || col >= l.cols) continue;
         Chan<V> ch;
-        ch.get(p, p.stats + (size_t)n * p.G * 2, col * V);
+        ch.get(p, n, col * V);
         float c1[V], c2[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -370,43 +407,53 @@ __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(const GnArgs p) {
             load<T, V>(dy + (long)i * p.py + col * V, d);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float xh = (v[j] - ch.mean[j]) * ch.rstd[j];
-                const float dg = d[j] * act_slope<sizeof(T) == 4>(ACT, fmaf(xh, ch.gamma[j], ch.beta[j])) * ch.gamma[j];
-                v[j] = ch.rstd[j] * (dg - fmaf(xh, c2[j], c1[j]));
+                const float u = v[j] - ch.mean[j];
+                const float dh = d[j] * act_slope<sizeof(T) == 4>(ACT, fmaf(u, ch.slope[j], ch.beta[j]));
+                v[j] = fmaf(dh, ch.slope[j], -fmaf(u, c2[j], c1[j]));
             }
             store<T, V>(dx + (size_t)i * p.C + col * V, v);
         }
     }
 }
 
-// pixels a range: enough ranges for four workgroups a compute unit, at least eight pixels a thread where there are that many
-void ranges(GnArgs& p, int V) {
+// pixels a range: enough ranges for `wgs` workgroups a compute unit, at least eight pixels a thread where there are that many
+void ranges(GnArgs& p, int V, int wgs) {
     const Lay l(p.C, V);
-    int s = (4 * 256 + p.N - 1) / p.N;
+    int s = (wgs * 256 + p.N - 1) / p.N;
     const int most = cdiv(p.P, l.rw * 8);
     if (s > most) s = most;
     if (s < 1) s = 1;
     p.rows = cdiv(cdiv(p.P, s), l.rw) * l.rw;
     p.splits = cdiv(p.P, p.rows);
 }
+// measured on 16 x 256 x 256 x 256 bf16, GELU: the statistics 128 us with 4, 155 with 8, 169 with 2; normalising 241 us with 4, 224 with
+// 8; the backward's sums 286 and 279, its dx 350 and 336
+constexpr int WG_STATS = 4, WG_REST = 8;
 int vec_of(int esz, const GnArgs& p, bool with_dy) {
     const int V = 16 / esz;
     const bool ok = p.C % V == 0 && p.px % V == 0 && p.sx % V == 0 && aligned16(p.x) && (!p.out || aligned16(p.out)) &&
                     (!with_dy || (p.py % V == 0 && p.sy % V == 0 && aligned16(p.dy)));
     return ok ? V : 1;
 }
-template <typename T, int V> int run_fwd(const GnArgs& p, hipStream_t s) {
+template <typename T, int V> int run_fwd(GnArgs& p, hipStream_t s) {
+    ranges(p, V, WG_STATS);
     gn_stats_kernel<T, V><<<p.N * p.splits, NT, (2 * p.C + 2 * NT * V) * sizeof(float), s>>>(p);
     LSAM_LAUNCH_CHECK();
+    if (p.splits > 1) {
+        gn_join_kernel<<<cdiv(p.N * p.G, NT / 64), NT, 0, s>>>(p);
+        LSAM_LAUNCH_CHECK();
+    }
+    ranges(p, V, WG_REST);
     auto k = p.act == LSAM_ACT_RELU   ? gn_apply_kernel<T, V, LSAM_ACT_RELU>
              : p.act == LSAM_ACT_SILU ? gn_apply_kernel<T, V, LSAM_ACT_SILU>
              : p.act == LSAM_ACT_GELU ? gn_apply_kernel<T, V, LSAM_ACT_GELU>
                                       : gn_apply_kernel<T, V, LSAM_ACT_NONE>;
-    k<<<p.N * p.splits, NT, 2 * p.G * sizeof(float), s>>>(p);
+    k<<<p.N * p.splits, NT, 0, s>>>(p);
     LSAM_LAUNCH_CHECK();
     return LSAM_OK;
 }
-template <typename T, int V> int run_bwd(const GnArgs& p, hipStream_t s) {
+template <typename T, int V> int run_bwd(GnArgs& p, hipStream_t s) {
+    ranges(p, V, WG_REST);
     auto k = p.act == LSAM_ACT_RELU   ? gn_bwd_sums_kernel<T, V, LSAM_ACT_RELU>
              : p.act == LSAM_ACT_SILU ? gn_bwd_sums_kernel<T, V, LSAM_ACT_SILU>
              : p.act == LSAM_ACT_GELU ? gn_bwd_sums_kernel<T, V, LSAM_ACT_GELU>
@@ -435,19 +482,13 @@ int gn_check(int N, int P, int C, int G, int act, long sx, long px) {
 }
 }  // namespace
 
-// the most that either layout needs
+// what ranges() may come to in any layout: at most 2048 / N + 1 ranges a sample, and P / 8 of them
 size_t gn_ws_bytes(int N, int P, int C, int G, int backward) {
-    size_t most = 0;
-    for (int V : {1, 4, 8}) {
-        if (C % V) continue;
-        GnArgs p{};
-        p.N = N > 0 ? N : 1; p.P = P > 0 ? P : 1; p.C = C;
-        ranges(p, V);
-        const size_t n = backward ? ((size_t)p.N * p.splits * C * 2 + (size_t)p.N * C * 2 + (size_t)p.N * G * 2) * sizeof(float)
-                                  : (size_t)p.N * p.splits * G * 2 * sizeof(float);
-        if (n > most) most = n;
-    }
-    return most;
+    const size_t n = N > 0 ? N : 1;
+    size_t split_rows = n + WG_REST * 256;
+    const size_t most = n * (size_t)(P > 0 ? cdiv(P, 8) : 1);
+    if (split_rows > most) split_rows = most;
+    return (backward ? split_rows * C * 2 + n * C * 2 + n * G * 2 : split_rows * G * 2 + n * G * 2) * sizeof(float);
 }
 
 template <typename T>
@@ -459,9 +500,10 @@ int launch_group_norm_act_fwd(const void* x, long sx, long px, const float* gamm
     LSAM_REQUIRE(ws_bytes >= gn_ws_bytes(N, P, C, G, 0), LSAM_ERR_WORKSPACE, "group_norm_act: workspace too small");
     GnArgs p{};
     p.x = x; p.sx = sx; p.px = px; p.gamma = gamma; p.beta = beta; p.N = N; p.P = P; p.C = C; p.G = G; p.act = act; p.eps = eps;
-    p.part = static_cast<float*>(ws); p.stats = stats; p.out = y;
+    p.stats = stats ? stats : static_cast<float*>(ws);
+    p.part = static_cast<float*>(ws) + (size_t)N * G * 2;
+    p.out = y;
     const int V = vec_of(sizeof(T), p, false);
-    ranges(p, V);
     return V > 1 ? run_fwd<T, 16 / sizeof(T)>(p, s) : run_fwd<T, 1>(p, s);
 }
 
@@ -489,7 +531,6 @@ int launch_group_norm_act_bwd(const void* dy, long sy, long py, const void* x, l
     }
     LSAM_REQUIRE(x && dy && dx && stats, LSAM_ERR_BAD_ARG, "group_norm_act: null operand");
     const int V = vec_of(sizeof(T), p, true);
-    ranges(p, V);
     return V > 1 ? run_bwd<T, 16 / sizeof(T)>(p, s) : run_bwd<T, 1>(p, s);
 }
 #define GN_INST(T)                                                                                                                              \

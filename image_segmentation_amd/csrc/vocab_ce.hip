@@ -486,7 +486,8 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
 #endif
 }
 // ---------------------------------------------------------------------------------------------------------------------
-// Row selection: the rows whose target is not ignored, in order.  One workgroup; 8 rows a thread and step.
+// Row selection: the rows whose target is not ignored, in order.  A workgroup takes 8192 rows; with more than one, a first launch counts
+// each one's rows and the second adds up those in front of its own.
 // ---------------------------------------------------------------------------------------------------------------------
 struct CeState {   // what the forward leaves for the backward
     int* n;        // rows that count
@@ -498,48 +499,72 @@ struct CeState {   // what the forward leaves for the backward
     char* xc;      // T [M][Dp] compact rows, columns padded with zeros
 };
 
+constexpr int ROWS_WG = 8192;
+
+__global__ __launch_bounds__(1024) void ce_count_kernel(const long long* __restrict__ target, int M, long long ignore, int* __restrict__ counts) {
+    __shared__ int wsum[16];
+    const int tid = threadIdx.x, b = blockIdx.x * ROWS_WG;
+    int cnt = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int m = b + j * 1024 + tid;
+        cnt += __popcll(__ballot(m < M && target[m < M ? m : M - 1] != ignore));
+    }
+    if ((tid & 63) == 0) wsum[tid >> 6] = cnt;
+    __syncthreads();
+    if (tid == 0) {
+        int s = 0;
+        for (int w = 0; w < 16; ++w) s += wsum[w];
+        counts[blockIdx.x] = s;
+    }
+}
+
 __global__ __launch_bounds__(1024) void ce_rows_kernel(const long long* __restrict__ target, int M, int V, long long ignore, CeState st,
-                                                       float* __restrict__ loss_none) {
-    __shared__ int wsum[16], total;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int base = 0;
-    for (int m0 = 0; m0 < M; m0 += 8192) {
-        const int b = m0 + tid * 8;
-        long long t[8];
-        int cnt = 0;
+                                                       const int* __restrict__ counts, float* __restrict__ loss_none) {
+    __shared__ int part[8][16], front[8 * 16], before;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x * ROWS_WG;
+    if (wave == 0) {   // rows that count in front of this workgroup's
+        int s = 0;
+        for (int i = lane; i < (int)blockIdx.x; i += 64) s += counts[i];
+        for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+        if (lane == 0) before = s;
+    }
+    long long t[8];
+    unsigned long long mask[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            t[j] = b + j < M ? target[b + j] : ignore;
-            cnt += b + j < M && t[j] != ignore;
-        }
-        int inc = cnt;
-#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int m = b + j * 1024 + tid;
+        t[j] = m < M ? target[m] : ignore;
+        mask[j] = __ballot(t[j] != ignore);
+        if (lane == 0) part[j][wave] = __popcll(mask[j]);
+    }
+    __syncthreads();
+    if (wave == 0) {   // exclusive sums over the 128 groups of 64 rows
+        const int a = (&part[0][0])[2 * lane], c = (&part[0][0])[2 * lane + 1];
+        int inc = a + c;
         for (int o = 1; o < 64; o <<= 1) {
             const int v = __shfl_up(inc, o);
             if (lane >= o) inc += v;
         }
-        if (lane == 63) wsum[wave] = inc;
-        __syncthreads();
-        int before = 0;
-        for (int w = 0; w < 16; ++w) before += w < wave ? wsum[w] : 0;
-        int r = base + before + inc - cnt;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (b + j >= M) break;
-            if (t[j] != ignore) {
-                st.idx[r] = b + j;
-                st.tgt[r] = t[j] >= 0 && t[j] < V ? (int)t[j] : ROW_BAD;
-                st.pos[b + j] = r++;
-            } else {
-                st.pos[b + j] = -1;
-                if (loss_none) loss_none[b + j] = 0.f;
-            }
-        }
-        if (tid == 1023) total = before + inc;
-        __syncthreads();
-        base += total;
+        front[2 * lane] = inc - a - c;
+        front[2 * lane + 1] = inc - c;
+        if (lane == 63 && blockIdx.x == gridDim.x - 1) *st.n = before + inc;
     }
-    if (tid == 0) *st.n = base;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int m = b + j * 1024 + tid;
+        if (m >= M) continue;
+        if (t[j] != ignore) {
+            const int r = before + front[j * 16 + wave] + __popcll(mask[j] & ((1ull << lane) - 1));
+            st.idx[r] = m;
+            st.tgt[r] = t[j] >= 0 && t[j] < V ? (int)t[j] : ROW_BAD;
+            st.pos[m] = r;
+        } else {
+            st.pos[m] = -1;
+            if (loss_none) loss_none[m] = 0.f;
+        }
+    }
 }
 
 // rows of `src` (through idx, or all of them) to [rows][Dp], columns D.. filled with zeros
@@ -675,6 +700,7 @@ __global__ __launch_bounds__(256) void ce_db_kernel(const float* __restrict__ db
     const int v = blockIdx.x * 256 + threadIdx.x, tiles = (*np + rows_tile - 1) / rows_tile;
     if (v >= V) return;
     float s = 0.f;
+#pragma unroll 8
     for (int t = 0; t < tiles; ++t) s += dbp[(size_t)t * ld + v];
     db[v] = tiles ? s * *factor : 0.f;
 }
@@ -764,7 +790,7 @@ template <typename T> struct CePlan {
         if (st) *st = s;
         return c.used;
     }
-    struct Fwd { char* wp; float *part, *zt, *row_loss; };
+    struct Fwd { char* wp; float *part, *zt, *row_loss; int* counts; };
     size_t fwd(char* base, Fwd* f, bool smooth) const {
         Carve c{base};
         Fwd w;
@@ -772,6 +798,7 @@ template <typename T> struct CePlan {
         w.part = c.take<float>((size_t)tiles_v * M * (smooth ? 3 : 2));
         w.zt = c.take<float>(M);
         w.row_loss = c.take<float>(M);
+        w.counts = c.take<int>(M / ROWS_WG + 1);
         if (f) *f = w;
         return c.used;
     }
@@ -855,7 +882,12 @@ int launch_linear_ce_fwd(const void* x, long ldx, const void* w, long ldw, const
     typename CePlan<T>::Fwd f;
     pl.state(static_cast<char*>(state), &st);
     LSAM_REQUIRE(pl.fwd(static_cast<char*>(ws), &f, smooth != 0.f) <= ws_bytes, LSAM_ERR_WORKSPACE, "linear_ce: workspace too small");
-    ce_rows_kernel<<<1, 1024, 0, s>>>(target, M, V, ignore, st, reduction == LSAM_REDUCE_NONE ? loss : nullptr);
+    const int wgs = M > 0 ? cdiv(M, ROWS_WG) : 1;
+    if (wgs > 1) {
+        ce_count_kernel<<<wgs, 1024, 0, s>>>(target, M, ignore, f.counts);
+        LSAM_LAUNCH_CHECK();
+    }
+    ce_rows_kernel<<<wgs, 1024, 0, s>>>(target, M, V, ignore, st, f.counts, reduction == LSAM_REDUCE_NONE ? loss : nullptr);
     LSAM_LAUNCH_CHECK();
     if (M > 0) {
         LSAM_TRY(gather<T>(x, ldx, st.idx, st.n, M, D, pl.Dp, st.xc, s));

@@ -23,6 +23,12 @@ def _f32(g: torch.Tensor) -> torch.Tensor:
     return ops.add_rows(g.view(-1, g.shape[-1]), None, torch.float32).view(g.shape)
 
 
+def _once(name: str):
+    """Backward passes of this module are not differentiable themselves; under create_graph=True their results would pass for constants."""
+    if torch.is_grad_enabled():
+        raise ops._C.LsamError(f"{name}: a second derivative (create_graph=True) is not built")
+
+
 def _as(g32: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     if dtype == torch.float32:
         return g32
@@ -256,12 +262,14 @@ class LinearCrossEntropyFn(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        _once("linear_cross_entropy")
         weight, bias, state = ctx.saved_tensors
         M, label_smoothing, reduction = ctx.cfg
         dx, dw, db = ops.linear_ce_bwd(g, state, weight, bias, M, label_smoothing, reduction, ctx.needs_input_grad[:3])
-        return dx, dw, db if db is None else db.to(bias.dtype), None, None, None, None
+        if db is not None and bias.dtype != torch.float32:
+            db = db.to(bias.dtype)
+        return dx, dw, db, None, None, None, None
 
 
 class GroupNormActFn(torch.autograd.Function):
@@ -277,9 +285,13 @@ class GroupNormActFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        _once("group_norm_act")
         x, stats, weight, bias = ctx.saved_tensors
         dx, dw, db = ops.group_norm_act_bwd(g, x, stats, weight, bias, ctx.act)
-        need = ctx.needs_input_grad
-        return (dx if need[0] else None, dw.to(weight.dtype) if need[1] else None, db.to(bias.dtype) if need[2] else None, None, None, None)
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        if need_w and weight.dtype != torch.float32:
+            dw = dw.to(weight.dtype)
+        if need_b and bias.dtype != torch.float32:
+            db = db.to(bias.dtype)
+        return dx if need_x else None, dw if need_w else None, db if need_b else None, None, None, None

@@ -215,6 +215,9 @@ def test_same_bits_stream_graph():
 
 
 def test_refusals():
+    l = torch.zeros(2, 8, 3, 3, device="cuda").requires_grad_(True)
+    with pytest.raises(LsamError, match="second derivative"):
+        torch.autograd.grad(group_norm_act(l, 2).sum(), l, create_graph=True)
     x = torch.zeros(2, 8, 3, 3, device="cuda").contiguous(memory_format=torch.channels_last)
     w = torch.ones(8, device="cuda")
     for args, kw in (((x, 3), {}), ((x, 0), {}), ((x.half(), 2), {}), ((x[0, 0, 0], 1), {}), ((x, 2, w[:4]), {}), ((x, 2, w.long()), {}),

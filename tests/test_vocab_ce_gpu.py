@@ -138,6 +138,21 @@ def test_rows_that_count(dtype, kind):
     assert (grads[1].double() - ref[1].double()).abs().max() <= 2.0 ** -7 * ref[1].abs().max()
 
 
+@pytest.mark.parametrize("M", [8191, 8192, 8193, 30000])
+def test_many_rows(M):
+    # rows of several selecting workgroups, whole ones of them ignored
+    x, w, t, b, g = make(M, 24, 60, torch.float32, True, M, ignored=0.5)
+    t[8000:16500] = -100
+    check(x, w, t, b, g, 0.0, "none")
+
+
+def test_second_derivative_is_refused():
+    x, w, t, b, g = make(20, 8, 30, torch.float32, False, 3)
+    x.requires_grad_(True)
+    with pytest.raises(LsamError, match="second derivative"):
+        torch.autograd.grad(linear_cross_entropy(x, w, t), x, create_graph=True)
+
+
 def test_no_rows():
     x = torch.zeros(0, 16, device="cuda", requires_grad=True)
     w = torch.randn(40, 16, device="cuda", requires_grad=True)

@@ -123,6 +123,8 @@ struct GnArgs {
     float* coef;                   // bwd: [N][G][2] rstd S1 / m, rstd^2 S2 / m
     void* out;                     // [N][P][C]
     float *dgamma, *dbeta;
+    int cb;                        // one-pass kernels: channels a workgroup
+    bool keep;                     // fwd: stats are the caller's, not workspace
 };
 
 // per-range statistics.  A thread takes its first pixel as the pivot of its channels: sums of (x - pivot) and their squares cannot
@@ -365,20 +367,24 @@ __global__ __launch_bounds__(NT) void gn_bwd_join_kernel(const GnArgs p) {
     }
 }
 
+__device__ __forceinline__ void params(const GnArgs& p, int c) {   // dgamma, dbeta of channel c: the samples' sums, in their order
+    if (c >= p.C) return;
+    float a = 0.f, b = 0.f;
+#pragma unroll 4
+    for (int n = 0; n < p.N; ++n) {
+        a += p.chan[((size_t)n * p.C + c) * 2];
+        b += p.chan[((size_t)n * p.C + c) * 2 + 1];
+    }
+    if (p.dbeta) p.dbeta[c] = a;
+    if (p.dgamma) p.dgamma[c] = b;
+}
+__global__ __launch_bounds__(NT) void gn_params_kernel(const GnArgs p) { params(p, blockIdx.x * NT + threadIdx.x); }
+
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(const GnArgs p) {
     const int tid = threadIdx.x;
-    if ((int)blockIdx.x >= p.N * p.splits) {   // the workgroups behind the maps': dgamma, dbeta
-        const int c = ((int)blockIdx.x - p.N * p.splits) * NT + tid;
-        if (c < p.C) {
-            float a = 0.f, b = 0.f;
-            for (int n = 0; n < p.N; ++n) {
-                a += p.chan[((size_t)n * p.C + c) * 2];
-                b += p.chan[((size_t)n * p.C + c) * 2 + 1];
-            }
-            if (p.dbeta) p.dbeta[c] = a;
-            if (p.dgamma) p.dgamma[c] = b;
-        }
+    if ((int)blockIdx.x >= p.N * p.splits) {   // the workgroups behind the maps'
+        params(p, ((int)blockIdx.x - p.N * p.splits) * NT + tid);
         return;
     }
     const Lay l(p.C, V);
@@ -416,6 +422,213 @@ __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(const GnArgs p) {
     }
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// One pass: where a sample's pixels times a block of whole groups fit a workgroup's registers (1024 threads x UMAX pieces), x (and dy)
+// are read once, the sums go through LDS, and the result is formed from the registers.  One launch where the passes above take three:
+// these sizes are bound by launches, not by bytes.  Neighbouring blocks of a sample, which share cache lines, run on one XCD.
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int ST = 1024;
+
+// column sums of a[rows][cols] into a[0][*]: halving, a fixed order
+__device__ __forceinline__ void fold(float* a, int rows, int cols) {
+    for (int n = rows; n > 1;) {
+        const int h = (n + 1) / 2;
+        for (int i = threadIdx.x; i < (n - h) * cols; i += ST) a[i] += a[i + h * cols];
+        __syncthreads();
+        n = h;
+    }
+}
+
+template <typename T, int V> struct Piece { using type = uint4; };
+template <> struct Piece<float, 1> { using type = float; };
+template <> struct Piece<bf16, 1> { using type = bf16; };
+template <typename T, int V> __device__ __forceinline__ void widen(const typename Piece<T, V>::type& r, float (&v)[V]) {
+    T e[V];
+    __builtin_memcpy(e, &r, sizeof(e));
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = to_f(e[j]);
+}
+
+template <typename T, int V, int UMAX, int ACT> __global__ __launch_bounds__(ST) void gn_one_fwd_kernel(const GnArgs p) {
+    extern __shared__ float sm[];   // [rw][cb] sums, then [cb / cpg][2] mean, rstd
+    using R = typename Piece<T, V>::type;
+    const int cw = p.cb / V, rw = ST / cw, tid = threadIdx.x, tx = tid % cw, ty = tid / cw, cpg = p.C / p.G, gb = p.cb / cpg;
+    const int rows = min(rw, p.P);   // thread rows that have a pixel
+    const int blocks = p.C / p.cb, id = xcd_remap(blockIdx.x, gridDim.x), n = id / blocks, c0 = (id - n * blocks) * p.cb;
+    float* grp = sm + ST * V;
+    const T* x = static_cast<const T*>(p.x) + n * p.sx + c0 + tx * V;
+    const int mine = ty < rw && ty < p.P ? (p.P - ty + rw - 1) / rw : 0;
+    R r[UMAX];
+#pragma unroll
+    for (int u = 0; u < UMAX; ++u)
+        if (u < mine) r[u] = *reinterpret_cast<const R*>(x + (long)(ty + u * rw) * p.px);
+    float s[V], m[V], v[V];
+    auto total = [&](auto f) {   // sum of f over this thread's pixels, a channel each, and over the workgroup's
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[j] = 0.f;
+#pragma unroll
+        for (int u = 0; u < UMAX; ++u)
+            if (u < mine) {
+                widen<T, V>(r[u], v);
+#pragma unroll
+                for (int j = 0; j < V; ++j) s[j] += f(v[j], j);
+            }
+        if (ty < rows) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) sm[tid * V + j] = s[j];
+        }
+        __syncthreads();
+        fold(sm, rows, p.cb);
+    };
+    const float cnt = (float)p.P * (float)cpg;
+    total([](float a, int) { return a; });
+    for (int g = tid; g < gb; g += ST) {
+        float a = 0.f;
+        for (int c = 0; c < cpg; ++c) a += sm[g * cpg + c];
+        grp[2 * g] = a / cnt;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < V; ++j) m[j] = grp[2 * ((tx * V + j) / cpg)];
+    total([&](float a, int j) { return (a - m[j]) * (a - m[j]); });
+    for (int g = tid; g < gb; g += ST) {
+        float a = 0.f;
+        for (int c = 0; c < cpg; ++c) a += sm[g * cpg + c];
+        const float rstd = 1.f / sqrtf(a / cnt + p.eps);
+        grp[2 * g + 1] = rstd;
+        if (p.stats) {
+            float* o = p.stats + ((size_t)n * p.G + c0 / cpg + g) * 2;
+            o[0] = grp[2 * g];
+            o[1] = rstd;
+        }
+    }
+    __syncthreads();
+    if (!mine) return;
+    float sl[V], be[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c = tx * V + j;
+        sl[j] = grp[2 * (c / cpg) + 1] * (p.gamma ? p.gamma[c0 + c] : 1.f);
+        be[j] = p.beta ? p.beta[c0 + c] : 0.f;
+    }
+    T* y = static_cast<T*>(p.out) + (size_t)n * p.P * p.C + c0 + tx * V;
+#pragma unroll
+    for (int u = 0; u < UMAX; ++u)
+        if (u < mine) {
+            widen<T, V>(r[u], v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = act_fwd<sizeof(T) == 4>(ACT, fmaf(v[j] - m[j], sl[j], be[j]));
+            store<T, V>(y + (size_t)(ty + u * rw) * p.C, v);
+        }
+}
+
+template <typename T, int V, int UMAX, int ACT> __global__ __launch_bounds__(ST) void gn_one_bwd_kernel(const GnArgs p) {
+    extern __shared__ float sm[];   // [rw][cb] sums of dh, then of dh (x - mean); [cb] the first ones' result; [cb / cpg][2] coefficients
+    using R = typename Piece<T, V>::type;
+    const int cw = p.cb / V, rw = ST / cw, tid = threadIdx.x, tx = tid % cw, ty = tid / cw, cpg = p.C / p.G, gb = p.cb / cpg;
+    const int rows = min(rw, p.P);   // thread rows that have a pixel
+    const int blocks = p.C / p.cb, id = xcd_remap(blockIdx.x, gridDim.x), n = id / blocks, c0 = (id - n * blocks) * p.cb;
+    float *sa = sm + ST * V, *grp = sa + p.cb;
+    const T* x = static_cast<const T*>(p.x) + n * p.sx + c0 + tx * V;
+    const T* dy = static_cast<const T*>(p.dy) + n * p.sy + c0 + tx * V;
+    const int mine = ty < rw && ty < p.P ? (p.P - ty + rw - 1) / rw : 0;
+    R r[UMAX], q[UMAX];
+#pragma unroll
+    for (int u = 0; u < UMAX; ++u)
+        if (u < mine) {
+            r[u] = *reinterpret_cast<const R*>(x + (long)(ty + u * rw) * p.px);
+            q[u] = *reinterpret_cast<const R*>(dy + (long)(ty + u * rw) * p.py);
+        }
+    Chan<V> ch;
+    ch.get(p, n, c0 + tx * V);
+    float a[V], b[V], v[V], d[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) a[j] = b[j] = 0.f;
+#pragma unroll
+    for (int u = 0; u < UMAX; ++u)
+        if (u < mine) {
+            widen<T, V>(r[u], v);
+            widen<T, V>(q[u], d);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float w = v[j] - ch.mean[j];
+                const float dh = d[j] * act_slope<sizeof(T) == 4>(ACT, fmaf(w, ch.slope[j], ch.beta[j]));
+                a[j] += dh;
+                b[j] = fmaf(dh, w, b[j]);
+            }
+        }
+    if (ty < rows) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) sm[tid * V + j] = a[j];
+    }
+    __syncthreads();
+    fold(sm, rows, p.cb);
+    for (int c = tid; c < p.cb; c += ST) sa[c] = sm[c];
+    __syncthreads();
+    if (ty < rows) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) sm[tid * V + j] = b[j];
+    }
+    __syncthreads();
+    fold(sm, rows, p.cb);
+    const float m = (float)p.P * (float)cpg;
+    for (int g = tid; g < gb; g += ST) {
+        const float rstd = p.stats[((size_t)n * p.G + c0 / cpg + g) * 2 + 1];
+        float s1 = 0.f, s2 = 0.f;
+        for (int i = 0; i < cpg; ++i) {
+            const int c = g * cpg + i;
+            const float gm = p.gamma ? p.gamma[c0 + c] : 1.f, t = sm[c] * rstd;
+            s1 = fmaf(gm, sa[c], s1);
+            s2 = fmaf(gm, t, s2);
+            if (p.N == 1) {
+                if (p.dbeta) p.dbeta[c0 + c] = sa[c];
+                if (p.dgamma) p.dgamma[c0 + c] = t;
+            } else {
+                float* o = p.chan + ((size_t)n * p.C + c0 + c) * 2;
+                o[0] = sa[c];
+                o[1] = t;
+            }
+        }
+        grp[2 * g] = rstd * s1 / m;
+        grp[2 * g + 1] = rstd * rstd * s2 / m;
+    }
+    __syncthreads();
+    if (!mine) return;
+    float c1[V], c2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        c1[j] = grp[2 * ((tx * V + j) / cpg)];
+        c2[j] = grp[2 * ((tx * V + j) / cpg) + 1];
+    }
+    T* dx = static_cast<T*>(p.out) + (size_t)n * p.P * p.C + c0 + tx * V;
+#pragma unroll
+    for (int u = 0; u < UMAX; ++u)
+        if (u < mine) {
+            widen<T, V>(r[u], v);
+            widen<T, V>(q[u], d);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float w = v[j] - ch.mean[j];
+                const float dh = d[j] * act_slope<sizeof(T) == 4>(ACT, fmaf(w, ch.slope[j], ch.beta[j]));
+                v[j] = fmaf(dh, ch.slope[j], -fmaf(w, c2[j], c1[j]));
+            }
+            store<T, V>(dx + (size_t)(ty + u * rw) * p.C, v);
+        }
+}
+
+// channels a workgroup of the one-pass kernels, 0 where they do not apply: the fewest whole groups that make whole pieces and 32 bytes of a
+// pixel, or 16 where that is too much for `umax` pieces a thread
+int one_pass(const GnArgs& p, int V, int esz, int umax) {
+    const int cpg = p.C / p.G;
+    for (int least : {32, 16}) {
+        int cb = cpg;
+        while (cb < p.C && (p.C % cb || cb % V || cb * esz < least)) cb += cpg;
+        if (cb % V || cb / V > ST) return 0;
+        if (cdiv(p.P, ST / (cb / V)) <= umax) return cb;
+    }
+    return 0;
+}
+
 // pixels a range: enough ranges for `wgs` workgroups a compute unit, at least eight pixels a thread where there are that many
 void ranges(GnArgs& p, int V, int wgs) {
     const Lay l(p.C, V);
@@ -436,6 +649,18 @@ int vec_of(int esz, const GnArgs& p, bool with_dy) {
     return ok ? V : 1;
 }
 template <typename T, int V> int run_fwd(GnArgs& p, hipStream_t s) {
+    constexpr int UF = V == 8 ? 8 : V > 1 ? 16 : 32;   // what 128 registers hold without spilling
+    p.cb = one_pass(p, V, sizeof(T), UF);
+    if (p.cb) {
+        if (!p.keep) p.stats = nullptr;
+        auto k = p.act == LSAM_ACT_RELU   ? gn_one_fwd_kernel<T, V, UF, LSAM_ACT_RELU>
+                 : p.act == LSAM_ACT_SILU ? gn_one_fwd_kernel<T, V, UF, LSAM_ACT_SILU>
+                 : p.act == LSAM_ACT_GELU ? gn_one_fwd_kernel<T, V, UF, LSAM_ACT_GELU>
+                                          : gn_one_fwd_kernel<T, V, UF, LSAM_ACT_NONE>;
+        k<<<p.N * (p.C / p.cb), ST, (ST * V + 2 * p.cb) * sizeof(float), s>>>(p);
+        LSAM_LAUNCH_CHECK();
+        return LSAM_OK;
+    }
     ranges(p, V, WG_STATS);
     gn_stats_kernel<T, V><<<p.N * p.splits, NT, (2 * p.C + 2 * NT * V) * sizeof(float), s>>>(p);
     LSAM_LAUNCH_CHECK();
@@ -453,6 +678,21 @@ template <typename T, int V> int run_fwd(GnArgs& p, hipStream_t s) {
     return LSAM_OK;
 }
 template <typename T, int V> int run_bwd(GnArgs& p, hipStream_t s) {
+    constexpr int UB = V == 8 ? 4 : V > 1 ? 8 : 32;
+    p.cb = one_pass(p, V, sizeof(T), UB);
+    if (p.cb) {
+        auto k = p.act == LSAM_ACT_RELU   ? gn_one_bwd_kernel<T, V, UB, LSAM_ACT_RELU>
+                 : p.act == LSAM_ACT_SILU ? gn_one_bwd_kernel<T, V, UB, LSAM_ACT_SILU>
+                 : p.act == LSAM_ACT_GELU ? gn_one_bwd_kernel<T, V, UB, LSAM_ACT_GELU>
+                                          : gn_one_bwd_kernel<T, V, UB, LSAM_ACT_NONE>;
+        k<<<p.N * (p.C / p.cb), ST, (ST * V + 3 * p.cb) * sizeof(float), s>>>(p);
+        LSAM_LAUNCH_CHECK();
+        if (p.N > 1 && (p.dgamma || p.dbeta)) {
+            gn_params_kernel<<<cdiv(p.C, NT), NT, 0, s>>>(p);
+            LSAM_LAUNCH_CHECK();
+        }
+        return LSAM_OK;
+    }
     ranges(p, V, WG_REST);
     auto k = p.act == LSAM_ACT_RELU   ? gn_bwd_sums_kernel<T, V, LSAM_ACT_RELU>
              : p.act == LSAM_ACT_SILU ? gn_bwd_sums_kernel<T, V, LSAM_ACT_SILU>
@@ -500,6 +740,7 @@ int launch_group_norm_act_fwd(const void* x, long sx, long px, const float* gamm
     LSAM_REQUIRE(ws_bytes >= gn_ws_bytes(N, P, C, G, 0), LSAM_ERR_WORKSPACE, "group_norm_act: workspace too small");
     GnArgs p{};
     p.x = x; p.sx = sx; p.px = px; p.gamma = gamma; p.beta = beta; p.N = N; p.P = P; p.C = C; p.G = G; p.act = act; p.eps = eps;
+    p.keep = stats != nullptr;
     p.stats = stats ? stats : static_cast<float*>(ws);
     p.part = static_cast<float*>(ws) + (size_t)N * G * 2;
     p.out = y;

@@ -43,86 +43,77 @@ struct CeArgs {
     long dbp_ld;
     int rows_cap;
     // outputs
-    void* out; long ldo;       // DZ, OUT: T; ACC, PART: fp32
+    void* out; long ldo;       // DZ, OUT: bf16; ACC, PART: fp32
     long split_stride;         // elements between the splits' outputs
     int splits, accumulate;
+    long plane_a, plane_b, plane_out;   // fp32 operands: bytes between the three bf16 planes of A, of B and of DZ's output
 };
 
-template <typename T> struct Ce;
-template <> struct Ce<bf16> {
-    static __device__ __forceinline__ void mma(const uint4& a, const uint4& b, f32x4& c) {
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    }
-};
-template <> struct Ce<float> {
-    static __device__ __forceinline__ void mma(const uint4& a, const uint4& b, f32x4& c) {
-        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
-    }
-};
+__device__ __forceinline__ void mma(const uint4& a, const uint4& b, f32x4& c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
 
-// One operand's tile in LDS.  KC: R rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7).  Transposed: 128 / sizeof(T) rows of
-// R * sizeof(T) bytes; bf16 is read with the transposing LDS load (16 lanes take 4 k-rows x 16 columns), whose 8 rows of a half
-// wave must fall on different banks: 32-byte column pair p of row k at p ^ h(k), h = k's bits 0, 1, 3; fp32 is read one dword a lane,
-// 64-byte column group at group ^ bit 2 of k.
+// fp32 operands go through the bf16 matrix pipes as three terms, x = x0 + x1 + x2 exactly: 8 bits of the 24 each, whatever is left being
+// rounded to the nearest 8.  |x1| <= 2^-9 |x|, |x2| <= 2^-18 |x|, so of the nine products the three left out, x1 y2, x2 y1 and x2 y2, come
+// to at most 2^-25 |x y|: half of what rounding one fp32 product costs.  Six bf16 products at 16 times the fp32 instructions' rate; the
+// small ones go first.  (2011 x 252 x 10007 forward and gradient: 416 us with fp32 matrix instructions.)
+constexpr unsigned TERM_A = 2 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 0 << 10, TERM_B = 0 | 2 << 2 | 1 << 4 | 0 << 6 | 1 << 8 | 0 << 10;
+constexpr int TERMS = 6;
+
+// One operand's tile in LDS.  KC: R rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7).  Transposed: 64 rows of R values, read
+// with the transposing LDS load (16 lanes take 4 k-rows x 16 columns), whose 8 rows of a half wave must fall on different banks: 32-byte
+// column pair p of row k at p ^ h(k), h = k's bits 0, 1, 3.
 // DMA instruction q (of NI a wave) fills 1 KB; from one q to the next a lane's source moves by a fixed number of rows, and its chunk
 // within the row stays, so one offset and one first k describe them all.  Rows of a KC tile behind the limit lie behind the
 // descriptor's last byte and read zeros; every other chunk that must not be read gets an offset that does.
-template <typename T, bool KC, int R, int NW> struct Tile {
-    static constexpr int ES = sizeof(T), EPC = 16 / ES, KE = 128 / ES, RB = R * ES;
+constexpr int KE = 64;   // k of a k-tile
+template <bool KC, int R, int NW> struct Tile {
+    static constexpr int RB = R * 2;
     static constexpr int NI = R * 128 / 1024 / NW;          // DMA instructions a wave and stage
     static constexpr int ROWS = KC ? NW * 8 : NW * 1024 / RB;   // rows from one of them to the next
-    static_assert(R * 128 % (1024 * NW) == 0 && (KC || (NW * 1024 % RB == 0 && ROWS % (ES == 2 ? 16 : 8) == 0)), "a lane's chunk stays");
+    static_assert(R * 128 % (1024 * NW) == 0 && (KC || (NW * 1024 % RB == 0 && ROWS % 16 == 0)), "a lane's chunk stays");
     unsigned vo;   // byte offset of this lane's first chunk in the k-tile's slab
     int ke, col;   // its first k; transposed: its first column in the tile
     __device__ __forceinline__ void init(int wave, int lane, long ld) {
         const int b = wave * 1024 + lane * 16;
         if constexpr (KC) {
             const int row = b >> 7, c = ((b >> 4) & 7) ^ (row & 7);
-            vo = (unsigned)((long)row * ld * ES + c * 16);
-            ke = c * EPC;
+            vo = (unsigned)((long)row * ld * 2 + c * 16);
+            ke = c * 8;
             col = 0;
         } else {
-            const int k = b / RB, pos = (b % RB) >> 4;
-            const int c = ES == 2 ? pos ^ (2 * ((k & 3) | (((k >> 3) & 1) << 2))) : pos ^ (4 * ((k >> 2) & 1));
-            vo = (unsigned)((long)k * ld * ES + c * 16);
+            const int k = b / RB, c = ((b % RB) >> 4) ^ (2 * ((k & 3) | (((k >> 3) & 1) << 2)));
+            vo = (unsigned)((long)k * ld * 2 + c * 16);
             ke = k;
-            col = c * EPC;
+            col = c * 8;
         }
     }
     // k-tile slab: KC advances 128 bytes along the rows, transposed KE rows
     static __device__ __forceinline__ const char* slab(const void* base, long ld, int r0, long k0) {
         const char* p = static_cast<const char*>(base);
-        return KC ? p + ((long)r0 * ld + k0) * ES : p + (k0 * ld + r0) * ES;
+        return KC ? p + ((long)r0 * ld + k0) * 2 : p + (k0 * ld + r0) * 2;
     }
-    static __device__ __forceinline__ long step(long ld) { return KC ? 128 : KE * ld * ES; }
+    static __device__ __forceinline__ long step(long ld) { return KC ? 128 : KE * ld * 2; }
     // DMA instruction q of a k-tile of which `left` k and `rows` rows (columns, transposed) exist
     __device__ __forceinline__ void issue(const char* slab_p, char* dst, int wave, int left, int q, long ld, int rows) const {
-        const int bytes = KC ? rows * (int)ld * ES : 0x7FFFFFFF;
+        const int bytes = KC ? rows * (int)ld * 2 : 0x7FFFFFFF;
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(slab_p), 0, bytes, 0x00020000);
         unsigned vo = this->vo;
         asm volatile("" : "+v"(vo));   // the NI offsets are not held across the loop
         const bool ok = KC ? ke < left : ke < left - q * ROWS && col < rows;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_p)(dst + (wave + NW * q) * 1024), 16,
-                                                 ok ? vo + (unsigned)(q * ROWS * ES) * (unsigned)ld : 0xFFFFFFFFu, 0, 0, 0);
+                                                 ok ? vo + (unsigned)(q * ROWS * 2) * (unsigned)ld : 0xFFFFFFFFu, 0, 0, 0);
     }
     // the fragment of 16-wide tile t, k-step ks (0, 1): lane (g, lr) holds column 16 t + lr, its share of the step's k
     static __device__ __forceinline__ uint4 read(const char* s, int t, int ks, int g, int lr) {
         if constexpr (KC) return *reinterpret_cast<const uint4*>(s + (t * 16 + lr) * 128 + (((ks * 4 + g) ^ (lr & 7)) << 4));
-        else if constexpr (ES == 2) {
-            using s4 = __attribute__((ext_vector_type(4))) short;
-            using s4p = __attribute__((address_space(3))) s4*;
-            const int h = (lr >> 2) | ((g & 1) << 2);
-            const char* a = s + (ks * 32 + 8 * g + (lr >> 2)) * RB + (lr & 3) * 8 + ((t ^ h) << 5);
-            const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)a), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)(a + 4 * RB));
-            const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, hi);
-            return make_uint4(x.x, x.y, y.x, y.y);
-        } else {
-            const char* a = s + (ks * 16 + 4 * g) * RB + lr * 4 + ((t ^ (g & 1)) << 6);
-            return make_uint4(*reinterpret_cast<const unsigned*>(a), *reinterpret_cast<const unsigned*>(a + RB),
-                              *reinterpret_cast<const unsigned*>(a + 2 * RB), *reinterpret_cast<const unsigned*>(a + 3 * RB));
-        }
+        using s4 = __attribute__((ext_vector_type(4))) short;
+        using s4p = __attribute__((address_space(3))) s4*;
+        const int h = (lr >> 2) | ((g & 1) << 2);
+        const char* a = s + (ks * 32 + 8 * g + (lr >> 2)) * RB + (lr & 3) * 8 + ((t ^ h) << 5);
+        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)a), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)(a + 4 * RB));
+        const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, hi);
+        return make_uint4(x.x, x.y, y.x, y.y);
     }
 };
 
@@ -137,16 +128,16 @@ __device__ __forceinline__ float row16_sum(float x) {   // over the 16 lanes tha
 // The scores' products (short k, long epilogue) are persistent: a workgroup takes every gridDim-th tile, and the DMA runs two k-tiles
 // ahead across the border of two tiles, so that the next tile's operands arrive under this one's epilogue.  Lane (g, lr) of wave (wi, wj) ends up with Out[j][i] at
 // j = j0 + (wj TJ + y) 16 + lr, i = i0 + (wi TI + x) 16 + 4 g + r in register r of accumulator (x, y).
-template <typename T, bool AKC, bool BKC, int MODE, int WI, int WJ, int TI, int TJ>
+// X3: operands of three planes; k runs through the six terms, one after another.
+template <bool X3, bool AKC, bool BKC, int MODE, int WI, int WJ, int TI, int TJ>
 __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p) {
 #if defined(__HIP_DEVICE_COMPILE__)   // the host pass needs the launch stub only, and cannot form the LDS builtins
     constexpr int NW = WI * WJ, IT = WI * TI * 16, JT = WJ * TJ * 16;
-    constexpr int KE = 128 / (int)sizeof(T);
     constexpr bool OPQ = !AKC && !BKC, ROWS_K = MODE == OUT || MODE == PART, SCORES = MODE == STATS || MODE == DZ;
     constexpr bool MORE = SCORES;   // more than one tile a workgroup
     static_assert(64 * NW >= IT && 64 * NW >= JT, "a thread a column and a row of the tile");
-    using TA = Tile<T, AKC, IT, NW>;
-    using TB = Tile<T, BKC, JT, NW>;
+    using TA = Tile<AKC, IT, NW>;
+    using TB = Tile<BKC, JT, NW>;
     // two stages of either operand, each a variable of its own: what the compiler can tell apart it does not make a read wait for
     __shared__ __attribute__((aligned(1024))) char sa0[IT * 128];
     __shared__ __attribute__((aligned(1024))) char sa1[IT * 128];
@@ -175,8 +166,8 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
         t.j0 = t.jt * JT;
         return t;
     };
-    // k-tiles of a tile: an even number, so that every tile begins in the same stage; those behind its share of k read zeros
-    const int kts = max(2, (min(per_split, kt_all) + 1) & ~1);
+    // k-tiles of a term, and of a tile: an even number, so that every tile begins in the same stage; those behind its share of k read zeros
+    const int kpt = max(1, min(per_split, kt_all)), kts = X3 ? TERMS * kpt : (kpt + 1) & ~1;
     int id = xcd_remap(blockIdx.x, gridDim.x);
     if (id >= tiles) return;
     TA ta;
@@ -185,9 +176,15 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
     tb.init(wave, lane, p.ldb);
     constexpr int NP = TA::NI + TB::NI;
     // Where the DMA is: the next k-tile to fetch, `fin` k-tiles into a tile.  It runs on into the workgroup's next tile.
-    struct Slab { const char *pa, *pb; int left, ra, rb; };   // first slabs; k left; rows (columns) of the tile that exist
+    struct Slab { const char *pa, *pb; int left, ra, rb; };   // slabs; k left; rows (columns) of the tile that exist
     Slab f, fnext;
     int fin = 0;
+    const char *ta0 = nullptr, *tb0 = nullptr;   // X3: the tile's first slabs in plane 0, its k, the term and the k-tile in it
+    int tleft = 0, term = 0, tin = 0;
+    auto plane = [&](const char* p, long stride, unsigned seq, int term) __attribute__((always_inline)) {
+        const long w = (seq >> (2 * term)) & 3;
+        return p + (stride & -(w & 1)) + ((2 * stride) & -(w >> 1));
+    };
     auto enter = [&](int id) __attribute__((always_inline)) {
         Slab f;
         const At t = at(id);
@@ -200,14 +197,33 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
         return f;
     };
     auto advance = [&] __attribute__((always_inline)) {
+        // choices by masks: a branch in the k-loop splits the blocks that its registers are planned over, and they spill
         f.pa += TA::step(p.lda);
         f.pb += TB::step(p.ldb);
         f.left -= KE;
-        if constexpr (MORE) {   // by masks: a branch in the k-loop splits the blocks that its registers are planned over, and they spill
+        if constexpr (X3) {
+            const long m = -(long)(++tin == kpt);
+            auto sel = [&](auto a, auto b) { return (decltype(a))(((long)b & m) | ((long)a & ~m)); };
+            term -= (int)m;
+            tin &= ~(int)m;
+            f.pa = sel(f.pa, plane(ta0, p.plane_a, TERM_A, term));
+            f.pb = sel(f.pb, plane(tb0, p.plane_b, TERM_B, term));
+            f.left = sel(f.left, term < TERMS ? tleft : 0);   // behind the last term nothing is fetched
+        }
+        if constexpr (MORE) {
             const long m = -(long)(++fin == kts);
             auto sel = [&](auto a, auto b) { return (decltype(a))(((long)b & m) | ((long)a & ~m)); };
-            f.pa = sel(f.pa, fnext.pa);
-            f.pb = sel(f.pb, fnext.pb);
+            if constexpr (X3) {
+                ta0 = sel(ta0, fnext.pa);
+                tb0 = sel(tb0, fnext.pb);
+                tleft = sel(tleft, fnext.left);
+                term &= ~(int)m;
+                f.pa = sel(f.pa, plane(fnext.pa, p.plane_a, TERM_A, 0));
+                f.pb = sel(f.pb, plane(fnext.pb, p.plane_b, TERM_B, 0));
+            } else {
+                f.pa = sel(f.pa, fnext.pa);
+                f.pb = sel(f.pb, fnext.pb);
+            }
             f.left = sel(f.left, fnext.left);
             f.ra = sel(f.ra, fnext.ra);
             f.rb = sel(f.rb, fnext.rb);
@@ -221,6 +237,13 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
         fnext.left = more ? fnext.left : 0;   // no such tile: nothing is fetched
     };
     f = enter(id);
+    if constexpr (X3) {
+        ta0 = f.pa;
+        tb0 = f.pb;
+        tleft = f.left;
+        f.pa = plane(ta0, p.plane_a, TERM_A, 0);
+        f.pb = plane(tb0, p.plane_b, TERM_B, 0);
+    }
     follow(id + gridDim.x);
     auto issue = [&](const Slab& t, char* sa, char* sb, int q) __attribute__((always_inline)) {   // DMA instruction q
         if (q < TA::NI) ta.issue(t.pa, sa, wave, t.left, q, p.lda, t.ra);
@@ -242,7 +265,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
 #pragma unroll
         for (int x = 0; x < TI; ++x) {
 #pragma unroll
-            for (int y = 0; y < TJ; ++y) Ce<T>::mma(a[x], bc[y], acc[x][y]);
+            for (int y = 0; y < TJ; ++y) mma(a[x], bc[y], acc[x][y]);
             if (meet && x == 0) {
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
@@ -406,7 +429,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
                     if (p.smooth_z != 0.f) p.part[2 * plane + o] = zs;
                 }
             } else {
-                T* out = static_cast<T*>(p.out);
+                bf16* out = static_cast<bf16*>(p.out);
 #pragma unroll
                 for (int y = 0; y < TJ; ++y) {
                     const int c = (wj * TJ + y) * 16 + lr_e, m = j0 + c;
@@ -423,13 +446,22 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
 #pragma unroll
                             for (int r = 0; r < 4; ++r) acc[x][y][r] -= 16 * x + r == t ? w * p.keep : 0.f;
                     }
-                    T* rowp = out + (size_t)(ok ? m : 0) * p.ldo + i0 + wi * TI * 16;
-                    if constexpr (sizeof(T) == 2) {
+                    bf16* rowp = out + (size_t)(ok ? m : 0) * p.ldo + i0 + wi * TI * 16;
 #pragma unroll
-                        for (int x = 0; x < TI; x += 2) store_bf16_tile_pair(rowp + 16 * x, g_e, acc[x][y], acc[x + 1][y], ok);
-                    } else if (ok) {
+                    for (int x = 0; x < TI; x += 2) {
+                        store_bf16_tile_pair(rowp + 16 * x, g_e, acc[x][y], acc[x + 1][y], ok);
+                        if constexpr (X3) {
+                            f32x4 u = acc[x][y], v = acc[x + 1][y];
 #pragma unroll
-                        for (int x = 0; x < TI; ++x) store4(rowp + 16 * x + 4 * g_e, acc[x][y]);
+                            for (int q = 1; q < 3; ++q) {
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) {
+                                    u[r] -= (float)(bf16)u[r];
+                                    v[r] -= (float)(bf16)v[r];
+                                }
+                                store_bf16_tile_pair(rowp + q * (p.plane_out / 2) + 16 * x, g_e, u, v, ok);
+                            }
+                        }
                     }
                 }
                 if (p.dbp) {
@@ -457,8 +489,8 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
 #pragma unroll
             for (int y = 0; y < TJ; ++y) {
                 const int j = jb + 16 * y;
-                if constexpr (MODE == OUT && sizeof(T) == 2) {   // every lane takes part in the exchange of a tile pair
-                    T* rowp = static_cast<T*>(p.out) + (size_t)min(j, J - 1) * p.ldo + i0 + wi * TI * 16;
+                if constexpr (MODE == OUT) {   // every lane takes part in the exchange of a tile pair
+                    bf16* rowp = static_cast<bf16*>(p.out) + (size_t)min(j, J - 1) * p.ldo + i0 + wi * TI * 16;
 #pragma unroll
                     for (int x = 0; x < TI; x += 2)
                         store_bf16_tile_pair(rowp + 16 * x, g_e, acc[x][y] * f, acc[x + 1][y] * f, j < J && i0 + (wi * TI + x) * 16 + 8 * g_e < p.I);
@@ -496,7 +528,7 @@ struct CeState {   // what the forward leaves for the backward
     int* tgt;      // [M] compact; ROW_BAD outside [0, V)
     float* base2;  // [M] compact: lse = (base2 + log2(sum)) / log2(e)
     float* sum;
-    char* xc;      // T [M][Dp] compact rows, columns padded with zeros
+    char* xc;      // bf16 [M][Dp] compact rows, columns padded with zeros; fp32: three planes
 };
 
 constexpr int ROWS_WG = 8192;
@@ -567,25 +599,32 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(const long long* __restri
     }
 }
 
-// rows of `src` (through idx, or all of them) to [rows][Dp], columns D.. filled with zeros
+// rows of `src` (through idx, or all of them) to bf16 [rows][Dp], columns D.. filled with zeros; fp32 to three planes, `plane` elements apart
 template <typename T>
 __global__ __launch_bounds__(256) void ce_gather_kernel(const T* __restrict__ src, long ld, const int* __restrict__ idx, const int* __restrict__ n,
-                                                        int rows, int D, int Dp, int vec, T* __restrict__ dst) {
-    constexpr int EPC = 16 / (int)sizeof(T);
-    const int cpr = Dp / EPC, lim = n ? min(rows, *n) : rows;
+                                                        int rows, int D, int Dp, int vec, bf16* __restrict__ dst, long plane) {
+    const int cpr = Dp / 8, lim = n ? min(rows, *n) : rows;
     const long total = (long)lim * cpr;
     for (long id = (long)blockIdx.x * 256 + threadIdx.x; id < total; id += (long)gridDim.x * 256) {
-        const int r = (int)(id / cpr), c = (int)(id - (long)r * cpr) * EPC;
+        const int r = (int)(id / cpr), c = (int)(id - (long)r * cpr) * 8;
         const T* s = src + (idx ? idx[r] : r) * ld + c;
-        uint4 v;
-        if (vec) v = *reinterpret_cast<const uint4*>(s);
+        T e[8];
+        if (vec) __builtin_memcpy(e, __builtin_assume_aligned(s, 16), sizeof(e));
         else {
-            T e[EPC];
 #pragma unroll
-            for (int j = 0; j < EPC; ++j) e[j] = c + j < D ? s[j] : from_f<T>(0.f);
-            __builtin_memcpy(&v, e, 16);
+            for (int j = 0; j < 8; ++j) e[j] = c + j < D ? s[j] : from_f<T>(0.f);
         }
-        *reinterpret_cast<uint4*>(dst + (size_t)r * Dp + c) = v;
+        bf16* o = dst + (size_t)r * Dp + c;
+#pragma unroll
+        for (int q = 0; q < (sizeof(T) == 4 ? 3 : 1); ++q) {
+            bf16x8 v;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = (bf16)e[j];
+                if constexpr (sizeof(T) == 4) e[j] -= (float)v[j];
+            }
+            *reinterpret_cast<bf16x8*>(o + q * plane) = v;
+        }
     }
 }
 
@@ -724,43 +763,41 @@ struct Carve {
 };
 
 // Tiles of 256 x 256 (8 waves of 128 x 64 or 64 x 128, one workgroup a CU) or 128 x 128 (64 x 32, two a CU).  The large one feeds the
-// bf16 matrix pipes from LDS at close to their rate; the small one balances where the large leaves CUs idle.  fp32 takes the small one
-// always: its matrix instructions are 16 times slower, LDS keeps up either way.
-// Rounds of tiles, a small one costed at a quarter of a large one and half as much again.
-inline bool small_tiles(bool fp32, long big, long small) { return fp32 || (big + CU - 1) / CU * 4 > ((small + CU - 1) / CU * 3 + 1) / 2; }
+// matrix pipes from LDS at close to their rate; the small one balances where the large leaves CUs idle.  Rounds of tiles, a small one
+// costed at a quarter of a large one and half as much again.
+inline bool small_tiles(long big, long small) { return (big + CU - 1) / CU * 4 > ((small + CU - 1) / CU * 3 + 1) / 2; }
 
 template <typename T> struct CePlan {
-    static constexpr int EPC = 16 / (int)sizeof(T);
-    static constexpr bool FP32 = sizeof(T) == 4;
+    static constexpr bool X3 = sizeof(T) == 4;
+    static constexpr int ES = X3 ? 6 : 2;   // bytes a value of the operands takes
     int M, D, V, Dp, tile, tiles_v, tiles_m;   // tile: of the scores
     bool pack_w, dx_small, dw_small;
     int piece, s_dx, s_dw;
     CePlan(int M_, int D_, int V_, bool pack) : M(M_), D(D_), V(V_), pack_w(pack) {
-        Dp = (D + EPC - 1) / EPC * EPC;
+        Dp = (D + 7) / 8 * 8;
         const int m = M > 0 ? M : 1;
-        tile = small_tiles(FP32, (long)cdiv(V, 256) * cdiv(m, 256), (long)cdiv(V, 128) * cdiv(m, 128)) ? 128 : 256;
+        tile = small_tiles((long)cdiv(V, 256) * cdiv(m, 256), (long)cdiv(V, 128) * cdiv(m, 128)) ? 128 : 256;
         tiles_v = cdiv(V, tile);
         tiles_m = cdiv(m, tile);
-        const size_t col = (size_t)m * sizeof(T) * 256;
+        const size_t col = (size_t)m * ES * 256;
         size_t pt = DZ_CAP / col;
         if (pt < 1) pt = 1;
         if (pt > 1024) pt = 1024;   // byte offsets within a tile's rows stay within 31 bits
         const int vt = cdiv(V, 256);
         if (pt > (size_t)vt) pt = vt;
         piece = (int)pt * 256;
+        // the other two products: the work of a CU is its rounds of tiles times their share of k
         auto pick = [&](int rows, int k, bool& small, int& cuts) {
             const long big = (long)cdiv(rows, 256) * cdiv(Dp, 256), lit = (long)cdiv(rows, 128) * cdiv(Dp, 128);
             const int sb = splits(big, k, false), sl = splits(lit, k, true);
-            small = small_tiles(FP32, big * sb, lit * sl);
-            // compare the work of a CU: rounds of tiles times their share of k
-            if (!FP32) small = (double)((big * sb + CU - 1) / CU) * 4 / sb > 1.5 * (double)((lit * sl + CU - 1) / CU) / sl;
+            small = (double)((big * sb + CU - 1) / CU) * 4 / sb > 1.5 * (double)((lit * sl + CU - 1) / CU) / sl;
             cuts = small ? sl : sb;
         };
         pick(m, piece, dx_small, s_dx);
         pick(piece, m, dw_small, s_dw);
     }
-    int splits(long tiles, int k, bool small) const {   // cuts of k that keep the CUs busy, at least four k-tiles each
-        const int slots = small ? 2 * CU : CU, most = k * (int)sizeof(T) / 512 > 0 ? k * (int)sizeof(T) / 512 : 1;
+    int splits(long tiles, int k, bool small) const {   // cuts of k that keep the CUs busy, at least four k-tiles (or six terms) each
+        const int slots = small ? 2 * CU : CU, least = X3 ? KE : 4 * KE, most = k / least > 0 ? k / least : 1;
         const long s = tiles >= slots ? 1 : slots / tiles;
         return (int)(s < most ? s : most);
     }
@@ -773,7 +810,7 @@ template <typename T> struct CePlan {
         return splits((long)rt * td, M, false) > 1 ? nv - (vt - rt) * 256 : 0;
     }
     // partial sums, or rows of dW that do not take four columns at a time: through fp32 and the joining kernel
-    bool dw_f32() const { return s_dw > 1 || D % EPC; }
+    bool dw_f32() const { return X3 || s_dw > 1 || D % 8; }
     size_t dw_floats() const {   // the rest's tiles times cuts: at most CU of 65536
         return dw_f32() ? (size_t)s_dw * piece * Dp : piece / 256 * cdiv(Dp, 256) > CU ? (size_t)CU * 65536 : 0;
     }
@@ -786,7 +823,7 @@ template <typename T> struct CePlan {
         s.tgt = c.take<int>(M);
         s.base2 = c.take<float>(M);
         s.sum = c.take<float>(M);
-        s.xc = c.take<char>((size_t)M * Dp * sizeof(T));
+        s.xc = c.take<char>((size_t)M * Dp * ES);
         if (st) *st = s;
         return c.used;
     }
@@ -794,7 +831,7 @@ template <typename T> struct CePlan {
     size_t fwd(char* base, Fwd* f, bool smooth) const {
         Carve c{base};
         Fwd w;
-        w.wp = c.take<char>(pack_w ? (size_t)V * Dp * sizeof(T) : 0);
+        w.wp = c.take<char>(pack_w ? (size_t)V * Dp * ES : 0);
         w.part = c.take<float>((size_t)tiles_v * M * (smooth ? 3 : 2));
         w.zt = c.take<float>(M);
         w.row_loss = c.take<float>(M);
@@ -806,8 +843,8 @@ template <typename T> struct CePlan {
     size_t bwd(char* base, Bwd* f, bool want_dx, bool want_dw, bool want_db) const {
         Carve c{base};
         Bwd w;
-        w.wp = c.take<char>(pack_w ? (size_t)V * Dp * sizeof(T) : 0);
-        w.dz = c.take<char>((size_t)M * piece * sizeof(T));
+        w.wp = c.take<char>(pack_w ? (size_t)V * Dp * ES : 0);
+        w.dz = c.take<char>((size_t)M * piece * ES);
         w.factor = c.take<float>(1);
         w.coef = c.take<float>(M);
         w.coef_s = c.take<float>(M);
@@ -819,35 +856,31 @@ template <typename T> struct CePlan {
     }
 };
 
-template <typename T, bool AKC, bool BKC, int MODE, int WI, int WJ, int TI, int TJ> int ce_gemm_run(const CeArgs& a, int a_cu, hipStream_t s) {
+template <bool X3, bool AKC, bool BKC, int MODE, int WI, int WJ, int TI, int TJ> int ce_gemm_run(const CeArgs& a, int a_cu, hipStream_t s) {
     constexpr int IT = WI * TI * 16, JT = WJ * TJ * 16;
     const long tiles = (long)cdiv(a.I, IT) * cdiv(a.J, JT) * a.splits, most = (long)CU * a_cu;
-    ce_gemm_kernel<T, AKC, BKC, MODE, WI, WJ, TI, TJ><<<(int)(tiles < most || !(MODE == STATS || MODE == DZ) ? tiles : most), 64 * WI * WJ, 0, s>>>(a);
+    ce_gemm_kernel<X3, AKC, BKC, MODE, WI, WJ, TI, TJ><<<(int)(tiles < most || !(MODE == STATS || MODE == DZ) ? tiles : most), 64 * WI * WJ, 0, s>>>(a);
     LSAM_LAUNCH_CHECK();
     return LSAM_OK;
 }
 // wave grids of the large tile: as many fragments of the operand that is cheaper to read.  4096^3: A transposed 64 x 128 waves 1333 TF/s
 // against 1177 with 128 x 64; both transposed 1205 against 1103 the other way round
-template <typename T, bool AKC, bool BKC, int MODE> int ce_gemm(const CeArgs& a, bool small, hipStream_t s) {
-    if constexpr (sizeof(T) == 2) {
-        if (!small) {
-            if constexpr (!AKC && BKC) return ce_gemm_run<T, AKC, BKC, MODE, 4, 2, 4, 8>(a, 1, s);
-            else return ce_gemm_run<T, AKC, BKC, MODE, 2, 4, 8, 4>(a, 1, s);
-        }
-    }
-    return ce_gemm_run<T, AKC, BKC, MODE, 2, 4, 4, 2>(a, 2, s);
+template <bool X3, bool AKC, bool BKC, int MODE> int ce_gemm(const CeArgs& a, bool small, hipStream_t s) {
+    if (small) return ce_gemm_run<X3, AKC, BKC, MODE, 2, 4, 4, 2>(a, 2, s);
+    if constexpr (!AKC && BKC) return ce_gemm_run<X3, AKC, BKC, MODE, 4, 2, 4, 8>(a, 1, s);
+    else return ce_gemm_run<X3, AKC, BKC, MODE, 2, 4, 8, 4>(a, 1, s);
 }
 
-template <typename T> bool rows_direct(const void* p, long ld, int D) {   // rows that 16-byte chunks can be fetched from in place
-    constexpr int EPC = 16 / (int)sizeof(T);
-    return D % EPC == 0 && ld % EPC == 0 && aligned16(p) && ld < (1l << 20);
+template <typename T> bool rows_aligned(const void* p, long ld, int D) { return D % 8 == 0 && ld % (16 / (int)sizeof(T)) == 0 && aligned16(p); }
+template <typename T> bool rows_direct(const void* p, long ld, int D) {   // rows that the DMA can fetch in place
+    return sizeof(T) == 2 && rows_aligned<T>(p, ld, D) && ld < (1l << 20);
 }
 
 template <typename T> int gather(const void* src, long ld, const int* idx, const int* n, int rows, int D, int Dp, void* dst, hipStream_t s) {
-    const long chunks = (long)rows * (Dp / (16 / (int)sizeof(T)));
+    const long chunks = (long)rows * (Dp / 8);
     const long blocks = (chunks + 255) / 256;
     ce_gather_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(static_cast<const T*>(src), ld, idx, n, rows, D, Dp,
-                                                                             rows_direct<T>(src, ld, D), static_cast<T*>(dst));
+                                                                             rows_aligned<T>(src, ld, D), static_cast<bf16*>(dst), (long)rows * Dp);
     LSAM_LAUNCH_CHECK();
     return LSAM_OK;
 }
@@ -873,6 +906,7 @@ template <typename T>
 int launch_linear_ce_fwd(const void* x, long ldx, const void* w, long ldw, const float* bias, const long long* target, int M, int D, int V,
                          long long ignore, float smooth, int reduction, float* loss, void* state, void* ws, size_t ws_bytes, hipStream_t s) {
     LSAM_TRY(ce_check(M, D, V, reduction, smooth));
+    constexpr bool X3 = CePlan<T>::X3;
     const CePlan<T> pl(M, D, V, !rows_direct<T>(w, ldw, D));
     LSAM_REQUIRE((M == 0 || (x && target)) && w && state && ws && (loss || (M == 0 && reduction == LSAM_REDUCE_NONE)), LSAM_ERR_BAD_ARG,
                  "linear_ce: null operand");
@@ -897,7 +931,8 @@ int launch_linear_ce_fwd(const void* x, long ldx, const void* w, long ldw, const
         a.B = st.xc; a.ldb = pl.Dp;
         a.I = V; a.J = M; a.K = pl.Dp; a.n = st.n;
         a.bias = bias; a.tgt = st.tgt; a.smooth_z = smooth; a.part = f.part; a.zt = f.zt; a.rows_cap = M; a.splits = 1;
-        LSAM_TRY((ce_gemm<T, true, true, STATS>(a, pl.tile == 128, s)));
+        a.plane_a = (long)V * pl.Dp * 2; a.plane_b = (long)M * pl.Dp * 2;
+        LSAM_TRY((ce_gemm<X3, true, true, STATS>(a, pl.tile == 128, s)));
     }
     const int blocks = M > 0 ? cdiv(M, 16) : 1;
     if (M > 0 || reduction != LSAM_REDUCE_NONE) {
@@ -915,6 +950,7 @@ template <typename T>
 int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float* gout, int M, int D, int V, float smooth, int reduction,
                          const void* state, void* dx, long lddx, void* dw, long lddw, float* db, void* ws, size_t ws_bytes, hipStream_t s) {
     LSAM_TRY(ce_check(M, D, V, reduction, smooth));
+    constexpr bool X3 = CePlan<T>::X3;
     const CePlan<T> pl(M, D, V, !rows_direct<T>(w, ldw, D));
     LSAM_REQUIRE(w && state && ws && (M == 0 || gout), LSAM_ERR_BAD_ARG, "linear_ce: null operand");
     LSAM_REQUIRE(ldw >= D && (!dx || lddx >= D) && (!dw || lddw >= D) && aligned16(state) && aligned16(ws), LSAM_ERR_BAD_ARG,
@@ -936,37 +972,39 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
         const int nv = V - v0 < pl.piece ? V - v0 : pl.piece;
         if (M > 0) {
             CeArgs a{};
-            a.A = W + (size_t)v0 * lw * sizeof(T); a.lda = lw;
+            a.A = W + (size_t)v0 * lw * 2; a.lda = lw; a.plane_a = (long)V * pl.Dp * 2;
+            a.plane_b = (long)M * pl.Dp * 2; a.plane_out = (long)M * pl.piece * 2;
             a.B = st.xc; a.ldb = pl.Dp;
             a.I = nv; a.J = M; a.K = pl.Dp; a.n = st.n;
             a.bias = bias ? bias + v0 : nullptr; a.tgt = st.tgt; a.i_base = v0;
             a.base2 = st.base2; a.coef = b.coef; a.coef_s = b.coef_s; a.sm = smooth / ((float)V * unit); a.keep = keep / unit;
             a.dbp = db ? b.dbp + v0 : nullptr; a.dbp_ld = V;
             a.out = b.dz; a.ldo = pl.piece; a.splits = 1;
-            LSAM_TRY((ce_gemm<T, true, true, DZ>(a, pl.tile == 128, s)));
+            LSAM_TRY((ce_gemm<X3, true, true, DZ>(a, pl.tile == 128, s)));
         }
         if (dx && M > 0) {
             CeArgs a{};
-            a.A = W + (size_t)v0 * lw * sizeof(T); a.lda = lw;
+            a.A = W + (size_t)v0 * lw * 2; a.lda = lw; a.plane_a = (long)V * pl.Dp * 2; a.plane_b = (long)M * pl.piece * 2;
             a.B = b.dz; a.ldb = pl.piece;
             a.I = pl.Dp; a.J = M; a.K = nv; a.n = st.n;
             a.out = b.dx; a.ldo = pl.Dp; a.split_stride = (long)M * pl.Dp; a.splits = pl.s_dx; a.accumulate = k > 0;
-            LSAM_TRY((ce_gemm<T, false, true, ACC>(a, pl.dx_small, s)));
+            LSAM_TRY((ce_gemm<X3, false, true, ACC>(a, pl.dx_small, s)));
         }
         if (dw) {
             // classes c0 .. c0 + nc of the piece; through fp32 where k is cut or T rows do not take four columns at a time
-            auto weight_grad = [&](int c0, int nc, bool f32, int cuts) -> int {
+            auto weight_grad = [&](int c0, int nc, [[maybe_unused]] bool f32, int cuts) -> int {
                 T* o = static_cast<T*>(dw) + (size_t)(v0 + c0) * lddw;
                 CeArgs a{};
                 a.A = st.xc; a.lda = pl.Dp;
-                a.B = b.dz + (size_t)c0 * sizeof(T); a.ldb = pl.piece;
+                a.B = b.dz + (size_t)c0 * 2; a.ldb = pl.piece; a.plane_a = (long)M * pl.Dp * 2; a.plane_b = (long)M * pl.piece * 2;
                 a.I = pl.Dp; a.J = nc; a.K = M; a.n = st.n; a.splits = cuts;
-                if (!f32) {
-                    a.out = o; a.ldo = lddw; a.factor = b.factor;
-                    return ce_gemm<T, false, false, OUT>(a, pl.dw_small, s);
-                }
+                if constexpr (!X3)
+                    if (!f32) {
+                        a.out = o; a.ldo = lddw; a.factor = b.factor;
+                        return ce_gemm<X3, false, false, OUT>(a, pl.dw_small, s);
+                    }
                 a.out = b.dw; a.ldo = pl.Dp; a.split_stride = (long)nc * pl.Dp;
-                LSAM_TRY((ce_gemm<T, false, false, PART>(a, pl.dw_small, s)));
+                LSAM_TRY((ce_gemm<X3, false, false, PART>(a, pl.dw_small, s)));
                 const long blocks = ((long)nc * (pl.Dp / 4) + 255) / 256;
                 ce_dx_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(b.dw, a.split_stride, cuts, nullptr, nc, D, pl.Dp, D % 4 == 0,
                                                                                      b.factor, o, lddw);

@@ -3,10 +3,11 @@
 //
 // Memory-bound: one read for the norm, then a read and a write where anything changes (in place with c = 1 the second pass ends at
 // once).  The list travels by value in the kernels' arguments, so a call needs no device table and can be captured; tensors are cut
-// into chunks and a workgroup takes one chunk.  Squares are summed in fp64 (free beside the loads: 136 us for
-// 212 M bf16 values against 133 in fp32): neither 1e-30 nor 1e30 leaves the
-// range, and the norm does not depend on how the list is cut beyond the last bit of an fp64 sum.  Chunk sums are joined in a fixed
-// order: same bits every time.
+// into chunks and a workgroup takes one chunk.  Squares are summed in fp64 (free beside the loads: 136 us for 212 M bf16 values against
+// 133 in fp32): neither 1e-30 nor 1e30 leaves the range, and the norm does not depend on how the list is cut beyond the last bit of an
+// fp64 sum.  Chunk sums are joined in a fixed order: same bits every time.
+// 212 M bf16 values clipped into fp32: norm 130 us (3.3 TB/s), joining 6, scaling 260 (4.9 TB/s; a copy: 5.07).  Lists of a few hundred
+// tensors are bound by the host's reading of them: 311 tensors, 69 M fp32 values with c = 1: 121 us, 70 of them the kernels'.
 #include <algorithm>
 #include <vector>
 
@@ -126,7 +127,8 @@ template <bool INF> __device__ __forceinline__ double join_parts(const double* p
     return block_join<INF>(a, red).value();
 }
 
-template <bool INF> __global__ __launch_bounds__(1024) void clip_join_kernel(const double* __restrict__ part, int parts, Limit l, float* __restrict__ out) {
+template <bool INF> __global__ __launch_bounds__(1024) void clip_join_kernel(const double* __restrict__ part, int parts, Limit l,
+                                                                             float* __restrict__ out) {
     __shared__ Acc<INF> red[16];
     const double s = join_parts<INF>(part, parts, red);
     if (threadIdx.x == 0) norm_and_factor(s, INF, l, out[0], out[1]);

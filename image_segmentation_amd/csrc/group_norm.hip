@@ -7,6 +7,10 @@
 // Memory-bound both ways.  A workgroup walks a range of pixels with whole rows of channels: consecutive lanes take consecutive
 // 16-byte pieces of a row, a thread keeps to its channels, so what a channel needs stays in its registers and the sums over pixels
 // need no exchange until the range ends.  Sums over ranges are joined in a fixed order by the next kernel: same bits every time.
+//
+// Two passes each way: 3 reads and writes of the map forward, 5 backward, bound by HBM.  Measured on 16 x 256 x 256 x 256 bf16 with GELU
+// (536 MB a map): statistics 124 us (4.3 TB/s), normalising 228 (4.7), the backward's sums 283 (3.8), its dx 342 (4.7); 900 us with the
+// host's part, where a copy's 5.07 TB/s would allow 847 (plain form 14.3 ms).
 #include "kernels.hpp"
 
 namespace lsam {
@@ -426,6 +430,7 @@ __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(const GnArgs p) {
 // One pass: where a sample's pixels times a block of whole groups fit a workgroup's registers (1024 threads x UMAX pieces), x (and dy)
 // are read once, the sums go through LDS, and the result is formed from the registers.  One launch where the passes above take three:
 // these sizes are bound by launches, not by bytes.  Neighbouring blocks of a sample, which share cache lines, run on one XCD.
+// 16 x 64 x 64 x 256 bf16 forward: 22 us, 33 by the passes above; 4 x 43 x 57 x 105 forward and backward: 141 us either way, the host's.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int ST = 1024;
 
@@ -712,8 +717,8 @@ template <typename T, int V> int run_bwd(GnArgs& p, hipStream_t s) {
 }
 
 int gn_check(int N, int P, int C, int G, int act, long sx, long px) {
-    LSAM_REQUIRE(N >= 0 && P >= 0 && C > 0 && G > 0 && C % G == 0, LSAM_ERR_BAD_ARG, "group_norm_act: %d samples, %d pixels, %d channels in %d groups", N, P,
-                 C, G);
+    LSAM_REQUIRE(N >= 0 && P >= 0 && C > 0 && G > 0 && C % G == 0, LSAM_ERR_BAD_ARG,
+                 "group_norm_act: %d samples, %d pixels, %d channels in %d groups", N, P, C, G);
     LSAM_REQUIRE(C <= MAXC && (long)N * G < (1l << 24) && N < (1 << 20) && P < (1 << 30), LSAM_ERR_UNSUPPORTED,
                  "group_norm_act: %d samples, %d pixels, %d channels, %d groups", N, P, C, G);
     LSAM_REQUIRE(act >= LSAM_ACT_NONE && act <= LSAM_ACT_GELU, LSAM_ERR_BAD_ARG, "group_norm_act: activation %d", act);

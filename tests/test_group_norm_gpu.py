@@ -85,6 +85,23 @@ def test_matches_float64(N, C, H, W, G, act, dtype):
     check(x, dy, w, b, G, act)
 
 
+# maps beyond one workgroup's registers, a range of pixels a workgroup: at most 16 pixels a thread, 64 threads' and 32 channels' sums one after
+# another (or a wave's), which the bounds above cover
+LARGE = [(2, 64, 130, 121, 8), (1, 300, 90, 71, 3), (1, 2056, 31, 33, 8), (3, 24, 97, 113, 24), (1, 7, 260, 250, 7), (1, 256, 100, 80, 1)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act", list(ACTS))
+@pytest.mark.parametrize("N, C, H, W, G", LARGE)
+def test_large_maps_match_float64(N, C, H, W, G, act, dtype):
+    x, dy, w, b = make(N, C, H, W, dtype, N * 1000 + C + H, mean=30.0 if act == "none" else 1.0)
+    check(x, dy, w, b, G, act)
+    if act == "silu":                                         # a channel slice off a vector's alignment; no parameters
+        wide = torch.full((N, H, W, C + 9), float("nan"), dtype=dtype, device="cuda").permute(0, 3, 1, 2)
+        wide[:, 3:3 + C] = x
+        check(wide[:, 3:3 + C], dy, None, None, G, act)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_far_mean_and_constant_groups(dtype):
     # means a thousand times the spread: the statistics are taken around a pixel's own value
@@ -148,9 +165,10 @@ def test_empty():
         assert gx.shape == shape and (gw == 0).all() and (gb == 0).all()
 
 
+@pytest.mark.parametrize("size", [9, 190])
 @pytest.mark.parametrize("act", list(ACTS))
-def test_not_finite_stays_in_its_group(act):
-    x, dy, w, b = make(2, 16, 9, 9, torch.float32, 9)
+def test_not_finite_stays_in_its_group(act, size):
+    x, dy, w, b = make(2, 16, size, size, torch.float32, 9)
     clean = group_norm_act(x, 4, w, b, act=act)
     for bad in (float("nan"), float("inf")):
         z = x.clone()
@@ -181,8 +199,9 @@ def test_gradient_against_differences():
         assert abs(got - ref) <= h * h / 6 * size + 2.0 ** -18 * float(dy.abs().sum()) / h
 
 
-def test_same_bits_stream_graph():
-    x, dy, w, b = make(4, 64, 40, 30, torch.bfloat16, 13)
+@pytest.mark.parametrize("H, W", [(40, 30), (130, 121)])
+def test_same_bits_stream_graph(H, W):
+    x, dy, w, b = make(4, 64, H, W, torch.bfloat16, 13)
 
     def step(leaves, dy):
         y = group_norm_act(leaves[0], 8, leaves[1], leaves[2], act="gelu")
@@ -202,7 +221,7 @@ def test_same_bits_stream_graph():
         with torch.cuda.graph(graph, stream=side):
             out = step(leaves, ds)
     for seed in (17, 19, 23):
-        x2, dy2, w2, b2 = make(4, 64, 40, 30, torch.bfloat16, seed)
+        x2, dy2, w2, b2 = make(4, 64, H, W, torch.bfloat16, seed)
         with torch.no_grad():
             for leaf, v in zip(leaves, (x2, w2, b2)):
                 leaf.copy_(v)

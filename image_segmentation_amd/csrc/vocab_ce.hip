@@ -3,10 +3,16 @@
 //   z = x W^T + b,  lse_m = log sum_v exp z_mv,  loss_m = (1-e)(lse_m - z_mt) + e (lse_m - mean_v z_mv)
 //   dz_mv = c_m (exp(z_mv - lse_m) - (1-e)[v = t_m] - e/V),  dx = dz W,  dW = dz^T x,  db = sum_m dz
 //
-// Forward: every 256-wide tile of z lives in accumulators only; its epilogue leaves one (max, sum of exponentials) pair a row and
-// tile.  Backward: a piece of the classes at a time, z is formed again, dz of the piece goes to a workspace in the operand type T,
-// and two more products read it.  Rows whose target is ignored are taken out first (order kept): they cost nothing, and what they
-// hold (NaN included) reaches no gradient.
+// Forward: every tile of z lives in accumulators only; its epilogue leaves one (base, sum of exponentials) pair a row and tile.
+// Backward: a piece of the classes at a time, z is formed again, dz of the piece goes to a workspace in bf16 (fp32: in three bf16
+// terms, see mma), and two more products read it.  Rows whose target is ignored are taken out first (order kept): they cost nothing,
+// and what they hold (NaN included) reaches no gradient.
+//
+// Bound by the matrix pipes: 2 M D V operations forward, 6 M D V backward, against (M + V) D values read.  With the scores in memory the
+// plain form moves 2 to 4 bytes of each several times over and takes the sum of three library products besides.  Measured, bf16, rows x
+// D x classes, forward and gradients: 16384 x 256 x 32000 in 1.31 ms (plain 10.6; scores 355 us, dz 465, dx 282, dW 242), 8192 x 896 x
+// 50257 in 2.5 ms (plain 19.2; scores 640, dz 695, dx 615, dW 645); forward alone 4096 x 448 x 65536 in 250 us (plain 2940).  The
+// products run at 0.9 to 1.2 PFLOP/s; the scores' and dz's epilogues (an exponential a score) are what D = 256 adds to them.
 #include "kernels.hpp"
 
 namespace lsam {
@@ -22,6 +28,20 @@ constexpr int ROW_BAD = -1;   // target outside [0, V): the row's loss and gradi
 // ---------------------------------------------------------------------------------------------------------------------
 enum Mode { STATS, DZ, ACC, OUT, PART };   // PART: OUT in fp32
 
+// The gradients of the scores are held in units of one number for all rows, `unit` times the incoming gradient (over n), chosen so that
+// what dominates them -- the target's entry of a row that is not learned yet -- is exactly -1 under MEAN and SUM.  Rounded to bf16 at its
+// own size, (1 - e) g / n, that entry would be off by the same fraction in every row, and the fraction would come through the sums
+// whole.  The factor is applied to the fp32 sums; without rows every sum is 0 and stays it, whatever 1 / n is.
+struct Grad {
+    const float* gout;
+    int reduction;
+    float unit;
+    __device__ __forceinline__ float factor(int n) const {
+        if (n == 0) return 0.f;
+        return reduction == LSAM_REDUCE_NONE ? unit : reduction == LSAM_REDUCE_MEAN ? gout[0] * unit / (float)n : gout[0] * unit;
+    }
+};
+
 struct CeArgs {
     const void* A; long lda;   // elements
     const void* B; long ldb;
@@ -34,11 +54,11 @@ struct CeArgs {
     float smooth_z;            // != 0: the sum of z over the classes is wanted too
     float* part;               // STATS: planes [tiles_i][rows_cap] of (base, sum of exponentials, sum of z)
     float* zt;                 // STATS: z of the target
-    const float* base2;        // DZ: the row's base, and its coefficient c and c / (sum of exponentials)
-    const float* coef;
-    const float* coef_s;
+    const float* base2;        // DZ: the row's base and its sum of exponentials
+    const float* sum;
+    const int* idx;
     float sm, keep;            // DZ: the subtrahends of every class and of the target, in units of the row's coefficient
-    const float* factor;       // OUT: what the product is multiplied with
+    Grad grad;                 // DZ, OUT
     float* dbp;                // DZ: [tiles_j][I_cap] partial column sums or null
     long dbp_ld;
     int rows_cap;
@@ -56,7 +76,7 @@ __device__ __forceinline__ void mma(const uint4& a, const uint4& b, f32x4& c) {
 // fp32 operands go through the bf16 matrix pipes as three terms, x = x0 + x1 + x2 exactly: 8 bits of the 24 each, whatever is left being
 // rounded to the nearest 8.  |x1| <= 2^-9 |x|, |x2| <= 2^-18 |x|, so of the nine products the three left out, x1 y2, x2 y1 and x2 y2, come
 // to at most 2^-25 |x y|: half of what rounding one fp32 product costs.  Six bf16 products at 16 times the fp32 instructions' rate; the
-// small ones go first.  (2011 x 252 x 10007 forward and gradient: 416 us with fp32 matrix instructions.)
+// small ones go first.  (2011 x 252 x 10007 forward and gradient: 360 us, 416 with fp32 matrix instructions.)
 constexpr unsigned TERM_A = 2 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 0 << 10, TERM_B = 0 | 2 << 2 | 1 << 4 | 0 << 6 | 1 << 8 | 0 << 10;
 constexpr int TERMS = 6;
 
@@ -126,9 +146,11 @@ __device__ __forceinline__ float row16_sum(float x) {   // over the 16 lanes tha
 }
 
 // The scores' products (short k, long epilogue) are persistent: a workgroup takes every gridDim-th tile, and the DMA runs two k-tiles
-// ahead across the border of two tiles, so that the next tile's operands arrive under this one's epilogue.  Lane (g, lr) of wave (wi, wj) ends up with Out[j][i] at
-// j = j0 + (wj TJ + y) 16 + lr, i = i0 + (wi TI + x) 16 + 4 g + r in register r of accumulator (x, y).
+// ahead across the border of two tiles, so that the next tile's operands arrive under this one's epilogue.  Lane (g, lr) of wave
+// (wi, wj) ends up with Out[j][i] at j = j0 + (wj TJ + y) 16 + lr, i = i0 + (wi TI + x) 16 + 4 g + r in register r of accumulator (x, y).
 // X3: operands of three planes; k runs through the six terms, one after another.
+// A fragment read feeds TJ (TI) products and the barrier stands once a k-tile, so the 256-wide tile waits for the matrix pipes, not for
+// LDS: 4096^3 at 1200 TF/s with both operands stored along k, 1205 with both transposed (library product: 1300).
 template <bool X3, bool AKC, bool BKC, int MODE, int WI, int WJ, int TI, int TJ>
 __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p) {
 #if defined(__HIP_DEVICE_COMPILE__)   // the host pass needs the launch stub only, and cannot form the LDS builtins
@@ -259,7 +281,8 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
     // read of this tile has landed -- the workgroup meets: the other stage is complete, this one is free for the k-tile after next,
     // whose DMA instructions go out between the rows.
     uint4 a[TI], b0[TJ], b1[TJ];
-    auto step = [&](const char* na, const char* nb, int ks, uint4 (&bc)[TJ], uint4 (&bn)[TJ], bool meet, char* fa, char* fb) __attribute__((always_inline)) {
+    auto step = [&](const char* na, const char* nb, int ks, uint4 (&bc)[TJ], uint4 (&bn)[TJ], bool meet, char* fa,
+                    char* fb) __attribute__((always_inline)) {
         // two transposed operands: their addresses are worked out here; held across the loop they spill (4096^3: 816 against 1100 TF/s)
         if (OPQ) asm volatile("" : "+v"(lr_k), "+v"(g_k));
 #pragma unroll
@@ -324,8 +347,8 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
                 row_t = p.tgt[m] - p.i_base;
                 if constexpr (MODE == DZ) {
                     row_base = p.base2[m];
-                    row_w = p.coef[m];
-                    row_s = p.coef_s[m];
+                    row_w = row_t + p.i_base == ROW_BAD ? NAN : p.grad.reduction == LSAM_REDUCE_NONE ? p.grad.gout[p.idx[m]] : 1.f;
+                    row_s = row_w / (p.grad.unit * p.sum[m]);
                 }
             }
         }
@@ -485,7 +508,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
                 }
             }
         } else {
-            const float f = MODE == OUT ? *p.factor : 1.f;
+            const float f = MODE == OUT ? p.grad.factor(n) : 1.f;
 #pragma unroll
             for (int y = 0; y < TJ; ++y) {
                 const int j = jb + 16 * y;
@@ -517,6 +540,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing may land in this workgroup's LDS after it
 #endif
 }
+
 // ---------------------------------------------------------------------------------------------------------------------
 // Row selection: the rows whose target is not ignored, in order.  A workgroup takes 8192 rows; with more than one, a first launch counts
 // each one's rows and the second adds up those in front of its own.
@@ -551,8 +575,45 @@ __global__ __launch_bounds__(1024) void ce_count_kernel(const long long* __restr
     }
 }
 
+// Rows of `src` (through idx, or all of them) to bf16 [rows][Dp], columns D.. filled with zeros; fp32 to three planes, `plane` elements apart.
+template <typename T> struct Gather {
+    const T* src; long ld;
+    const int* idx;
+    int D, Dp, vec;
+    bf16* dst; long plane;
+    __device__ __forceinline__ void run(int rows, long first, long step) const {
+        const int cpr = Dp / 8;
+        for (long id = first; id < (long)rows * cpr; id += step) {
+            const int r = (int)(id / cpr), c = (int)(id - (long)r * cpr) * 8;
+            const T* s = src + (idx ? idx[r] : r) * ld + c;
+            T e[8];
+            if (vec) __builtin_memcpy(e, __builtin_assume_aligned(s, 16), sizeof(e));
+            else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) e[j] = c + j < D ? s[j] : from_f<T>(0.f);
+            }
+            bf16* o = dst + (size_t)r * Dp + c;
+#pragma unroll
+            for (int q = 0; q < (sizeof(T) == 4 ? 3 : 1); ++q) {
+                bf16x8 v;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    v[j] = (bf16)e[j];
+                    if constexpr (sizeof(T) == 4) e[j] -= (float)v[j];
+                }
+                *reinterpret_cast<bf16x8*>(o + q * plane) = v;
+            }
+        }
+    }
+};
+template <typename T> __global__ __launch_bounds__(256) void ce_gather_kernel(const Gather<T> g, const int* __restrict__ n, int rows) {
+    g.run(n ? min(rows, *n) : rows, (long)blockIdx.x * 256 + threadIdx.x, (long)gridDim.x * 256);
+}
+
+// `take`: the one workgroup gathers the rows too
+template <typename T>
 __global__ __launch_bounds__(1024) void ce_rows_kernel(const long long* __restrict__ target, int M, int V, long long ignore, CeState st,
-                                                       const int* __restrict__ counts, float* __restrict__ loss_none) {
+                                                       const int* __restrict__ counts, float* __restrict__ loss_none, int take, const Gather<T> g) {
     __shared__ int part[8][16], front[8 * 16], before;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x * ROWS_WG;
     if (wave == 0) {   // rows that count in front of this workgroup's
@@ -597,34 +658,9 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(const long long* __restri
             if (loss_none) loss_none[m] = 0.f;
         }
     }
-}
-
-// rows of `src` (through idx, or all of them) to bf16 [rows][Dp], columns D.. filled with zeros; fp32 to three planes, `plane` elements apart
-template <typename T>
-__global__ __launch_bounds__(256) void ce_gather_kernel(const T* __restrict__ src, long ld, const int* __restrict__ idx, const int* __restrict__ n,
-                                                        int rows, int D, int Dp, int vec, bf16* __restrict__ dst, long plane) {
-    const int cpr = Dp / 8, lim = n ? min(rows, *n) : rows;
-    const long total = (long)lim * cpr;
-    for (long id = (long)blockIdx.x * 256 + threadIdx.x; id < total; id += (long)gridDim.x * 256) {
-        const int r = (int)(id / cpr), c = (int)(id - (long)r * cpr) * 8;
-        const T* s = src + (idx ? idx[r] : r) * ld + c;
-        T e[8];
-        if (vec) __builtin_memcpy(e, __builtin_assume_aligned(s, 16), sizeof(e));
-        else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) e[j] = c + j < D ? s[j] : from_f<T>(0.f);
-        }
-        bf16* o = dst + (size_t)r * Dp + c;
-#pragma unroll
-        for (int q = 0; q < (sizeof(T) == 4 ? 3 : 1); ++q) {
-            bf16x8 v;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[j] = (bf16)e[j];
-                if constexpr (sizeof(T) == 4) e[j] -= (float)v[j];
-            }
-            *reinterpret_cast<bf16x8*>(o + q * plane) = v;
-        }
+    if (take) {
+        __syncthreads();
+        g.run(before + front[127] + part[7][15], tid, 1024);
     }
 }
 
@@ -695,53 +731,46 @@ __global__ __launch_bounds__(1024) void ce_sum_kernel(const float* __restrict__ 
     if (threadIdx.x == 0) loss[0] = (float)(reduction == LSAM_REDUCE_MEAN ? part[0] / (double)n : part[0]);
 }
 
-// dz is held in T in units of `factor`, one number for all rows, chosen so that what dominates it -- the target's entry of a row that
-// is not learned yet -- is exactly -1 under MEAN and SUM: (1 - e) gout / n.  Rounded to bf16 at its own size that entry would be off by
-// the same fraction in every row, and that fraction would come through the sums whole.  The factor is applied to the fp32 sums.
-__global__ __launch_bounds__(256) void ce_coef_kernel(const float* __restrict__ gout, int reduction, float unit, CeState st, float* __restrict__ coef,
-                                                      float* __restrict__ coef_s, float* __restrict__ factor) {
-    const int r = blockIdx.x * 256 + threadIdx.x, n = *st.n;
-    if (r == 0)   // without rows every sum is 0 and stays it, whatever 1 / n is
-        *factor = n == 0 ? 0.f : reduction == LSAM_REDUCE_NONE ? unit : reduction == LSAM_REDUCE_MEAN ? gout[0] * unit / (float)n : gout[0] * unit;
-    if (r >= n) return;
-    float c = reduction == LSAM_REDUCE_NONE ? gout[st.idx[r]] : 1.f;
-    if (st.tgt[r] == ROW_BAD) c = NAN;
-    coef[r] = c;
-    coef_s[r] = c / (unit * st.sum[r]);
-}
-
-// dx[m] = factor * (sum of the splits' rows), or zeros where the row was ignored
-template <typename T>
-__global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ acc, long stride, int splits, const int* __restrict__ pos, int M, int D,
-                                                    int Dp, int vec, const float* __restrict__ factor,
-                                                    T* __restrict__ dx, long lddx) {
-    const int cpr = Dp / 4;
-    const float f = *factor;
-    for (long id = (long)blockIdx.x * 256 + threadIdx.x; id < (long)M * cpr; id += (long)gridDim.x * 256) {
-        const int m = (int)(id / cpr), c = (int)(id - (long)m * cpr) * 4, r = pos ? pos[m] : m;
-        if (c >= D) continue;
+// out[m] = factor * (sum of the splits' rows), or zeros where the row was ignored.  Workgroups from `first_db` on: the bias gradient, the
+// row tiles' column sums in their order.
+struct Finish {
+    const float* acc; long stride; int splits;
+    const int *pos, *n;
+    int M, D, Dp;
+    Grad grad;
+    void* out; long ldo;
+    int first_db, V, rows_tile;
+    const float* dbp; float* db;
+};
+template <typename T> __global__ __launch_bounds__(256) void ce_finish_kernel(const Finish p) {
+    const int n = *p.n;
+    const float f = p.grad.factor(n);
+    if ((int)blockIdx.x >= p.first_db) {
+        const int v = ((int)blockIdx.x - p.first_db) * 256 + threadIdx.x, tiles = (n + p.rows_tile - 1) / p.rows_tile;
+        if (v >= p.V) return;
+        float s = 0.f;
+#pragma unroll 8
+        for (int t = 0; t < tiles; ++t) s += p.dbp[(size_t)t * p.V + v];
+        p.db[v] = tiles ? s * f : 0.f;
+        return;
+    }
+    const int cpr = p.Dp / 4;
+    for (long id = (long)blockIdx.x * 256 + threadIdx.x; id < (long)p.M * cpr; id += (long)p.first_db * 256) {
+        const int m = (int)(id / cpr), c = (int)(id - (long)m * cpr) * 4, r = p.pos ? p.pos[m] : m;
+        if (c >= p.D) continue;
         f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (r >= 0)
-            for (int s = 0; s < splits; ++s) v += load4(acc + s * stride + (size_t)r * Dp + c);
-        if (r >= 0) v *= f;
-        T* o = dx + (size_t)m * lddx + c;
-        if (vec) store4(o, v);
+        if (r >= 0) {
+            for (int s = 0; s < p.splits; ++s) v += load4(p.acc + s * p.stride + (size_t)r * p.Dp + c);
+            v *= f;
+        }
+        T* o = static_cast<T*>(p.out) + (size_t)m * p.ldo + c;
+        if (p.D % 4 == 0) store4(o, v);
         else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (c + j < D) o[j] = from_f<T>(v[j]);
+                if (c + j < p.D) o[j] = from_f<T>(v[j]);
         }
     }
-}
-
-__global__ __launch_bounds__(256) void ce_db_kernel(const float* __restrict__ dbp, long ld, const int* __restrict__ np, int rows_tile, int V,
-                                                    const float* __restrict__ factor, float* __restrict__ db) {
-    const int v = blockIdx.x * 256 + threadIdx.x, tiles = (*np + rows_tile - 1) / rows_tile;
-    if (v >= V) return;
-    float s = 0.f;
-#pragma unroll 8
-    for (int t = 0; t < tiles; ++t) s += dbp[(size_t)t * ld + v];
-    db[v] = tiles ? s * *factor : 0.f;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -764,8 +793,10 @@ struct Carve {
 
 // Tiles of 256 x 256 (8 waves of 128 x 64 or 64 x 128, one workgroup a CU) or 128 x 128 (64 x 32, two a CU).  The large one feeds the
 // matrix pipes from LDS at close to their rate; the small one balances where the large leaves CUs idle.  Rounds of tiles, a small one
-// costed at a quarter of a large one and half as much again.
-inline bool small_tiles(long big, long small) { return (big + CU - 1) / CU * 4 > ((small + CU - 1) / CU * 3 + 1) / 2; }
+// costed at a quarter of a large one and half as much again (16384 x 256 x 32000 scores: 440 us against 364; weight gradient of
+// 8192 x 896 x 50257: 769 against 644).
+constexpr double SMALL = 1.5;
+inline bool small_tiles(long big, long small) { return (double)((big + CU - 1) / CU) * 4 > SMALL * (double)((small + CU - 1) / CU); }
 
 template <typename T> struct CePlan {
     static constexpr bool X3 = sizeof(T) == 4;
@@ -790,7 +821,7 @@ template <typename T> struct CePlan {
         auto pick = [&](int rows, int k, bool& small, int& cuts) {
             const long big = (long)cdiv(rows, 256) * cdiv(Dp, 256), lit = (long)cdiv(rows, 128) * cdiv(Dp, 128);
             const int sb = splits(big, k, false), sl = splits(lit, k, true);
-            small = (double)((big * sb + CU - 1) / CU) * 4 / sb > 1.5 * (double)((lit * sl + CU - 1) / CU) / sl;
+            small = (double)((big * sb + CU - 1) / CU) * 4 / sb > SMALL * (double)((lit * sl + CU - 1) / CU) / sl;
             cuts = small ? sl : sb;
         };
         pick(m, piece, dx_small, s_dx);
@@ -839,15 +870,12 @@ template <typename T> struct CePlan {
         if (f) *f = w;
         return c.used;
     }
-    struct Bwd { char *wp, *dz; float *factor, *coef, *coef_s, *dx, *dw, *dbp; };
+    struct Bwd { char *wp, *dz; float *dx, *dw, *dbp; };
     size_t bwd(char* base, Bwd* f, bool want_dx, bool want_dw, bool want_db) const {
         Carve c{base};
         Bwd w;
         w.wp = c.take<char>(pack_w ? (size_t)V * Dp * ES : 0);
         w.dz = c.take<char>((size_t)M * piece * ES);
-        w.factor = c.take<float>(1);
-        w.coef = c.take<float>(M);
-        w.coef_s = c.take<float>(M);
         w.dx = c.take<float>(want_dx ? (size_t)s_dx * M * Dp : 0);
         w.dw = c.take<float>(want_dw ? dw_floats() : 0);
         w.dbp = c.take<float>(want_db ? (size_t)tiles_m * V : 0);
@@ -859,7 +887,8 @@ template <typename T> struct CePlan {
 template <bool X3, bool AKC, bool BKC, int MODE, int WI, int WJ, int TI, int TJ> int ce_gemm_run(const CeArgs& a, int a_cu, hipStream_t s) {
     constexpr int IT = WI * TI * 16, JT = WJ * TJ * 16;
     const long tiles = (long)cdiv(a.I, IT) * cdiv(a.J, JT) * a.splits, most = (long)CU * a_cu;
-    ce_gemm_kernel<X3, AKC, BKC, MODE, WI, WJ, TI, TJ><<<(int)(tiles < most || !(MODE == STATS || MODE == DZ) ? tiles : most), 64 * WI * WJ, 0, s>>>(a);
+    const int wgs = (int)(tiles < most || !(MODE == STATS || MODE == DZ) ? tiles : most);
+    ce_gemm_kernel<X3, AKC, BKC, MODE, WI, WJ, TI, TJ><<<wgs, 64 * WI * WJ, 0, s>>>(a);
     LSAM_LAUNCH_CHECK();
     return LSAM_OK;
 }
@@ -876,11 +905,12 @@ template <typename T> bool rows_direct(const void* p, long ld, int D) {   // row
     return sizeof(T) == 2 && rows_aligned<T>(p, ld, D) && ld < (1l << 20);
 }
 
-template <typename T> int gather(const void* src, long ld, const int* idx, const int* n, int rows, int D, int Dp, void* dst, hipStream_t s) {
-    const long chunks = (long)rows * (Dp / 8);
-    const long blocks = (chunks + 255) / 256;
-    ce_gather_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(static_cast<const T*>(src), ld, idx, n, rows, D, Dp,
-                                                                             rows_aligned<T>(src, ld, D), static_cast<bf16*>(dst), (long)rows * Dp);
+template <typename T> Gather<T> gather_of(const void* src, long ld, const int* idx, int rows, int D, int Dp, void* dst) {
+    return {static_cast<const T*>(src), ld, idx, D, Dp, rows_aligned<T>(src, ld, D), static_cast<bf16*>(dst), (long)rows * Dp};
+}
+template <typename T> int gather(const Gather<T>& g, const int* n, int rows, hipStream_t s) {
+    const long blocks = ((long)rows * (g.Dp / 8) + 255) / 256;
+    ce_gather_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(g, n, rows);
     LSAM_LAUNCH_CHECK();
     return LSAM_OK;
 }
@@ -921,11 +951,13 @@ int launch_linear_ce_fwd(const void* x, long ldx, const void* w, long ldw, const
         ce_count_kernel<<<wgs, 1024, 0, s>>>(target, M, ignore, f.counts);
         LSAM_LAUNCH_CHECK();
     }
-    ce_rows_kernel<<<wgs, 1024, 0, s>>>(target, M, V, ignore, st, f.counts, reduction == LSAM_REDUCE_NONE ? loss : nullptr);
+    const Gather<T> gx = gather_of<T>(x, ldx, st.idx, M, D, pl.Dp, st.xc);
+    const bool take = wgs == 1 && (long)M * pl.Dp <= 32768;   // a launch less; a CU copies 64 KB in that time
+    ce_rows_kernel<T><<<wgs, 1024, 0, s>>>(target, M, V, ignore, st, f.counts, reduction == LSAM_REDUCE_NONE ? loss : nullptr, take, gx);
     LSAM_LAUNCH_CHECK();
     if (M > 0) {
-        LSAM_TRY(gather<T>(x, ldx, st.idx, st.n, M, D, pl.Dp, st.xc, s));
-        if (pl.pack_w) LSAM_TRY(gather<T>(w, ldw, nullptr, nullptr, V, D, pl.Dp, f.wp, s));
+        if (!take) LSAM_TRY(gather<T>(gx, st.n, M, s));
+        if (pl.pack_w) LSAM_TRY(gather<T>(gather_of<T>(w, ldw, nullptr, V, D, pl.Dp, f.wp), nullptr, V, s));
         CeArgs a{};
         a.A = pl.pack_w ? f.wp : w; a.lda = pl.pack_w ? pl.Dp : ldw;
         a.B = st.xc; a.ldb = pl.Dp;
@@ -962,12 +994,21 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
     pl.state(static_cast<char*>(const_cast<void*>(state)), &st);
     LSAM_REQUIRE(pl.bwd(static_cast<char*>(ws), &b, dx != nullptr, dw != nullptr, db != nullptr) <= ws_bytes, LSAM_ERR_WORKSPACE,
                  "linear_ce: workspace too small");
-    if (pl.pack_w) LSAM_TRY(gather<T>(w, ldw, nullptr, nullptr, V, D, pl.Dp, b.wp, s));
+    if (pl.pack_w) LSAM_TRY(gather<T>(gather_of<T>(w, ldw, nullptr, V, D, pl.Dp, b.wp), nullptr, V, s));
     const char* W = pl.pack_w ? b.wp : static_cast<const char*>(w);
     const long lw = pl.pack_w ? pl.Dp : ldw;
     const float keep = 1.f - smooth, unit = keep > 0.f ? keep : 1.f;
-    ce_coef_kernel<<<cdiv(M > 0 ? M : 1, 256), 256, 0, s>>>(gout, reduction, unit, st, b.coef, b.coef_s, b.factor);
-    LSAM_LAUNCH_CHECK();
+    const Grad grad{gout, reduction, unit};
+    auto finish = [&](const Finish& p, long values) -> int {
+        const long blocks = (values / 4 + 255) / 256;
+        Finish q = p;
+        q.grad = grad;
+        q.n = st.n;
+        q.first_db = (int)(blocks < 8192 ? blocks : 8192);
+        ce_finish_kernel<T><<<q.first_db + (q.db ? cdiv(V, 256) : 0), 256, 0, s>>>(q);
+        LSAM_LAUNCH_CHECK();
+        return LSAM_OK;
+    };
     for (int v0 = 0, k = 0; v0 < V; v0 += pl.piece, ++k) {
         const int nv = V - v0 < pl.piece ? V - v0 : pl.piece;
         if (M > 0) {
@@ -977,7 +1018,7 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
             a.B = st.xc; a.ldb = pl.Dp;
             a.I = nv; a.J = M; a.K = pl.Dp; a.n = st.n;
             a.bias = bias ? bias + v0 : nullptr; a.tgt = st.tgt; a.i_base = v0;
-            a.base2 = st.base2; a.coef = b.coef; a.coef_s = b.coef_s; a.sm = smooth / ((float)V * unit); a.keep = keep / unit;
+            a.base2 = st.base2; a.sum = st.sum; a.idx = st.idx; a.grad = grad; a.sm = smooth / ((float)V * unit); a.keep = keep / unit;
             a.dbp = db ? b.dbp + v0 : nullptr; a.dbp_ld = V;
             a.out = b.dz; a.ldo = pl.piece; a.splits = 1;
             LSAM_TRY((ce_gemm<X3, true, true, DZ>(a, pl.tile == 128, s)));
@@ -1000,32 +1041,22 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
                 a.I = pl.Dp; a.J = nc; a.K = M; a.n = st.n; a.splits = cuts;
                 if constexpr (!X3)
                     if (!f32) {
-                        a.out = o; a.ldo = lddw; a.factor = b.factor;
+                        a.out = o; a.ldo = lddw; a.grad = grad;
                         return ce_gemm<X3, false, false, OUT>(a, pl.dw_small, s);
                     }
                 a.out = b.dw; a.ldo = pl.Dp; a.split_stride = (long)nc * pl.Dp;
                 LSAM_TRY((ce_gemm<X3, false, false, PART>(a, pl.dw_small, s)));
-                const long blocks = ((long)nc * (pl.Dp / 4) + 255) / 256;
-                ce_dx_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(b.dw, a.split_stride, cuts, nullptr, nc, D, pl.Dp, D % 4 == 0,
-                                                                                     b.factor, o, lddw);
-                LSAM_LAUNCH_CHECK();
-                return LSAM_OK;
+                return finish(Finish{b.dw, a.split_stride, cuts, nullptr, nullptr, nc, D, pl.Dp, {}, o, lddw, 0, 0, 0, nullptr, nullptr},
+                              (long)nc * pl.Dp);
             };
             const int rest = pl.rest(nv);
             LSAM_TRY(weight_grad(0, nv - rest, pl.dw_f32(), pl.s_dw));
             if (rest) LSAM_TRY(weight_grad(nv - rest, rest, true, pl.splits((long)cdiv(rest, 256) * cdiv(pl.Dp, 256), M, false)));
         }
     }
-    if (dx && M > 0) {
-        const long blocks = ((long)M * (pl.Dp / 4) + 255) / 256;
-        ce_dx_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(b.dx, (long)M * pl.Dp, pl.s_dx, st.pos, M, D, pl.Dp,
-                                                                             D % 4 == 0, b.factor, static_cast<T*>(dx), lddx);
-        LSAM_LAUNCH_CHECK();
-    }
-    if (db) {
-        ce_db_kernel<<<cdiv(V, 256), 256, 0, s>>>(b.dbp, V, st.n, pl.tile, V, b.factor, db);
-        LSAM_LAUNCH_CHECK();
-    }
+    if (dx || db)
+        LSAM_TRY(finish(Finish{b.dx, (long)M * pl.Dp, pl.s_dx, st.pos, nullptr, dx ? M : 0, D, pl.Dp, {}, dx, lddx, 0, V, pl.tile, b.dbp, db},
+                        dx ? (long)M * pl.Dp : 0));
     return LSAM_OK;
 }
 #define CE_INST(T)                                                                                                                          \

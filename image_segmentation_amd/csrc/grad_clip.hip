@@ -222,6 +222,7 @@ template <bool INF> int run(const std::vector<Table>& tabs, bool scale, double* 
 }  // namespace
 
 size_t clip_ws_bytes(const long long* n, int count) {
+    if (!n) return sizeof(double);
     const long k = chunks_of(n, count, chunk_of(total_of(n, count)));
     return (size_t)(k > 0 ? k : 1) * sizeof(double);
 }

@@ -34,7 +34,8 @@ def clip_grads_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float
     fp32 / bf16 tensors of any mix on one GPU; `out` may have other types than `grads` (bf16 gradients into fp32 buffers).  norm_type
     2 or inf.  Squares are summed in fp64.  A norm that is not finite makes the factor what torch.nn.utils.clip_grad_norm_ makes it
     (NaN, or 0 for an infinite one); error_if_nonfinite looks at the norm on the host first and raises, with nothing changed.
-    max_norm = inf: the norm alone.  Two tensors that share memory are refused."""
+    max_norm = inf: the norm alone.  Contiguous tensors that share memory are refused where anything would be written, and so are others
+    that begin at one address or repeat their elements (expanded ones)."""
     grads = list(grads)
     inf_norm = float(norm_type) == float("inf")
     if not inf_norm and float(norm_type) != 2.0:
@@ -53,6 +54,10 @@ def clip_grads_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float
     dense = torch.Tensor.is_contiguous
     src = grads if all(map(dense, grads)) else [g.contiguous() for g in grads]   # another layout goes through a contiguous copy
     dst = src if out is None else into if all(map(dense, into)) else [t.contiguous() for t in into]
+    if dst is not into and (max_norm != float("inf") or grad_scale != 1.0 or out is not None):   # copies hide what the kernel's check sees
+        starts = [t.data_ptr() for t in into if t.numel()]
+        if len(set(starts)) != len(starts) or any(n > 1 and s == 0 for t in into for n, s in zip(t.shape, t.stride())):
+            raise ops._C.LsamError("clip_grads_: tensors that share memory, or repeat their elements")
     if error_if_nonfinite:
         norm = ops._clip_grads(src, src, float("inf"), inf_norm, 1.0)[0] * abs(grad_scale)
         if not bool(torch.isfinite(norm)):
@@ -176,6 +181,9 @@ class LoRAGradReducer:
         """grads <- mean over ranks.  Missing grads count as zero (DDP semantics).  With `max_norm` the mean is clipped to that global
         norm as it is written (one pass with the division by the ranks: clip_grads_), and the norm before clipping is returned; every
         rank clips the same sums, so the ranks stay alike without another exchange."""
+        if max_norm is not None and not (float(max_norm) >= 0.0 and self.flat.is_cuda):   # before any exchange, on every rank alike
+            raise ops._C.LsamError(f"LoRAGradReducer.reduce: max_norm {max_norm} on {self.flat.device}; a norm >= 0 on the MI355X (there is "
+                                   "no CPU fallback)")
         if not self.active():
             return None if max_norm is None else clip_grad_norm_(self.params, max_norm)
         ws = self.world_size()
@@ -192,10 +200,12 @@ class LoRAGradReducer:
             b.pending = []
             b.work, b.filled = None, False
         if max_norm is not None:
-            for p in self.params:
+            out = [torch.empty_like(p) if p.grad is None else p.grad for p in self.params]
+            norm = clip_grads_(self.views, max_norm, out=out, grad_scale=1.0 / ws)
+            for p, g in zip(self.params, out):
                 if p.grad is None:
-                    p.grad = torch.empty_like(p)
-            return clip_grads_(self.views, max_norm, out=[p.grad for p in self.params], grad_scale=1.0 / ws)
+                    p.grad = g
+            return norm
         if ws > 1:
             self.flat.mul_(1.0 / ws)
         for p, v in zip(self.params, self.views):

@@ -87,7 +87,8 @@ def test_matches_float64(N, C, H, W, G, act, dtype):
 
 # maps beyond one workgroup's registers, a range of pixels a workgroup: at most 16 pixels a thread, 64 threads' and 32 channels' sums one after
 # another (or a wave's), which the bounds above cover
-LARGE = [(2, 64, 130, 121, 8), (1, 300, 90, 71, 3), (1, 2056, 31, 33, 8), (3, 24, 97, 113, 24), (1, 7, 260, 250, 7), (1, 256, 100, 80, 1)]
+LARGE = [(2, 64, 130, 121, 8), (1, 300, 90, 71, 3), (1, 2056, 31, 33, 8), (3, 24, 97, 113, 24), (1, 7, 260, 250, 7), (1, 256, 100, 80, 1),
+         (1, 8192, 10, 10, 8), (2, 8192, 9, 9, 8192)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])

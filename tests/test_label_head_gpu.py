@@ -8,8 +8,8 @@ import torch
 import torch.nn.functional as F
 
 from conftest import TINY, rel_err
-from image_segmentation_amd import (GroupNormAct, LoRAGradReducer, build_image_encoder, clip_grad_norm_, linear_cross_entropy,
-                                    wrap_image_encoder_lora)
+from image_segmentation_amd import (GroupNormAct, LoRAGradReducer, build_image_encoder, clip_grad_norm_, clip_grads_, group_norm_act,
+                                    linear_cross_entropy, wrap_image_encoder_lora)
 from image_segmentation_amd.synth import fill_synthetic_, synth_frames, synth_tensor
 
 pytestmark = pytest.mark.gpu
@@ -88,3 +88,65 @@ def test_behind_the_encoder(dtype):
     assert rel_err(n, before) < 1e-6
     for p, g in zip(lora, got):
         assert rel_err(p.grad, g * (0.1 * before / (before + 1e-6))) < 1e-6
+
+
+def _case(seed, dtype, M=700, side=26):
+    """A step of all three operators, on its own tensors: (leaves, rest, function of them)."""
+    gen = torch.Generator().manual_seed(seed)
+    r = lambda *n: torch.randn(*n, generator=gen).cuda()
+    x = r(2, side, side, 32).to(dtype).permute(0, 3, 1, 2).requires_grad_(True)
+    gw, gb, w, b = r(32).requires_grad_(True), r(32).requires_grad_(True), (r(M, 32) / 6).to(dtype).requires_grad_(True), r(M).requires_grad_(True)
+    t = torch.randint(-1, M, (2, side, side), generator=gen).cuda()
+
+    def step():
+        h = group_norm_act(x, 8, gw, gb, act="gelu")
+        loss = linear_cross_entropy(h.movedim(1, -1), w, t, bias=b, ignore_index=-1)
+        grads = torch.autograd.grad(loss, (x, gw, gb, w, b))
+        norm = clip_grads_([torch.empty_like(g, memory_format=torch.contiguous_format).copy_(g) for g in grads], 0.1, out=(out := [
+            torch.empty(g.shape, device="cuda") for g in grads]))
+        return [loss.detach(), norm, *out]
+
+    return (x, gw, gb, w, b), t, step
+
+
+def test_two_streams_at_once():
+    cases = [_case(s, d, side=k) for s, d, k in ((1, torch.bfloat16, 26), (2, torch.float32, 31))]
+    want = [step() for *_, step in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(8):                                        # both queues filled in turn, nothing waited for between
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(cases[i][2]())
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for run in g:
+            assert all(torch.equal(a, e) for a, e in zip(run, w))
+
+
+def test_two_graphs_of_one_pool():
+    cases = [_case(s, torch.bfloat16) for s in (3, 4)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], []
+    with torch.cuda.stream(side):
+        for *_, step in cases:
+            step()
+        for *_, step in cases:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, pool=graphs[0].pool() if graphs else None, stream=side):
+                outs.append(step())
+            graphs.append(g)
+    for seed in (5, 6, 7):
+        for i in (0, 1):                                      # in the order they were captured in, as a shared pool asks
+            fresh, t, step = _case(seed + 10 * i, torch.bfloat16)
+            with torch.no_grad():
+                for leaf, v in zip(cases[i][0], fresh):
+                    leaf.copy_(v)
+                cases[i][1].copy_(t)
+            torch.cuda.synchronize()
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, e) for a, e in zip(outs[i], step()))

@@ -5,7 +5,7 @@ from array import array
 import pytest
 import torch
 
-from image_segmentation_amd import GroupNormAct, _C, clip_grad_norm_, clip_grads_, group_norm_act, ops
+from image_segmentation_amd import GroupNormAct, LoRAGradReducer, _C, clip_grad_norm_, clip_grads_, group_norm_act, ops
 
 
 def test_cpu_tensors_are_refused():
@@ -98,3 +98,23 @@ def test_module_is_group_norm():
     m.load_state_dict(torch.nn.GroupNorm(4, 16).state_dict())
     with pytest.raises(_C.LsamError):
         GroupNormAct(4, 16, act="tanh")
+
+
+def test_clip_of_copies_refuses_shared_memory():
+    # tensors that are not contiguous go through copies; what they share is looked at before
+    g = torch.ones(4, 6)
+    for grads, kw in (([g.t(), g.t()], {}), ([g.t(), g], {}), ([g.t(), torch.ones(3).expand(2, 3)], {}),
+                      ([g, g + 1], dict(out=[g.t().contiguous().t(), torch.zeros(4, 1).expand(4, 6)]))):
+        with pytest.raises(_C.LsamError, match="share memory"):
+            clip_grads_(grads, 1.0, **kw)
+
+
+@pytest.mark.parametrize("max_norm", [1.0, -1.0, float("nan")])
+def test_reducer_refuses_before_the_exchange(max_norm):
+    p = torch.nn.Parameter(torch.zeros(3))
+    red = LoRAGradReducer([p])
+    with pytest.raises(_C.LsamError, match="max_norm"):
+        red.reduce(max_norm)
+    assert p.grad is None and red.stats["all_reduce"] == 0
+    red.reduce()                                              # without it, as before
+    assert p.grad is None

@@ -137,12 +137,13 @@ template <bool KC, int R, int NW> struct Tile {
     }
 };
 
-__device__ __forceinline__ float row16_sum(float x) {   // over the 16 lanes that share lane >> 4
-    x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x128, 0xf, 0xf, false));
-    x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x124, 0xf, 0xf, false));
-    x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x122, 0xf, 0xf, false));
-    x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x121, 0xf, 0xf, false));
-    return x;
+// over the 16 lanes that share lane >> 4, four values side by side: a sum's result can be moved across lanes three instructions later
+__device__ __forceinline__ void row16_sum(float (&v)[4]) {
+#define ROW16(ctrl)                                                                                                                             \
+    _Pragma("unroll") for (int r = 0; r < 4; ++r) v[r] +=                                                                                       \
+        __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v[r]), ctrl, 0xf, 0xf, true));
+    ROW16(0x128) ROW16(0x124) ROW16(0x122) ROW16(0x121)
+#undef ROW16
 }
 
 // The scores' products (short k, long epilogue) are persistent: a workgroup takes every gridDim-th tile, and the DMA runs two k-tiles
@@ -179,8 +180,11 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
         At t;
         int ti = tiles_i, tj = tiles_j;
         asm volatile("" : "+s"(ti), "+s"(tj));   // the divisions' reciprocals are not kept in registers across the k-loop
-        t.split = id / (ti * tj);
-        id -= t.split * ti * tj;
+        t.split = 0;
+        if constexpr (!SCORES) {
+            t.split = id / (ti * tj);
+            id -= t.split * ti * tj;
+        }
         const int per = 8 * ti, grp = id / per, in = id - grp * per, gj = min(8, tj - grp * 8);
         t.it = in / gj;
         t.jt = grp * 8 + in - t.it * gj;
@@ -314,6 +318,9 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
         asm volatile("" ::: "memory");
     };
 
+    // the next tile's first operands, fetched during this one's last steps, are waited for before the epilogue's stores go out behind them
+    auto landed = [&] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
+
 #pragma unroll
     for (int q = 0; q < NP; ++q) issue(f, sa0, sb0, q);
     advance();
@@ -364,9 +371,10 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
         asm volatile("" : "+v"(lr_e), "+v"(g_e), "+v"(tid_e));
         const int i0 = cur.i0, j0 = cur.j0, ib = i0 + wi * TI * 16 + 4 * g_e, jb = j0 + wj * TJ * 16 + lr_e;
         if constexpr (SCORES) {
-            __shared__ float col[IT], rbase[JT], rw[JT], rs[JT];
+            __shared__ __attribute__((aligned(16))) float col[IT];   // read four at a time, like red written
+            __shared__ float rbase[JT], rw[JT], rs[JT];
             __shared__ int rt[JT];
-            __shared__ float red[MODE == STATS ? WI * 3 * JT : WJ * IT];
+            __shared__ __attribute__((aligned(16))) float red[MODE == STATS ? WI * 3 * JT : WJ * IT];
             // a class masked with the type's lowest value: a base of its size would not be a whole number's step away from its
             // scores; -inf and NaN stay what they are
             if (fabsf(col_b) > 1e9f && fabsf(col_b) != INFINITY) col_b = copysignf(1e9f, col_b);
@@ -380,11 +388,13 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
                 }
             }
             meet_lds();
+            if (p.bias || i0 + IT > p.I) {
 #pragma unroll
-            for (int x = 0; x < TI; ++x) {
-                const f32x4 b = *reinterpret_cast<const f32x4*>(col + (wi * TI + x) * 16 + 4 * g_e);
+                for (int x = 0; x < TI; ++x) {
+                    const f32x4 b = *reinterpret_cast<const f32x4*>(col + (wi * TI + x) * 16 + 4 * g_e);
 #pragma unroll
-                for (int y = 0; y < TJ; ++y) acc[x][y] += b;
+                    for (int y = 0; y < TJ; ++y) acc[x][y] += b;
+                }
             }
             if constexpr (MODE == STATS) {
 #pragma unroll
@@ -423,9 +433,12 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
                     const float sub = base == -INFINITY ? 0.f : base;   // every class of the tile at -inf: its exponentials are 0
                     float s = 0.f;
 #pragma unroll
-                    for (int x = 0; x < TI; ++x)
+                    for (int x = 0; x < TI; ++x) {   // four at a time: an exponential's result can be used two instructions later
+                        f32x4 e;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[x][y][r], LOG2E, -sub));
+                        for (int r = 0; r < 4; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(acc[x][y][r], LOG2E, -sub));
+                        s += (e[0] + e[1]) + (e[2] + e[3]);
+                    }
                     s = group4_sum(s);
                     if (g_e == 0) {
                         const int c = (wj * TJ + y) * 16 + lr_e;
@@ -434,6 +447,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
                         red[(wi * 3 + 2) * JT + c] = zs;
                     }
                 }
+                landed();
                 meet_lds();
                 if (tid_e < JT && j0 + tid_e < J) {
                     const int c = tid_e;
@@ -469,6 +483,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
 #pragma unroll
                             for (int r = 0; r < 4; ++r) acc[x][y][r] -= 16 * x + r == t ? w * p.keep : 0.f;
                     }
+                    if (y == 0) landed();
                     bf16* rowp = out + (size_t)(ok ? m : 0) * p.ldo + i0 + wi * TI * 16;
 #pragma unroll
                     for (int x = 0; x < TI; x += 2) {
@@ -489,15 +504,17 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
                 }
                 if (p.dbp) {
 #pragma unroll
-                    for (int x = 0; x < TI; ++x)
+                    for (int x = 0; x < TI; ++x) {
+                        float s[4];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            float s = 0.f;
+                            s[r] = acc[x][0][r];
 #pragma unroll
-                            for (int y = 0; y < TJ; ++y) s += acc[x][y][r];
-                            s = row16_sum(s);
-                            if (lr_e == 0) red[wj * IT + (wi * TI + x) * 16 + 4 * g_e + r] = s;
+                            for (int y = 1; y < TJ; ++y) s[r] += acc[x][y][r];
                         }
+                        row16_sum(s);
+                        if (lr_e == 0) *reinterpret_cast<f32x4*>(red + wj * IT + (wi * TI + x) * 16 + 4 * g_e) = f32x4{s[0], s[1], s[2], s[3]};
+                    }
                     meet_lds();
                     if (tid_e < IT && i0 + tid_e < p.I) {
                         float s = 0.f;
@@ -532,9 +549,7 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
             }
         }
         if (!MORE || id + (int)gridDim.x >= tiles) break;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
+        if constexpr (MODE == DZ) meet_lds();
         first(sa0, sb0);   // read here: held through the epilogue they cost 48 registers
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing may land in this workgroup's LDS after it

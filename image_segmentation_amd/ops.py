@@ -786,14 +786,18 @@ def _on_device(*ts):
             raise _C.LsamError(f"operands on different devices: {sorted({str(t.device) for t in ts if t is not None})}")
     if d < 0:
         _need_gpu(*ts)
-    return d, _HERE if torch.cuda.current_device() == d else torch.cuda.device(d)
+    return d, _HERE if torch._C._cuda_getDevice() == d else torch.cuda.device(d)
+
+
+def _vec(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """_f32c for what only its address is taken of: no alias is made where the tensor will do as it is."""
+    return t if t is None or (t.dtype is torch.float32 and t.is_contiguous()) else _f32c(t)
 
 
 def _unit_stride(t: torch.Tensor) -> torch.Tensor:
     """2-D tensor whose rows are contiguous and do not overlap (a leading dimension is passed separately); else a copy."""
-    t = t.detach()
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
+    if not t.is_contiguous() and ((t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
+        t = t.detach().contiguous()
     return t
 
 
@@ -808,11 +812,12 @@ def linear_ce_fwd(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     dev, on = _on_device(x, weight, bias, target)
     with on:
         code = dtype_code(x.dtype)
-        x, weight, b = _unit_stride(x), _unit_stride(weight), _f32c(bias)
-        target = target.detach().to(torch.int64).contiguous()
-        (M, D), V = x.shape, weight.shape[0]
-        loss = torch.empty((M,) if reduction == "none" else (), dtype=torch.float32, device=x.device)
-        L, u8 = lib(), dict(dtype=torch.uint8, device=x.device)
+        x, weight, b = _unit_stride(x), _unit_stride(weight), _vec(bias)
+        if target.dtype is not torch.int64 or not target.is_contiguous():
+            target = target.to(torch.int64).contiguous()
+        (M, D), V, device = x.shape, weight.shape[0], x.device
+        loss = torch.empty((M,) if reduction == "none" else (), dtype=torch.float32, device=device)
+        L, u8 = lib(), dict(dtype=torch.uint8, device=device)
         state = torch.empty(L.lsam_linear_ce_state_bytes(code, M, D), **u8)
         ws = torch.empty(L.lsam_linear_ce_ws_bytes(code, M, D, V, ptr(weight), _ld(weight), label_smoothing, 0), **u8)
         check(L.lsam_linear_ce_fwd(code, ptr(x), _ld(x), ptr(weight), _ld(weight), ptr(b), ptr(target), M, D, V, ignore_index,
@@ -826,17 +831,17 @@ def linear_ce_bwd(gout: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
     dev, on = _on_device(gout, state, weight, bias)
     with on:
         code = dtype_code(weight.dtype)
-        weight, b, gout = _unit_stride(weight), _f32c(bias), _f32c(gout)
-        V, D = weight.shape
-        dx = torch.empty(M, D, dtype=weight.dtype, device=weight.device) if want[0] else None
-        dw = torch.empty(V, D, dtype=weight.dtype, device=weight.device) if want[1] else None
-        db = torch.empty(V, dtype=torch.float32, device=weight.device) if want[2] and bias is not None else None
+        weight, b, gout = _unit_stride(weight), _vec(bias), _vec(gout)
+        (V, D), dtype, device = weight.shape, weight.dtype, weight.device
+        dx = torch.empty(M, D, dtype=dtype, device=device) if want[0] else None
+        dw = torch.empty(V, D, dtype=dtype, device=device) if want[1] else None
+        db = torch.empty(V, dtype=torch.float32, device=device) if want[2] and bias is not None else None
         L = lib()
         flags = (dx is not None) + 2 * (dw is not None) + 4 * (db is not None)
         if not flags:
             return None, None, None
         ws = torch.empty(L.lsam_linear_ce_ws_bytes(code, M, D, V, ptr(weight), _ld(weight), label_smoothing, flags), dtype=torch.uint8,
-                         device=weight.device)
+                         device=device)
         check(L.lsam_linear_ce_bwd(code, ptr(weight), _ld(weight), ptr(b), ptr(gout), M, D, V, label_smoothing, REDUCTIONS[reduction],
                                    ptr(state), ptr(dx), D, ptr(dw), D, ptr(db), ptr(ws), ws.numel(), stream_of(dev)))
     return dx, dw, db
@@ -884,17 +889,16 @@ def group_norm_act_fwd(x: torch.Tensor, groups: int, weight: Optional[torch.Tens
     [N, groups, 2] (mean, 1 / std) for group_norm_act_bwd."""
     dev, on = _on_device(x, weight, bias)
     with on:
-        x = x.detach()
         lay = channels_last_rows(x)
         if lay is None:
             raise _C.LsamError(f"group_norm_act: shape {tuple(x.shape)} with strides {x.stride()} is not channels last "
                                "(x.contiguous(memory_format=torch.channels_last))")
         N, P, sx, px = lay
-        Cc, w, b, L = x.shape[1], _f32c(weight), _f32c(bias), lib()
+        Cc, w, b, L, device = x.shape[1], _vec(weight), _vec(bias), lib(), x.device
         y = _channels_last_like(x, lay)
-        stats = torch.empty((N, groups, 2), dtype=torch.float32, device=x.device) if want_stats else None
+        stats = torch.empty((N, groups, 2), dtype=torch.float32, device=device) if want_stats else None
         nws = L.lsam_group_norm_act_ws_bytes(N, P, Cc, groups, 0)
-        ws = torch.empty(nws, dtype=torch.uint8, device=x.device)
+        ws = torch.empty(nws, dtype=torch.uint8, device=device)
         check(L.lsam_group_norm_act_fwd(dtype_code(x.dtype), x.data_ptr(), sx, px, ptr(w), ptr(b), N, P, Cc, groups, eps, ACTIVATIONS[act],
                                         y.data_ptr(), ptr(stats), ws.data_ptr(), nws, stream_of(dev)))
     return (y, stats) if want_stats else y
@@ -905,7 +909,6 @@ def group_norm_act_bwd(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, w
     """(dx T channels last, dweight fp32, dbias fp32) of group_norm_act_fwd; dy of any layout (copied to channels last if it is not)."""
     dev, on = _on_device(dy, x, stats, weight, bias)
     with on:
-        x, dy = x.detach(), dy.detach()
         lay = channels_last_rows(x)
         if dy.dtype != x.dtype:
             dy = dy.to(x.dtype)
@@ -914,11 +917,11 @@ def group_norm_act_bwd(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, w
             dy = _channels_last_like(x).copy_(dy)
             lay_y = channels_last_rows(dy)
         N, P, sx, px = lay
-        Cc, G, w, b, L = x.shape[1], stats.shape[1], _f32c(weight), _f32c(bias), lib()
+        Cc, G, w, b, L, device = x.shape[1], stats.shape[1], _vec(weight), _vec(bias), lib(), x.device
         dx = _channels_last_like(x, lay)
-        dw, db = torch.empty((2, Cc), dtype=torch.float32, device=x.device).unbind()
+        dw, db = torch.empty(Cc, dtype=torch.float32, device=device), torch.empty(Cc, dtype=torch.float32, device=device)
         nws = L.lsam_group_norm_act_ws_bytes(N, P, Cc, G, 1)
-        ws = torch.empty(nws, dtype=torch.uint8, device=x.device)
+        ws = torch.empty(nws, dtype=torch.uint8, device=device)
         check(L.lsam_group_norm_act_bwd(dtype_code(x.dtype), dy.data_ptr(), lay_y[2], lay_y[3], x.data_ptr(), sx, px, ptr(w), ptr(b),
                                         stats.data_ptr(), N, P, Cc, G, ACTIVATIONS[act], dx.data_ptr(), dw.data_ptr(), db.data_ptr(),
                                         ws.data_ptr(), nws, stream_of(dev)))

@@ -11,6 +11,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import ops
 
@@ -21,6 +22,18 @@ def _f32(g: torch.Tensor) -> torch.Tensor:
         return g if g.is_contiguous() else g.contiguous()
     g = g.contiguous()
     return ops.add_rows(g.view(-1, g.shape[-1]), None, torch.float32).view(g.shape)
+
+
+def no_derivative(*ts) -> bool:
+    """Nobody asks for a derivative through these operands (None among them): the call needs no autograd node, which costs as much on the
+    host as a small kernel's launch."""
+    if forward_ad._current_level >= 0:
+        return False                                          # inside forward-mode differentiation: the node says that it is not built
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return False
+    return True
 
 
 def _once(name: str):

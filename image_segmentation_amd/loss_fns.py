@@ -18,6 +18,7 @@ import torch
 import torch.nn as nn
 
 from . import heads_autograd as HA
+from . import ops
 from ._C import LsamError
 
 CORE_LOSS_KEY = "core_loss"   # training/trainer.py:57
@@ -102,8 +103,8 @@ def linear_cross_entropy(inputs, weight, targets, bias=None, ignore_index: int =
         raise ValueError(f"{reduction} is not a valid value for reduction")
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError(f"label_smoothing must be between 0.0 and 1.0, got {label_smoothing}")
-    loss = HA.LinearCrossEntropyFn.apply(inputs.reshape(-1, inputs.shape[-1]), weight, bias, targets.reshape(-1), int(ignore_index),
-                                         float(label_smoothing), reduction)
+    args = (inputs.reshape(-1, inputs.shape[-1]), weight, bias, targets.reshape(-1), int(ignore_index), float(label_smoothing), reduction)
+    loss = ops.linear_ce_fwd(*args)[0] if HA.no_derivative(inputs, weight, bias) else HA.LinearCrossEntropyFn.apply(*args)
     return loss.view(targets.shape) if reduction == "none" else loss
 
 

@@ -32,6 +32,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
             raise LsamError(f"group_norm_act: {name} {tuple(t.shape)} {t.dtype} does not match {x.shape[1]} channels")
     if ops.channels_last_rows(x) is None:
         x = x.movedim(1, -1).contiguous().movedim(-1, 1)
+    if HA.no_derivative(x, weight, bias):
+        return ops.group_norm_act_fwd(x, int(num_groups), weight, bias, float(eps), act)
     return HA.GroupNormActFn.apply(x, weight, bias, int(num_groups), float(eps), act)
 
 

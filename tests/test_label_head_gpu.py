@@ -150,3 +150,24 @@ def test_two_graphs_of_one_pool():
             graphs[i].replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, e) for a, e in zip(outs[i], step()))
+
+
+def test_without_a_derivative_and_in_forward_mode():
+    import torch.autograd.forward_ad as fwd
+    (x, gw, gb, w, b), t, _ = _case(8, torch.float32)
+    rows = lambda v: v.movedim(1, -1)
+    h = group_norm_act(x, 8, gw, gb, act="silu")
+    loss = linear_cross_entropy(rows(h), w, t, bias=b, ignore_index=-1)
+    assert h.requires_grad and loss.requires_grad
+    with torch.no_grad():
+        h0 = group_norm_act(x, 8, gw, gb, act="silu")
+        assert torch.equal(h0, h) and torch.equal(linear_cross_entropy(rows(h0), w, t, bias=b, ignore_index=-1), loss)
+    x, gw, gb, w, b = (v.detach() for v in (x, gw, gb, w, b))
+    h1 = group_norm_act(x, 8, gw, gb, act="silu")
+    assert not h1.requires_grad and torch.equal(h1, h) and torch.equal(linear_cross_entropy(rows(h1), w, t, bias=b, ignore_index=-1), loss)
+    with fwd.dual_level():                                    # not built: an error, not a result without its tangent
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        with pytest.raises(Exception):
+            group_norm_act(dual, 8, gw, gb)
+        with pytest.raises(Exception):
+            linear_cross_entropy(rows(dual), w, t)

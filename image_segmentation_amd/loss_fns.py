@@ -103,9 +103,10 @@ def linear_cross_entropy(inputs, weight, targets, bias=None, ignore_index: int =
         raise ValueError(f"{reduction} is not a valid value for reduction")
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError(f"label_smoothing must be between 0.0 and 1.0, got {label_smoothing}")
-    args = (inputs.reshape(-1, inputs.shape[-1]), weight, bias, targets.reshape(-1), int(ignore_index), float(label_smoothing), reduction)
+    rows = inputs if inputs.dim() == 2 else inputs.reshape(-1, inputs.shape[-1])
+    args = (rows, weight, bias, targets if targets.dim() == 1 else targets.reshape(-1), int(ignore_index), float(label_smoothing), reduction)
     loss = ops.linear_ce_fwd(*args)[0] if HA.no_derivative(inputs, weight, bias) else HA.LinearCrossEntropyFn.apply(*args)
-    return loss.view(targets.shape) if reduction == "none" else loss
+    return loss.view(targets.shape) if loss.shape != targets.shape and reduction == "none" else loss
 
 
 class MultiStepMultiMasksAndIous(nn.Module):

@@ -6,8 +6,9 @@
 // into chunks and a workgroup takes one chunk.  Squares are summed in fp64 (free beside the loads: 136 us for 212 M bf16 values against
 // 133 in fp32): neither 1e-30 nor 1e30 leaves the range, and the norm does not depend on how the list is cut beyond the last bit of an
 // fp64 sum.  Chunk sums are joined in a fixed order: same bits every time.
-// 212 M bf16 values clipped into fp32: norm 130 us (3.3 TB/s), joining 6, scaling 260 (4.9 TB/s; a copy: 5.07).  Lists of a few hundred
-// tensors are bound by the host's reading of them: 311 tensors, 69 M fp32 values with c = 1: 121 us, 70 of them the kernels'.
+// 599 tensors, 212 M bf16 values clipped into fp32: norm 120 us (3.5 TB/s; 129 in launches of 128 tensors), joining 6, scaling 257 (4.9 TB/s;
+// a copy: 5.07).  Lists of a few hundred tensors are bound by the host's reading of them: 311 tensors, 69 M fp32 values with c = 1: 105 us,
+// 61 of them the kernels'.
 #include <algorithm>
 #include <vector>
 
@@ -15,20 +16,23 @@
 
 namespace lsam {
 namespace {
-constexpr int NT = 256, TAB = 128;       // tensors a launch: the table stays below the 4 KB that kernel arguments may take
+constexpr int NT = 256;
 constexpr int SELF_JOIN = 1024;          // up to so many chunk sums the second pass joins them itself: two launches instead of three
 
-struct Table {
+// Tensors of a launch, as many as stay below the 4 KB that kernel arguments may take: 208 that are read (and written in place), 128 with an
+// output apart.
+template <bool APART> struct Table {
+    static constexpr int TAB = APART ? 128 : 208;
     const void* src[TAB];
-    void* dst[TAB];
+    void* dst[APART ? TAB : 1];
     unsigned n[TAB];          // elements; longer tensors take several entries
     int first[TAB];           // first chunk of the entry, counted in this launch
     unsigned char kind[TAB];  // bit 0: src bf16, bit 1: dst bf16
     int count, chunks, chunk, base;   // entries, chunks of this launch, elements a chunk, chunks before this launch
 };
-static_assert(sizeof(Table) <= 3600, "kernel arguments");
+static_assert(sizeof(Table<false>) <= 3700 && sizeof(Table<true>) <= 3700, "kernel arguments");
 
-__device__ __forceinline__ int entry_of(const Table& t, int c) {   // last entry whose first chunk is <= c
+template <typename Tab> __device__ __forceinline__ int entry_of(const Tab& t, int c) {   // last entry whose first chunk is <= c
     int lo = 0, hi = t.count - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -96,7 +100,7 @@ template <typename T, bool INF> __device__ __forceinline__ void chunk_norm(const
     if (rest + tid < n) a.add(to_f(p[rest + tid]));
 }
 
-template <bool INF> __global__ __launch_bounds__(NT) void clip_norm_kernel(const Table t, double* __restrict__ part) {
+template <bool INF> __global__ __launch_bounds__(NT) void clip_norm_kernel(const Table<false> t, double* __restrict__ part) {
     __shared__ Acc<INF> red[NT / 64];
     const int c = blockIdx.x, e = entry_of(t, c);
     const unsigned o = (unsigned)(c - t.first[e]) * (unsigned)t.chunk;
@@ -161,8 +165,9 @@ template <typename S, typename D> __device__ __forceinline__ void chunk_scale(co
 }
 
 // `parts` > 0: joins the chunk sums itself (every workgroup the same way) and the first one reports norm and factor
-template <bool INF>
-__global__ __launch_bounds__(NT) void clip_scale_kernel(const Table t, const double* __restrict__ part, int parts, Limit l, float* __restrict__ out) {
+template <bool INF, bool APART>
+__global__ __launch_bounds__(NT) void clip_scale_kernel(const Table<APART> t, const double* __restrict__ part, int parts, Limit l,
+                                                        float* __restrict__ out) {
     __shared__ Acc<INF> red[NT / 64];
     float norm, f;
     if (parts > 0) {
@@ -172,14 +177,19 @@ __global__ __launch_bounds__(NT) void clip_scale_kernel(const Table t, const dou
             out[1] = f;
         }
     } else f = out[1];
+    if (!APART && f == 1.f) return;   // nothing changes
     const int c = blockIdx.x, e = entry_of(t, c), kind = t.kind[e];
-    if (f == 1.f && t.src[e] == t.dst[e]) return;
+    const void* src = t.src[e];
+    void* dst = APART ? t.dst[e] : const_cast<void*>(src);
+    if (f == 1.f && src == dst) return;
     const unsigned o = (unsigned)(c - t.first[e]) * (unsigned)t.chunk;
     const int n = (int)min((unsigned)t.chunk, t.n[e] - o);
-    if (kind == 0) chunk_scale(static_cast<const float*>(t.src[e]) + o, static_cast<float*>(t.dst[e]) + o, n, f);
-    else if (kind == 1) chunk_scale(static_cast<const bf16*>(t.src[e]) + o, static_cast<float*>(t.dst[e]) + o, n, f);
-    else if (kind == 2) chunk_scale(static_cast<const float*>(t.src[e]) + o, static_cast<bf16*>(t.dst[e]) + o, n, f);
-    else chunk_scale(static_cast<const bf16*>(t.src[e]) + o, static_cast<bf16*>(t.dst[e]) + o, n, f);
+    if (kind == 0) chunk_scale(static_cast<const float*>(src) + o, static_cast<float*>(dst) + o, n, f);
+    else if (kind == 3) chunk_scale(static_cast<const bf16*>(src) + o, static_cast<bf16*>(dst) + o, n, f);
+    else if constexpr (APART) {   // in place the types are one
+        if (kind == 1) chunk_scale(static_cast<const bf16*>(src) + o, static_cast<float*>(dst) + o, n, f);
+        else chunk_scale(static_cast<const float*>(src) + o, static_cast<bf16*>(dst) + o, n, f);
+    }
 }
 
 constexpr long ENTRY = 1l << 30;   // elements an entry of the table may have
@@ -202,8 +212,47 @@ long total_of(const long long* n, int count) {
     return t;
 }
 
-template <bool INF> int run(const std::vector<Table>& tabs, bool scale, double* part, int parts, Limit l, float* out, hipStream_t s) {
-    for (const Table& t : tabs) {
+// the list cut into tables
+template <bool APART>
+std::vector<Table<APART>> tables(const unsigned long long* src, const unsigned long long* dst, const long long* n, const unsigned char* kind, int count,
+                                 int chunk) {
+    std::vector<Table<APART>> tabs;
+    long chunks = 0;
+    for (int i = 0; i < count; ++i)
+        for (long o = 0; o < (long)n[i]; o += ENTRY) {
+            if (tabs.empty() || tabs.back().count == Table<APART>::TAB || tabs.back().chunks > (1 << 24)) {
+                tabs.emplace_back();
+                Table<APART>& f = tabs.back();
+                f.count = f.chunks = 0;
+                f.chunk = chunk;
+                f.base = (int)chunks;
+            }
+            Table<APART>& t = tabs.back();
+            const long left = (long)n[i] - o, take = left < ENTRY ? left : ENTRY;
+            t.src[t.count] = reinterpret_cast<const void*>(src[i] + (unsigned long long)o * (kind[i] & 1 ? 2 : 4));
+            if constexpr (APART) t.dst[t.count] = reinterpret_cast<void*>(dst[i] + (unsigned long long)o * (kind[i] & 2 ? 2 : 4));
+            t.n[t.count] = (unsigned)take;
+            t.first[t.count] = t.chunks;
+            t.kind[t.count++] = kind[i];
+            const int k = (int)((take + chunk - 1) / chunk);
+            t.chunks += k;
+            chunks += k;
+        }
+    return tabs;
+}
+
+template <bool INF, bool APART>
+int scale_all(const std::vector<Table<APART>>& tabs, const double* part, int parts, Limit l, float* out, hipStream_t s) {
+    for (const Table<APART>& t : tabs) {
+        clip_scale_kernel<INF, APART><<<t.chunks, NT, 0, s>>>(t, part, parts, l, out);
+        LSAM_LAUNCH_CHECK();
+    }
+    return LSAM_OK;
+}
+template <bool INF>
+int run(const std::vector<Table<false>>& read, const std::vector<Table<true>>& apart, bool scale, double* part, int parts, Limit l, float* out,
+        hipStream_t s) {
+    for (const Table<false>& t : read) {
         clip_norm_kernel<INF><<<t.chunks, NT, 0, s>>>(t, part);
         LSAM_LAUNCH_CHECK();
     }
@@ -212,12 +261,8 @@ template <bool INF> int run(const std::vector<Table>& tabs, bool scale, double* 
         clip_join_kernel<INF><<<1, 1024, 0, s>>>(part, parts, l, out);
         LSAM_LAUNCH_CHECK();
     }
-    if (scale)
-        for (const Table& t : tabs) {
-            clip_scale_kernel<INF><<<t.chunks, NT, 0, s>>>(t, part, self ? parts : 0, l, out);
-            LSAM_LAUNCH_CHECK();
-        }
-    return LSAM_OK;
+    if (!scale) return LSAM_OK;
+    return apart.empty() ? scale_all<INF>(read, part, self ? parts : 0, l, out, s) : scale_all<INF>(apart, part, self ? parts : 0, l, out, s);
 }
 }  // namespace
 
@@ -259,31 +304,14 @@ int launch_clip_grads(const unsigned long long* src, const unsigned long long* d
         }
     }
     const int chunk = chunk_of(total_of(n, count));
-    std::vector<Table> tabs;
-    long chunks = 0;
-    for (int i = 0; i < count; ++i)
-        for (long o = 0; o < (long)n[i]; o += ENTRY) {
-            if (tabs.empty() || tabs.back().count == TAB || tabs.back().chunks > (1 << 24)) {
-                tabs.emplace_back();
-                Table& f = tabs.back();
-                f.count = f.chunks = 0;
-                f.chunk = chunk;
-                f.base = (int)chunks;
-            }
-            Table& t = tabs.back();
-            const long left = (long)n[i] - o, take = left < ENTRY ? left : ENTRY;
-            t.src[t.count] = reinterpret_cast<const void*>(src[i] + (unsigned long long)o * (kind[i] & 1 ? 2 : 4));
-            t.dst[t.count] = reinterpret_cast<void*>(dst[i] + (unsigned long long)o * (kind[i] & 2 ? 2 : 4));
-            t.n[t.count] = (unsigned)take;
-            t.first[t.count] = t.chunks;
-            t.kind[t.count++] = kind[i];
-            const int k = (int)((take + chunk - 1) / chunk);
-            t.chunks += k;
-            chunks += k;
-        }
+    const long chunks = chunks_of(n, count, chunk);
     LSAM_REQUIRE(chunks < (1l << 30), LSAM_ERR_UNSUPPORTED, "clip_grads: too many elements");
+    bool apart = false;
+    for (int i = 0; i < count; ++i) apart |= scaled && n[i] && (src[i] != dst[i] || (kind[i] != 0 && kind[i] != 3));
+    const auto read = tables<false>(src, dst, n, kind, count, chunk);
+    const auto other = apart ? tables<true>(src, dst, n, kind, count, chunk) : std::vector<Table<true>>();
     const Limit l{max_norm, scale};
-    return inf ? run<true>(tabs, scaled, static_cast<double*>(ws), (int)chunks, l, out, s)
-               : run<false>(tabs, scaled, static_cast<double*>(ws), (int)chunks, l, out, s);
+    return inf ? run<true>(read, other, scaled, static_cast<double*>(ws), (int)chunks, l, out, s)
+               : run<false>(read, other, scaled, static_cast<double*>(ws), (int)chunks, l, out, s);
 }
 }  // namespace lsam

@@ -932,6 +932,15 @@ def group_norm_act_bwd(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, w
 _PTR, _NUMEL, _DEV, _CONTIG, _SIZE = (torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous,
                                       torch.Tensor.size)
 _KIND = {torch.float32: 0, torch.bfloat16: 1}
+_DTYPE = torch.Tensor.dtype.__get__
+_IN_PLACE = bytes((0, 3)) + bytes(254)                       # kind of a tensor that is read and written
+
+
+def _kinds(ts) -> bytes:
+    """0 for fp32, 1 for bf16, a byte a tensor; lists of one type, which most are, without a look-up a tensor."""
+    d = list(map(_DTYPE, ts))
+    k = _KIND[d[0]]
+    return bytes((k,)) * len(d) if d.count(d[0]) == len(d) else bytes(map(_KIND.__getitem__, d))
 
 
 def clip_grads(src: Sequence[torch.Tensor], dst: Sequence[torch.Tensor], max_norm: float, inf_norm: bool = False, scale: float = 1.0):
@@ -957,8 +966,8 @@ def _clip_grads(src, dst, max_norm, inf_norm, scale):
         raise _C.LsamError("clip_grads: the tensors must be on one MI355X (there is no CPU fallback)")
     n = array("q", map(_NUMEL, src))
     try:
-        ks = [_KIND[t.dtype] for t in src]
-        kinds = bytes([3 * k for k in ks]) if place else bytes([a + 2 * _KIND[b.dtype] for a, b in zip(ks, dst)])
+        a = _kinds(src)
+        kinds = a.translate(_IN_PLACE) if place else bytes([k + 2 * m for k, m in zip(a, _kinds(dst))])
     except KeyError as e:
         raise _C.LsamError(f"clip_grads: unsupported type {e.args[0]}; float32 and bfloat16 are") from None
     dev, device = devs.pop(), src[0].device

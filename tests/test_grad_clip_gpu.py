@@ -58,6 +58,18 @@ def test_matches_float64(sizes, kinds, form, p):
     assert abs(float(norm) - want) <= 2 * E * want and all(torch.equal(g, s) for g, s in zip(src, make(sizes, kinds, sum(sizes))))
 
 
+def test_some_in_place():
+    # outputs that are their own inputs beside others that are not, over more tensors than a launch takes
+    grads = make([40 + i for i in range(230)], [BF if i % 3 == 0 else FP for i in range(230)], 31)
+    src = [g.clone() for g in grads]
+    out = [g if i % 2 else torch.empty_like(g, dtype=FP) for i, g in enumerate(grads)]
+    want = total(src)
+    for limit in (2.0 * want, 0.5 * want):
+        clip_grads_(grads, limit, out=out)
+        check_scaled(out, src, min(1.0, limit / (want + 1e-6)))
+        assert all(torch.equal(g, s) for i, (g, s) in enumerate(zip(grads, src)) if i % 2 == 0 or limit > want)
+
+
 @pytest.mark.parametrize("kind", [FP, BF])
 def test_alignment(kind):
     # views that begin anywhere in one buffer, with guards between them

@@ -230,6 +230,25 @@ def test_not_finite():
         assert gx[9].isnan().all() and int(gx.isnan().any(1).sum()) == 1
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_magnitudes(dtype):
+    # columns of x scaled by powers of two and those of w by their inverses: every product, and so every score, stays what it was, and
+    # the gradients scale with them, all without a rounding
+    x, w, t, b, _ = make(150, 96, 500, dtype, True, 43)
+    k = torch.linspace(-60, 60, 96, device="cuda").round()
+    k = torch.where(torch.arange(96, device="cuda") % 2 == 0, k, -k)
+    up = torch.exp2(k).to(dtype)
+
+    def step(x, w):
+        leaves = [v.detach().requires_grad_(True) for v in (x, w, b)]
+        loss = linear_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2], label_smoothing=0.05)
+        return [loss.detach(), *torch.autograd.grad(loss, leaves)]
+
+    want, got = step(x, w), step(x * up, w / up)
+    got[1], got[2] = got[1] * up, got[2] / up
+    assert all(torch.equal(a, e) for a, e in zip(got, want))
+
+
 def test_gradient_against_differences():
     x, w, t, b, _ = make(20, 24, 50, torch.float32, True, 19)
     leaves = [v.requires_grad_(True) for v in (x, w, b)]

@@ -75,29 +75,31 @@ __device__ __forceinline__ void mma(const uint4& a, const uint4& b, f32x4& c) {
 
 // fp32 operands go through the bf16 matrix pipes as three terms, x = x0 + x1 + x2 exactly: 8 bits of the 24 each, whatever is left being
 // rounded to the nearest 8.  |x1| <= 2^-9 |x|, |x2| <= 2^-18 |x|, so of the nine products the three left out, x1 y2, x2 y1 and x2 y2, come
-// to at most 2^-25 |x y|: half of what rounding one fp32 product costs.  Six bf16 products at 16 times the fp32 instructions' rate; the
-// small ones go first.  (2011 x 252 x 10007 forward and gradient: 360 us, 416 with fp32 matrix instructions.)
-constexpr unsigned TERM_A = 2 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 0 << 10, TERM_B = 0 | 2 << 2 | 1 << 4 | 0 << 6 | 1 << 8 | 0 << 10;
-constexpr int TERMS = 6;
+// to at most 2^-25 |x y|: half of what rounding one fp32 product costs.  Six bf16 products at 16 times the fp32 instructions' rate; of a
+// k-tile the small ones go first.  A k-tile holds all three planes of both operands, so that each is fetched and read once for its six
+// products.  (2011 x 252 x 10007 forward and gradient: 294 us; 416 with
+// fp32 matrix instructions, 357 with k run through once a product.)
 
-// One operand's tile in LDS.  KC: R rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7).  Transposed: 64 rows of R values, read
+// One operand's tile in LDS.  KC: R rows of KE values, 16-byte chunk c of row r at c ^ (r & 7) (KE = 32, four chunks: c ^ (r / 4 & 3)), so
+// that sixteen rows' reads of one chunk fall on different banks.  Transposed: KE rows of R values, read
 // with the transposing LDS load (16 lanes take 4 k-rows x 16 columns), whose 8 rows of a half wave must fall on different banks: 32-byte
 // column pair p of row k at p ^ h(k), h = k's bits 0, 1, 3.
 // DMA instruction q (of NI a wave) fills 1 KB; from one q to the next a lane's source moves by a fixed number of rows, and its chunk
 // within the row stays, so one offset and one first k describe them all.  Rows of a KC tile behind the limit lie behind the
 // descriptor's last byte and read zeros; every other chunk that must not be read gets an offset that does.
-constexpr int KE = 64;   // k of a k-tile
-template <bool KC, int R, int NW> struct Tile {
-    static constexpr int RB = R * 2;
-    static constexpr int NI = R * 128 / 1024 / NW;          // DMA instructions a wave and stage
-    static constexpr int ROWS = KC ? NW * 8 : NW * 1024 / RB;   // rows from one of them to the next
-    static_assert(R * 128 % (1024 * NW) == 0 && (KC || (NW * 1024 % RB == 0 && ROWS % 16 == 0)), "a lane's chunk stays");
+template <bool KC, int R, int NW, int KE> struct Tile {
+    static constexpr int RB = R * 2, KB = KE * 2, BYTES = R * KB;
+    static constexpr int NI = BYTES / 1024 / NW;               // DMA instructions a wave and stage
+    static constexpr int ROWS = NW * 1024 / (KC ? KB : RB);    // rows from one of them to the next
+    static_assert(KE == 64 || KE == 32, "chunks of a KC row");
+    static_assert(BYTES % (1024 * NW) == 0 && NW * 1024 % (KC ? KB : RB) == 0 && ROWS % 16 == 0, "a lane's chunk stays");
+    static __device__ __forceinline__ int swizzle(int c, int row) { return KE == 64 ? c ^ (row & 7) : c ^ ((row >> 2) & 3); }
     unsigned vo;   // byte offset of this lane's first chunk in the k-tile's slab
     int ke, col;   // its first k; transposed: its first column in the tile
     __device__ __forceinline__ void init(int wave, int lane, long ld) {
         const int b = wave * 1024 + lane * 16;
         if constexpr (KC) {
-            const int row = b >> 7, c = ((b >> 4) & 7) ^ (row & 7);
+            const int row = b / KB, c = swizzle((b % KB) >> 4, row);
             vo = (unsigned)((long)row * ld * 2 + c * 16);
             ke = c * 8;
             col = 0;
@@ -108,12 +110,12 @@ template <bool KC, int R, int NW> struct Tile {
             col = c * 8;
         }
     }
-    // k-tile slab: KC advances 128 bytes along the rows, transposed KE rows
+    // k-tile slab: KC advances KE values along the rows, transposed KE rows
     static __device__ __forceinline__ const char* slab(const void* base, long ld, int r0, long k0) {
         const char* p = static_cast<const char*>(base);
         return KC ? p + ((long)r0 * ld + k0) * 2 : p + (k0 * ld + r0) * 2;
     }
-    static __device__ __forceinline__ long step(long ld) { return KC ? 128 : KE * ld * 2; }
+    static __device__ __forceinline__ long step(long ld) { return KC ? KB : KE * ld * 2; }
     // DMA instruction q of a k-tile of which `left` k and `rows` rows (columns, transposed) exist
     __device__ __forceinline__ void issue(const char* slab_p, char* dst, int wave, int left, int q, long ld, int rows) const {
         const int bytes = KC ? rows * (int)ld * 2 : 0x7FFFFFFF;
@@ -126,7 +128,7 @@ template <bool KC, int R, int NW> struct Tile {
     }
     // the fragment of 16-wide tile t, k-step ks (0, 1): lane (g, lr) holds column 16 t + lr, its share of the step's k
     static __device__ __forceinline__ uint4 read(const char* s, int t, int ks, int g, int lr) {
-        if constexpr (KC) return *reinterpret_cast<const uint4*>(s + (t * 16 + lr) * 128 + (((ks * 4 + g) ^ (lr & 7)) << 4));
+        if constexpr (KC) return *reinterpret_cast<const uint4*>(s + (t * 16 + lr) * KB + (swizzle(ks * 4 + g, lr) << 4));
         using s4 = __attribute__((ext_vector_type(4))) short;
         using s4p = __attribute__((address_space(3))) s4*;
         const int h = (lr >> 2) | ((g & 1) << 2);
@@ -149,7 +151,7 @@ __device__ __forceinline__ void row16_sum(float (&v)[4]) {
 // The scores' products (short k, long epilogue) are persistent: a workgroup takes every gridDim-th tile, and the DMA runs two k-tiles
 // ahead across the border of two tiles, so that the next tile's operands arrive under this one's epilogue.  Lane (g, lr) of wave
 // (wi, wj) ends up with Out[j][i] at j = j0 + (wj TJ + y) 16 + lr, i = i0 + (wi TI + x) 16 + 4 g + r in register r of accumulator (x, y).
-// X3: operands of three planes; k runs through the six terms, one after another.
+// X3: operands of three planes.
 // A fragment read feeds TJ (TI) products and the barrier stands once a k-tile, so the 256-wide tile waits for the matrix pipes, not for
 // LDS: 4096^3 at 1200 TF/s with both operands stored along k, 1205 with both transposed (library product: 1300).
 template <bool X3, bool AKC, bool BKC, int MODE, int WI, int WJ, int TI, int TJ>
@@ -159,13 +161,14 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
     constexpr bool OPQ = !AKC && !BKC, ROWS_K = MODE == OUT || MODE == PART, SCORES = MODE == STATS || MODE == DZ;
     constexpr bool MORE = SCORES;   // more than one tile a workgroup
     static_assert(64 * NW >= IT && 64 * NW >= JT, "a thread a column and a row of the tile");
-    using TA = Tile<AKC, IT, NW>;
-    using TB = Tile<BKC, JT, NW>;
+    constexpr int PL = X3 ? 3 : 1, KE = X3 ? 32 : 64;   // planes of an operand; k of a k-tile
+    using TA = Tile<AKC, IT, NW, KE>;
+    using TB = Tile<BKC, JT, NW, KE>;
     // two stages of either operand, each a variable of its own: what the compiler can tell apart it does not make a read wait for
-    __shared__ __attribute__((aligned(1024))) char sa0[IT * 128];
-    __shared__ __attribute__((aligned(1024))) char sa1[IT * 128];
-    __shared__ __attribute__((aligned(1024))) char sb0[JT * 128];
-    __shared__ __attribute__((aligned(1024))) char sb1[JT * 128];
+    __shared__ __attribute__((aligned(1024))) char sa0[PL * TA::BYTES];
+    __shared__ __attribute__((aligned(1024))) char sa1[PL * TA::BYTES];
+    __shared__ __attribute__((aligned(1024))) char sb0[PL * TB::BYTES];
+    __shared__ __attribute__((aligned(1024))) char sb1[PL * TB::BYTES];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wi = wave % WI, wj = wave / WI, g = lane >> 4, lr = lane & 15;
@@ -192,25 +195,19 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
         t.j0 = t.jt * JT;
         return t;
     };
-    // k-tiles of a term, and of a tile: an even number, so that every tile begins in the same stage; those behind its share of k read zeros
-    const int kpt = max(1, min(per_split, kt_all)), kts = X3 ? TERMS * kpt : (kpt + 1) & ~1;
+    // k-tiles of a tile: an even number, so that every tile begins in the same stage; those behind its share of k read zeros
+    const int kts = (max(1, min(per_split, kt_all)) + 1) & ~1;
     int id = xcd_remap(blockIdx.x, gridDim.x);
     if (id >= tiles) return;
     TA ta;
     TB tb;
     ta.init(wave, lane, p.lda);
     tb.init(wave, lane, p.ldb);
-    constexpr int NP = TA::NI + TB::NI;
+    constexpr int NP = PL * (TA::NI + TB::NI);
     // Where the DMA is: the next k-tile to fetch, `fin` k-tiles into a tile.  It runs on into the workgroup's next tile.
     struct Slab { const char *pa, *pb; int left, ra, rb; };   // slabs; k left; rows (columns) of the tile that exist
     Slab f, fnext;
     int fin = 0;
-    const char *ta0 = nullptr, *tb0 = nullptr;   // X3: the tile's first slabs in plane 0, its k, the term and the k-tile in it
-    int tleft = 0, term = 0, tin = 0;
-    auto plane = [&](const char* p, long stride, unsigned seq, int term) __attribute__((always_inline)) {
-        const long w = (seq >> (2 * term)) & 3;
-        return p + (stride & -(w & 1)) + ((2 * stride) & -(w >> 1));
-    };
     auto enter = [&](int id) __attribute__((always_inline)) {
         Slab f;
         const At t = at(id);
@@ -227,29 +224,11 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
         f.pa += TA::step(p.lda);
         f.pb += TB::step(p.ldb);
         f.left -= KE;
-        if constexpr (X3) {
-            const long m = -(long)(++tin == kpt);
-            auto sel = [&](auto a, auto b) { return (decltype(a))(((long)b & m) | ((long)a & ~m)); };
-            term -= (int)m;
-            tin &= ~(int)m;
-            f.pa = sel(f.pa, plane(ta0, p.plane_a, TERM_A, term));
-            f.pb = sel(f.pb, plane(tb0, p.plane_b, TERM_B, term));
-            f.left = sel(f.left, term < TERMS ? tleft : 0);   // behind the last term nothing is fetched
-        }
         if constexpr (MORE) {
             const long m = -(long)(++fin == kts);
             auto sel = [&](auto a, auto b) { return (decltype(a))(((long)b & m) | ((long)a & ~m)); };
-            if constexpr (X3) {
-                ta0 = sel(ta0, fnext.pa);
-                tb0 = sel(tb0, fnext.pb);
-                tleft = sel(tleft, fnext.left);
-                term &= ~(int)m;
-                f.pa = sel(f.pa, plane(fnext.pa, p.plane_a, TERM_A, 0));
-                f.pb = sel(f.pb, plane(fnext.pb, p.plane_b, TERM_B, 0));
-            } else {
-                f.pa = sel(f.pa, fnext.pa);
-                f.pb = sel(f.pb, fnext.pb);
-            }
+            f.pa = sel(f.pa, fnext.pa);
+            f.pb = sel(f.pb, fnext.pb);
             f.left = sel(f.left, fnext.left);
             f.ra = sel(f.ra, fnext.ra);
             f.rb = sel(f.rb, fnext.rb);
@@ -263,21 +242,19 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
         fnext.left = more ? fnext.left : 0;   // no such tile: nothing is fetched
     };
     f = enter(id);
-    if constexpr (X3) {
-        ta0 = f.pa;
-        tb0 = f.pb;
-        tleft = f.left;
-        f.pa = plane(ta0, p.plane_a, TERM_A, 0);
-        f.pb = plane(tb0, p.plane_b, TERM_B, 0);
-    }
     follow(id + gridDim.x);
     auto issue = [&](const Slab& t, char* sa, char* sb, int q) __attribute__((always_inline)) {   // DMA instruction q
-        if (q < TA::NI) ta.issue(t.pa, sa, wave, t.left, q, p.lda, t.ra);
-        else tb.issue(t.pb, sb, wave, t.left, q - TA::NI, p.ldb, t.rb);
+        constexpr int NA = PL * TA::NI;
+        if (q < NA) ta.issue(t.pa + q / TA::NI * p.plane_a, sa + q / TA::NI * TA::BYTES, wave, t.left, q % TA::NI, p.lda, t.ra);
+        else tb.issue(t.pb + (q - NA) / TB::NI * p.plane_b, sb + (q - NA) / TB::NI * TB::BYTES, wave, t.left, (q - NA) % TB::NI, p.ldb, t.rb);
     };
     int lr_k = lr, g_k = g;
-    auto rd_a = [&](const char* s, int x, int ks) __attribute__((always_inline)) { return TA::read(s, wi * TI + x, ks, g_k, lr_k); };
-    auto rd_b = [&](const char* s, int y, int ks) __attribute__((always_inline)) { return TB::read(s, wj * TJ + y, ks, g_k, lr_k); };
+    auto rd_a = [&](const char* s, int x, int ks, int plane = 0) __attribute__((always_inline)) {
+        return TA::read(s + plane * TA::BYTES, wi * TI + x, ks, g_k, lr_k);
+    };
+    auto rd_b = [&](const char* s, int y, int ks, int plane = 0) __attribute__((always_inline)) {
+        return TB::read(s + plane * TB::BYTES, wj * TJ + y, ks, g_k, lr_k);
+    };
 
     f32x4 acc[TI][TJ];
     // A k-step is TI rows of TJ MFMAs.  Behind row x its A fragment is replaced by the next step's (needed TI rows later), the next
@@ -312,6 +289,51 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
         }
         if (meet) advance();
     };
+    // X3: a k-step is the six products of the planes (2, 0) (0, 2) (1, 1) (1, 0) (0, 1) (0, 0).  A plane's fragments are replaced behind its
+    // last product -- B's plane 0, wanted to the end, by a second set -- and the workgroup meets behind the first row, as above.
+    uint4 a1[TI], a2[TI], q1[TJ], q2[TJ];
+    auto step3 = [&](const char* na, const char* nb, uint4 (&bc)[TJ], uint4 (&bn)[TJ], char* fa, char* fb) __attribute__((always_inline)) {
+        if (OPQ) asm volatile("" : "+v"(lr_k), "+v"(g_k));
+        auto rows = [&](int term, uint4 (&ax)[TI], uint4 (&by)[TJ], auto behind) __attribute__((always_inline)) {
+#pragma unroll
+            for (int x = 0; x < TI; ++x) {
+#pragma unroll
+                for (int y = 0; y < TJ; ++y) mma(ax[x], by[y], acc[x][y]);
+                if (term == 0 && x == 0) {
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                behind(x);
+#pragma unroll
+                for (int q = 0; q < NP; ++q)
+                    if (q == term * TI + x) issue(f, fa, fb, q);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        static_assert(NP <= 6 * TI, "a DMA instruction a row");
+        rows(0, a2, bc, [&](int x) __attribute__((always_inline)) { a2[x] = rd_a(na, x, 0, 2); });
+        rows(1, a, q2, [&](int x) __attribute__((always_inline)) {
+            if (x == TI - 1) {
+#pragma unroll
+                for (int y = 0; y < TJ; ++y) q2[y] = rd_b(nb, y, 0, 2);
+            }
+        });
+        rows(2, a1, q1, [&](int x) __attribute__((always_inline)) {
+            if (x < TJ) bn[x] = rd_b(nb, x, 0, 0);
+        });
+        rows(3, a1, bc, [&](int x) __attribute__((always_inline)) { a1[x] = rd_a(na, x, 0, 1); });
+        rows(4, a, q1, [&](int x) __attribute__((always_inline)) {
+            if (x == TI - 1) {
+#pragma unroll
+                for (int y = 0; y < TJ; ++y) q1[y] = rd_b(nb, y, 0, 1);
+            }
+        });
+        rows(5, a, bc, [&](int x) __attribute__((always_inline)) { a[x] = rd_a(na, x, 0, 0); });
+        advance();
+    };
+    static_assert(!X3 || TJ <= TI, "B's plane 0 is read a fragment a row");
     auto meet_lds = [&] {   // LDS writes of the epilogue only: the DMA in flight is not waited for
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
@@ -335,6 +357,18 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
         for (int x = 0; x < TI; ++x) a[x] = rd_a(na, x, 0);
 #pragma unroll
         for (int y = 0; y < TJ; ++y) b0[y] = rd_b(nb, y, 0);
+        if constexpr (X3) {
+#pragma unroll
+            for (int x = 0; x < TI; ++x) {
+                a1[x] = rd_a(na, x, 0, 1);
+                a2[x] = rd_a(na, x, 0, 2);
+            }
+#pragma unroll
+            for (int y = 0; y < TJ; ++y) {
+                q1[y] = rd_b(nb, y, 0, 1);
+                q2[y] = rd_b(nb, y, 0, 2);
+            }
+        }
     };
     first(sa0, sb0);
     for (;; id += gridDim.x) {
@@ -360,10 +394,15 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
             }
         }
         for (int kt = 0; kt < kts; kt += 2) {
-            step(sa0, sb0, 1, b0, b1, false, nullptr, nullptr);
-            step(sa1, sb1, 0, b1, b0, true, sa0, sb0);
-            step(sa1, sb1, 1, b0, b1, false, nullptr, nullptr);
-            step(sa0, sb0, 0, b1, b0, true, sa1, sb1);
+            if constexpr (X3) {
+                step3(sa1, sb1, b0, b1, sa0, sb0);
+                step3(sa0, sb0, b1, b0, sa1, sb1);
+            } else {
+                step(sa0, sb0, 1, b0, b1, false, nullptr, nullptr);
+                step(sa1, sb1, 0, b1, b0, true, sa0, sb0);
+                step(sa1, sb1, 1, b0, b1, false, nullptr, nullptr);
+                step(sa0, sb0, 0, b1, b0, true, sa1, sb1);
+            }
         }
 
         // opaque copies: nothing of an epilogue's addresses is worked out ahead of the k-loop, where every register is taken
@@ -809,22 +848,23 @@ struct Carve {
 // Tiles of 256 x 256 (8 waves of 128 x 64 or 64 x 128, one workgroup a CU) or 128 x 128 (64 x 32, two a CU).  The large one feeds the
 // matrix pipes from LDS at close to their rate; the small one balances where the large leaves CUs idle.  Rounds of tiles, a small one
 // costed at a quarter of a large one and half as much again (16384 x 256 x 32000 scores: 440 us against 364; weight gradient of
-// 8192 x 896 x 50257: 769 against 644).
-constexpr double SMALL = 1.5;
-inline bool small_tiles(long big, long small) { return (double)((big + CU - 1) / CU) * 4 > SMALL * (double)((small + CU - 1) / CU); }
-
+// 8192 x 896 x 50257: 769 against 644).  fp32: 256 x 128 (64 x 64 a wave) or 128 x 128, one workgroup a CU, a small one costed at half a
+// large one and a fifth more (scores of 2011 x 252 x 10007: 64 against 66 us, of 4096 x 512 x 4096: 96 against 86).
+constexpr double SMALL = 1.5, SMALL3 = 1.2;
 template <typename T> struct CePlan {
     static constexpr bool X3 = sizeof(T) == 4;
     static constexpr int ES = X3 ? 6 : 2;   // bytes a value of the operands takes
-    int M, D, V, Dp, tile, tiles_v, tiles_m;   // tile: of the scores
-    bool pack_w, dx_small, dw_small;
+    static constexpr int JL = X3 ? 128 : 256;   // rows of a large tile: three planes of 256 x 128 fill the LDS
+    int M, D, V, Dp, tile_m, tiles_v, tiles_m;   // tile_m: rows of the scores' tiles
+    bool pack_w, small, dx_small, dw_small;
     int piece, s_dx, s_dw;
     CePlan(int M_, int D_, int V_, bool pack) : M(M_), D(D_), V(V_), pack_w(pack) {
         Dp = (D + 7) / 8 * 8;
         const int m = M > 0 ? M : 1;
-        tile = small_tiles((long)cdiv(V, 256) * cdiv(m, 256), (long)cdiv(V, 128) * cdiv(m, 128)) ? 128 : 256;
-        tiles_v = cdiv(V, tile);
-        tiles_m = cdiv(m, tile);
+        small = smaller((long)cdiv(V, 256) * cdiv(m, JL), 1, (long)cdiv(V, 128) * cdiv(m, 128), 1);
+        tile_m = small ? 128 : JL;
+        tiles_v = cdiv(V, small ? 128 : 256);
+        tiles_m = cdiv(m, tile_m);
         const size_t col = (size_t)m * ES * 256;
         size_t pt = DZ_CAP / col;
         if (pt < 1) pt = 1;
@@ -834,16 +874,19 @@ template <typename T> struct CePlan {
         piece = (int)pt * 256;
         // the other two products: the work of a CU is its rounds of tiles times their share of k
         auto pick = [&](int rows, int k, bool& small, int& cuts) {
-            const long big = (long)cdiv(rows, 256) * cdiv(Dp, 256), lit = (long)cdiv(rows, 128) * cdiv(Dp, 128);
+            const long big = (long)cdiv(rows, Dp <= 128 ? 256 : JL) * cdiv(Dp, 256), lit = (long)cdiv(rows, 128) * cdiv(Dp, 128);
             const int sb = splits(big, k, false), sl = splits(lit, k, true);
-            small = (double)((big * sb + CU - 1) / CU) * 4 / sb > SMALL * (double)((lit * sl + CU - 1) / CU) / sl;
+            small = smaller(big, sb, lit, sl);
             cuts = small ? sl : sb;
         };
         pick(m, piece, dx_small, s_dx);
         pick(piece, m, dw_small, s_dw);
     }
+    static bool smaller(long big, int sb, long lit, int sl) {   // tiles, cuts of k
+        return (double)((big * sb + CU - 1) / CU) * (X3 ? 2 : 4) / sb > (X3 ? SMALL3 : SMALL) * (double)((lit * sl + CU - 1) / CU) / sl;
+    }
     int splits(long tiles, int k, bool small) const {   // cuts of k that keep the CUs busy, at least four k-tiles (or six terms) each
-        const int slots = small ? 2 * CU : CU, least = X3 ? KE : 4 * KE, most = k / least > 0 ? k / least : 1;
+        const int slots = small && !X3 ? 2 * CU : CU, least = X3 ? 64 : 256, most = k / least > 0 ? k / least : 1;
         const long s = tiles >= slots ? 1 : slots / tiles;
         return (int)(s < most ? s : most);
     }
@@ -910,7 +953,12 @@ template <bool X3, bool AKC, bool BKC, int MODE, int WI, int WJ, int TI, int TJ>
 // wave grids of the large tile: as many fragments of the operand that is cheaper to read.  4096^3: A transposed 64 x 128 waves 1333 TF/s
 // against 1177 with 128 x 64; both transposed 1205 against 1103 the other way round
 template <bool X3, bool AKC, bool BKC, int MODE> int ce_gemm(const CeArgs& a, bool small, hipStream_t s) {
-    if (small) return ce_gemm_run<X3, AKC, BKC, MODE, 2, 4, 4, 2>(a, 2, s);
+    if (small) return ce_gemm_run<X3, AKC, BKC, MODE, 2, 4, 4, 2>(a, X3 ? 1 : 2, s);
+    if constexpr (X3 && (MODE == ACC || MODE == PART))
+        if (a.I <= 128)   // narrow rows: 128 x 256.  8000 x 128 x 8000: dx 146 us, dW 132; with 128 x 128 tiles 199 and 170
+            return ce_gemm_run<X3, AKC, BKC, MODE, 2, 4, 4, 4>(a, 1, s);
+    if constexpr (X3) return ce_gemm_run<X3, AKC, BKC, MODE, 4, 2, 4, 4>(a, 1, s);
+    else
     if constexpr (!AKC && BKC) return ce_gemm_run<X3, AKC, BKC, MODE, 4, 2, 4, 8>(a, 1, s);
     else return ce_gemm_run<X3, AKC, BKC, MODE, 2, 4, 8, 4>(a, 1, s);
 }
@@ -979,7 +1027,7 @@ int launch_linear_ce_fwd(const void* x, long ldx, const void* w, long ldw, const
         a.I = V; a.J = M; a.K = pl.Dp; a.n = st.n;
         a.bias = bias; a.tgt = st.tgt; a.smooth_z = smooth; a.part = f.part; a.zt = f.zt; a.rows_cap = M; a.splits = 1;
         a.plane_a = (long)V * pl.Dp * 2; a.plane_b = (long)M * pl.Dp * 2;
-        LSAM_TRY((ce_gemm<X3, true, true, STATS>(a, pl.tile == 128, s)));
+        LSAM_TRY((ce_gemm<X3, true, true, STATS>(a, pl.small, s)));
     }
     const int blocks = M > 0 ? cdiv(M, 16) : 1;
     if (M > 0 || reduction != LSAM_REDUCE_NONE) {
@@ -1036,7 +1084,7 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
             a.base2 = st.base2; a.sum = st.sum; a.idx = st.idx; a.grad = grad; a.sm = smooth / ((float)V * unit); a.keep = keep / unit;
             a.dbp = db ? b.dbp + v0 : nullptr; a.dbp_ld = V;
             a.out = b.dz; a.ldo = pl.piece; a.splits = 1;
-            LSAM_TRY((ce_gemm<X3, true, true, DZ>(a, pl.tile == 128, s)));
+            LSAM_TRY((ce_gemm<X3, true, true, DZ>(a, pl.small, s)));
         }
         if (dx && M > 0) {
             CeArgs a{};
@@ -1070,7 +1118,7 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
         }
     }
     if (dx || db)
-        LSAM_TRY(finish(Finish{b.dx, (long)M * pl.Dp, pl.s_dx, st.pos, nullptr, dx ? M : 0, D, pl.Dp, {}, dx, lddx, 0, V, pl.tile, b.dbp, db},
+        LSAM_TRY(finish(Finish{b.dx, (long)M * pl.Dp, pl.s_dx, st.pos, nullptr, dx ? M : 0, D, pl.Dp, {}, dx, lddx, 0, V, pl.tile_m, b.dbp, db},
                         dx ? (long)M * pl.Dp : 0));
     return LSAM_OK;
 }

@@ -10,8 +10,8 @@
 //
 // Bound by the matrix pipes: 2 M D V operations forward, 6 M D V backward, against (M + V) D values read.  With the scores in memory the
 // plain form moves 2 to 4 bytes of each several times over and takes the sum of three library products besides.  Measured, bf16, rows x
-// D x classes, forward and gradients: 16384 x 256 x 32000 in 1.31 ms (plain 10.6; scores 355 us, dz 465, dx 282, dW 242), 8192 x 896 x
-// 50257 in 2.5 ms (plain 19.2; scores 640, dz 695, dx 615, dW 645); forward alone 4096 x 448 x 65536 in 250 us (plain 2940).  The
+// D x classes, forward and gradients: 16384 x 256 x 32000 in 1.23 ms (plain 10.6; scores 347 us, dz 440, dx 282, dW 242), 8192 x 896 x
+// 50257 in 2.4 ms (plain 19.2; scores 618, dz 688, dx 615, dW 645); forward alone 4096 x 448 x 65536 in 219 us (plain 2930).  The
 // products run at 0.9 to 1.2 PFLOP/s; the scores' and dz's epilogues (an exponential a score) are what D = 256 adds to them.
 #include "kernels.hpp"
 

@@ -11,8 +11,11 @@
 // Bound by the matrix pipes: 2 M D V operations forward, 6 M D V backward, against (M + V) D values read.  With the scores in memory the
 // plain form moves 2 to 4 bytes of each several times over and takes the sum of three library products besides.  Measured, bf16, rows x
 // D x classes, forward and gradients: 16384 x 256 x 32000 in 1.23 ms (plain 10.6; scores 347 us, dz 440, dx 282, dW 242), 8192 x 896 x
-// 50257 in 2.4 ms (plain 19.2; scores 618, dz 688, dx 615, dW 645); forward alone 4096 x 448 x 65536 in 219 us (plain 2930).  The
+// 50257 in 2.4 ms (plain 19.2; scores 618, dz 688, dx 615, dW 645); forward alone 4096 x 448 x 65536 in 219 us (plain 2930); few rows
+// are bound by the table's bytes, read three times and its gradient written once: 1 x 896 x 50257 in 110 us (3.3 TB/s).  The
 // products run at 0.9 to 1.2 PFLOP/s; the scores' and dz's epilogues (an exponential a score) are what D = 256 adds to them.
+#include <type_traits>
+
 #include "kernels.hpp"
 
 namespace lsam {
@@ -63,7 +66,8 @@ struct CeArgs {
     long dbp_ld;
     int rows_cap;
     // outputs
-    void* out; long ldo;       // DZ, OUT: bf16; ACC, PART: fp32
+    void* out; long ldo;       // DZ: bf16; OUT: the operands' type; ACC, PART: fp32
+    int cols, vec;             // OUT: columns of a row; rows take whole vectors
     long split_stride;         // elements between the splits' outputs
     int splits, accumulate;
     long plane_a, plane_b, plane_out;   // fp32 operands: bytes between the three bf16 planes of A, of B and of DZ's output
@@ -77,7 +81,7 @@ __device__ __forceinline__ void mma(const uint4& a, const uint4& b, f32x4& c) {
 // rounded to the nearest 8.  |x1| <= 2^-9 |x|, |x2| <= 2^-18 |x|, so of the nine products the three left out, x1 y2, x2 y1 and x2 y2, come
 // to at most 2^-25 |x y|: half of what rounding one fp32 product costs.  Six bf16 products at 16 times the fp32 instructions' rate; of a
 // k-tile the small ones go first.  A k-tile holds all three planes of both operands, so that each is fetched and read once for its six
-// products.  (2011 x 252 x 10007 forward and gradient: 294 us; 416 with
+// products.  (2011 x 252 x 10007 forward and gradient: 305 us; 416 with
 // fp32 matrix instructions, 357 with k run through once a product.)
 
 // One operand's tile in LDS.  KC: R rows of KE values, 16-byte chunk c of row r at c ^ (r & 7) (KE = 32, four chunks: c ^ (r / 4 & 3)), so
@@ -568,11 +572,28 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
 #pragma unroll
             for (int y = 0; y < TJ; ++y) {
                 const int j = jb + 16 * y;
-                if constexpr (MODE == OUT) {   // every lane takes part in the exchange of a tile pair
-                    bf16* rowp = static_cast<bf16*>(p.out) + (size_t)min(j, J - 1) * p.ldo + i0 + wi * TI * 16;
+                if constexpr (MODE == OUT) {
+                    using T = std::conditional_t<X3, float, bf16>;
+                    T* row = static_cast<T*>(p.out) + (size_t)min(j, J - 1) * p.ldo;
+                    if (!X3 && p.vec) {   // every lane takes part in the exchange of a tile pair
+                        bf16* rowp = static_cast<bf16*>(p.out) + (size_t)min(j, J - 1) * p.ldo + i0 + wi * TI * 16;
 #pragma unroll
-                    for (int x = 0; x < TI; x += 2)
-                        store_bf16_tile_pair(rowp + 16 * x, g_e, acc[x][y] * f, acc[x + 1][y] * f, j < J && i0 + (wi * TI + x) * 16 + 8 * g_e < p.I);
+                        for (int x = 0; x < TI; x += 2)
+                            store_bf16_tile_pair(rowp + 16 * x, g_e, acc[x][y] * f, acc[x + 1][y] * f, j < J && i0 + (wi * TI + x) * 16 + 8 * g_e < p.I);
+                    } else if (j < J) {
+#pragma unroll
+                        for (int x = 0; x < TI; ++x) {
+                            const int i = ib + 16 * x;
+                            const f32x4 v = acc[x][y] * f;
+                            if (X3 && p.vec) {
+                                if (i < p.cols) store4(row + i, v);
+                            } else {
+#pragma unroll
+                                for (int r = 0; r < 4; ++r)
+                                    if (i + r < p.cols) row[i + r] = from_f<T>(v[r]);
+                            }
+                        }
+                    }
                 } else {
                     if (j >= J) continue;
 #pragma unroll
@@ -785,8 +806,9 @@ __global__ __launch_bounds__(1024) void ce_sum_kernel(const float* __restrict__ 
     if (threadIdx.x == 0) loss[0] = (float)(reduction == LSAM_REDUCE_MEAN ? part[0] / (double)n : part[0]);
 }
 
-// out[m] = factor * (sum of the splits' rows), or zeros where the row was ignored.  Workgroups from `first_db` on: the bias gradient, the
-// row tiles' column sums in their order.
+// out[m] = factor * (sum of the splits' rows), or zeros where the row was ignored; `lanes` threads share a sum of many splits where
+// there are few sums (6 x 592 of 512 splits: 4 us, 20 with a thread a sum; 2011 x 252 of 16: 23 and 16).  Workgroups from `first_db` on: the bias gradient, the row tiles'
+// column sums in their order.
 struct Finish {
     const float* acc; long stride; int splits;
     const int *pos, *n;
@@ -795,12 +817,14 @@ struct Finish {
     void* out; long ldo;
     int first_db, V, rows_tile;
     const float* dbp; float* db;
+    int lanes;
 };
 template <typename T> __global__ __launch_bounds__(256) void ce_finish_kernel(const Finish p) {
-    const int n = *p.n;
+    __shared__ f32x4 sh[256];
+    const int n = *p.n, tid = threadIdx.x;
     const float f = p.grad.factor(n);
     if ((int)blockIdx.x >= p.first_db) {
-        const int v = ((int)blockIdx.x - p.first_db) * 256 + threadIdx.x, tiles = (n + p.rows_tile - 1) / p.rows_tile;
+        const int v = ((int)blockIdx.x - p.first_db) * 256 + tid, tiles = (n + p.rows_tile - 1) / p.rows_tile;
         if (v >= p.V) return;
         float s = 0.f;
 #pragma unroll 8
@@ -808,17 +832,33 @@ template <typename T> __global__ __launch_bounds__(256) void ce_finish_kernel(co
         p.db[v] = tiles ? s * f : 0.f;
         return;
     }
-    const int cpr = p.Dp / 4;
-    for (long id = (long)blockIdx.x * 256 + threadIdx.x; id < (long)p.M * cpr; id += (long)p.first_db * 256) {
-        const int m = (int)(id / cpr), c = (int)(id - (long)m * cpr) * 4, r = p.pos ? p.pos[m] : m;
-        if (c >= p.D) continue;
+    const int cpr = p.Dp / 4, per = 256 / p.lanes, lane = tid / per;
+    const long total = (long)p.M * cpr;
+    for (long base = (long)blockIdx.x * per; base < total; base += (long)p.first_db * per) {
+        const long id = base + tid % per;
+        const int m = (int)(id / cpr), c = (int)(id - (long)m * cpr) * 4;
+        const bool on = id < total && c < p.D;
+        const int r = !on ? -1 : p.pos ? p.pos[m] : m;
         f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
         if (r >= 0) {
-            for (int s = 0; s < p.splits; ++s) v += load4(p.acc + s * p.stride + (size_t)r * p.Dp + c);
-            v *= f;
+            const float* a = p.acc + (size_t)r * p.Dp + c;
+#pragma unroll 4
+            for (int s = lane; s < p.splits; s += p.lanes) v += load4(a + s * p.stride);
         }
+        if (p.lanes > 1) {
+            sh[tid] = v;
+            __syncthreads();
+            for (int o = p.lanes / 2; o; o >>= 1) {
+                if (lane < o) sh[tid] += sh[tid + o * per];
+                __syncthreads();
+            }
+            v = sh[tid % per];
+            __syncthreads();
+        }
+        if (!on || lane) continue;
+        v *= f;
         T* o = static_cast<T*>(p.out) + (size_t)m * p.ldo + c;
-        if (p.D % 4 == 0) store4(o, v);
+        if (p.D % 4 == 0 && p.ldo % 4 == 0) store4(o, v);
         else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -894,14 +934,13 @@ template <typename T> struct CePlan {
     // k cut (8192 x 896 x 50257: 788 tiles on 256 CUs).  How many of nv classes do.
     int rest(int nv) const {
         const int td = cdiv(Dp, 256), vt = cdiv(nv, 256), over = vt * td % CU;
-        if (dw_small || dw_f32() || vt * td <= CU || over == 0 || over >= CU / 2) return 0;
+        if (X3 || dw_small || dw_f32() || vt * td <= CU || over == 0 || over >= CU / 2) return 0;
         const int rt = cdiv(over, td);
         return splits((long)rt * td, M, false) > 1 ? nv - (vt - rt) * 256 : 0;
     }
-    // partial sums, or rows of dW that do not take four columns at a time: through fp32 and the joining kernel
-    bool dw_f32() const { return X3 || s_dw > 1 || D % 8; }
+    bool dw_f32() const { return s_dw > 1; }   // partial sums: through fp32 and the joining kernel
     size_t dw_floats() const {   // the rest's tiles times cuts: at most CU of 65536
-        return dw_f32() ? (size_t)s_dw * piece * Dp : piece / 256 * cdiv(Dp, 256) > CU ? (size_t)CU * 65536 : 0;
+        return dw_f32() ? (size_t)s_dw * piece * Dp : !X3 && piece / 256 * cdiv(Dp, 256) > CU ? (size_t)CU * 65536 : 0;
     }
     size_t state(char* base, CeState* st) const {
         Carve c{base};
@@ -954,7 +993,7 @@ template <bool X3, bool AKC, bool BKC, int MODE, int WI, int WJ, int TI, int TJ>
 // against 1177 with 128 x 64; both transposed 1205 against 1103 the other way round
 template <bool X3, bool AKC, bool BKC, int MODE> int ce_gemm(const CeArgs& a, bool small, hipStream_t s) {
     if (small) return ce_gemm_run<X3, AKC, BKC, MODE, 2, 4, 4, 2>(a, X3 ? 1 : 2, s);
-    if constexpr (X3 && (MODE == ACC || MODE == PART))
+    if constexpr (X3 && (!(MODE == STATS || MODE == DZ)))
         if (a.I <= 128)   // narrow rows: 128 x 256.  8000 x 128 x 8000: dx 146 us, dW 132; with 128 x 128 tiles 199 and 170
             return ce_gemm_run<X3, AKC, BKC, MODE, 2, 4, 4, 4>(a, 1, s);
     if constexpr (X3) return ce_gemm_run<X3, AKC, BKC, MODE, 4, 2, 4, 4>(a, 1, s);
@@ -1063,8 +1102,9 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
     const float keep = 1.f - smooth, unit = keep > 0.f ? keep : 1.f;
     const Grad grad{gout, reduction, unit};
     auto finish = [&](const Finish& p, long values) -> int {
-        const long blocks = (values / 4 + 255) / 256;
         Finish q = p;
+        q.lanes = p.splits >= 16 && values / 4 < 32768 ? 16 : 1;
+        const long blocks = (values / 4 * q.lanes + 255) / 256;
         q.grad = grad;
         q.n = st.n;
         q.first_db = (int)(blocks < 8192 ? blocks : 8192);
@@ -1095,21 +1135,21 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
             LSAM_TRY((ce_gemm<X3, false, true, ACC>(a, pl.dx_small, s)));
         }
         if (dw) {
-            // classes c0 .. c0 + nc of the piece; through fp32 where k is cut or T rows do not take four columns at a time
-            auto weight_grad = [&](int c0, int nc, [[maybe_unused]] bool f32, int cuts) -> int {
+            // classes c0 .. c0 + nc of the piece; through fp32 where k is cut
+            auto weight_grad = [&](int c0, int nc, bool f32, int cuts) -> int {
                 T* o = static_cast<T*>(dw) + (size_t)(v0 + c0) * lddw;
                 CeArgs a{};
                 a.A = st.xc; a.lda = pl.Dp;
                 a.B = b.dz + (size_t)c0 * 2; a.ldb = pl.piece; a.plane_a = (long)M * pl.Dp * 2; a.plane_b = (long)M * pl.piece * 2;
                 a.I = pl.Dp; a.J = nc; a.K = M; a.n = st.n; a.splits = cuts;
-                if constexpr (!X3)
-                    if (!f32) {
-                        a.out = o; a.ldo = lddw; a.grad = grad;
-                        return ce_gemm<X3, false, false, OUT>(a, pl.dw_small, s);
-                    }
+                if (!f32) {
+                    a.out = o; a.ldo = lddw; a.grad = grad; a.cols = D;
+                    a.vec = X3 ? D % 4 == 0 && lddw % 4 == 0 : D % 8 == 0;
+                    return ce_gemm<X3, false, false, OUT>(a, pl.dw_small, s);
+                }
                 a.out = b.dw; a.ldo = pl.Dp; a.split_stride = (long)nc * pl.Dp;
                 LSAM_TRY((ce_gemm<X3, false, false, PART>(a, pl.dw_small, s)));
-                return finish(Finish{b.dw, a.split_stride, cuts, nullptr, nullptr, nc, D, pl.Dp, {}, o, lddw, 0, 0, 0, nullptr, nullptr},
+                return finish(Finish{b.dw, a.split_stride, cuts, nullptr, nullptr, nc, D, pl.Dp, {}, o, lddw, 0, 0, 0, nullptr, nullptr, 1},
                               (long)nc * pl.Dp);
             };
             const int rest = pl.rest(nv);
@@ -1118,7 +1158,7 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
         }
     }
     if (dx || db)
-        LSAM_TRY(finish(Finish{b.dx, (long)M * pl.Dp, pl.s_dx, st.pos, nullptr, dx ? M : 0, D, pl.Dp, {}, dx, lddx, 0, V, pl.tile_m, b.dbp, db},
+        LSAM_TRY(finish(Finish{b.dx, (long)M * pl.Dp, pl.s_dx, st.pos, nullptr, dx ? M : 0, D, pl.Dp, {}, dx, lddx, 0, V, pl.tile_m, b.dbp, db, 1},
                         dx ? (long)M * pl.Dp : 0));
     return LSAM_OK;
 }

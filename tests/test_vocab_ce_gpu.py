@@ -100,6 +100,17 @@ def test_large_tiles(M, D, V, dtype):
     check(x, w, t, b, g, 0.1 if D == 100 else 0.0, "none" if D == 200 else "mean")
 
 
+# few rows against many classes (sums over hundreds of splits), many against few, and rows of dW of every alignment
+FEW = [(1, 100, 20000), (6, 587, 9001), (30, 101, 30000), (5, 592, 24000), (9000, 70, 5), (2100, 254, 40), (2100, 257, 700), (130, 129, 4000)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M, D, V", FEW)
+def test_long_and_narrow(M, D, V, dtype):
+    x, w, t, b, g = make(M, D, V, dtype, True, M + D + V, ignored=0.0 if M < 10 else 0.2)
+    check(x, w, t, b, g, 0.1 if D % 2 else 0.0, "sum" if M < 100 else "none")
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_several_pieces_of_the_classes(dtype):
     # gradients of the scores over a piece's 1 GiB in either type: the products accumulate over pieces

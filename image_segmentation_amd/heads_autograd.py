@@ -301,10 +301,10 @@ class GroupNormActFn(torch.autograd.Function):
     def backward(ctx, g):
         _once("group_norm_act")
         x, stats, weight, bias = ctx.saved_tensors
-        dx, dw, db = ops.group_norm_act_bwd(g, x, stats, weight, bias, ctx.act)
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        if need_w and weight.dtype != torch.float32:
+        want = ctx.needs_input_grad[:3]
+        dx, dw, db = ops.group_norm_act_bwd(g, x, stats, weight, bias, ctx.act, want)
+        if dw is not None and weight.dtype != torch.float32:
             dw = dw.to(weight.dtype)
-        if need_b and bias.dtype != torch.float32:
+        if db is not None and bias.dtype != torch.float32:
             db = db.to(bias.dtype)
-        return dx if need_x else None, dw if need_w else None, db if need_b else None, None, None, None
+        return dx if want[0] else None, dw, db, None, None, None

@@ -30,7 +30,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     for t, name in ((weight, "weight"), (bias, "bias")):
         if t is not None and (t.shape != x.shape[1:2] or not t.is_floating_point()):
             raise LsamError(f"group_norm_act: {name} {tuple(t.shape)} {t.dtype} does not match {x.shape[1]} channels")
-    if ops.channels_last_rows(x) is None:
+    if not (x.dim() == 4 and x.is_contiguous(memory_format=torch.channels_last)) and ops.channels_last_rows(x) is None:
         x = x.movedim(1, -1).contiguous().movedim(-1, 1)
     if HA.no_derivative(x, weight, bias):
         return ops.group_norm_act_fwd(x, int(num_groups), weight, bias, float(eps), act)

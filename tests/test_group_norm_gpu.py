@@ -155,6 +155,21 @@ def test_layouts(dtype):
     assert m.weight.grad.dtype == dtype and m.bias.grad.dtype == dtype
 
 
+@pytest.mark.parametrize("size", [6, 150])
+def test_only_some_gradients(size):
+    x, dy, w, b = make(2, 24, size, size, torch.float32, 33)
+    leaves = [v.detach().requires_grad_(True) for v in (x, w, b)]
+    full = torch.autograd.grad(group_norm_act(leaves[0], 4, leaves[1], leaves[2], act="gelu"), leaves, dy)
+    for i in range(3):
+        l = [v.detach().requires_grad_(i == j) for j, v in enumerate((x, w, b))]
+        (g,) = torch.autograd.grad(group_norm_act(l[0], 4, l[1], l[2], act="gelu"), [l[i]], dy)
+        assert torch.equal(g, full[i])
+    l = x.detach().requires_grad_(True)                       # no parameters, or one
+    for ps in ((None, None), (w, None), (None, b)):
+        (g,) = torch.autograd.grad(group_norm_act(l, 4, *ps, act="gelu"), [l], dy)
+        assert torch.isfinite(g).all()
+
+
 def test_empty():
     w = torch.ones(8, device="cuda", requires_grad=True)
     b = torch.zeros(8, device="cuda", requires_grad=True)

@@ -622,12 +622,13 @@ template <typename T, int V, int UMAX, int ACT> __global__ __launch_bounds__(ST)
 }
 
 // channels a workgroup of the one-pass kernels, 0 where they do not apply: the fewest whole groups that make whole pieces and 32 bytes of a
-// pixel, or 16 where that is too much for `umax` pieces a thread
+// pixel, or 16 where that is too much for `umax` pieces a thread; more of them where the launch would come to 2^32 threads, which the
+// runtime cuts short without an error (rows of features: 262,144 samples of 256 channels)
 int one_pass(const GnArgs& p, int V, int esz, int umax) {
     const int cpg = p.C / p.G;
     for (int least : {32, 16}) {
         int cb = cpg;
-        while (cb < p.C && (p.C % cb || cb % V || cb * esz < least)) cb += cpg;
+        while (cb < p.C && (p.C % cb || cb % V || cb * esz < least || (long)p.N * (p.C / cb) >= (1l << 32) / ST)) cb += cpg;
         if (cb % V || cb / V > ST) return 0;
         if (cdiv(p.P, ST / (cb / V)) <= umax) return cb;
     }

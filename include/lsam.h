@@ -514,7 +514,7 @@ int lsam_linear_ce_bwd(int dtype, const void* w, long ldw, const float* bias, co
 /* ---- group norm with an activation, channels last ------------------------------------------------------------------------------
  * x T [N] samples of P pixels of C channels: sample stride sx, pixel stride px (elements), channels contiguous; groups of C / G
  * neighbouring channels.  y = act((x - mean) rstd gamma + beta), T, contiguous [N][P][C]; gamma / beta fp32 [C] or NULL (1, 0).
- * stats fp32 [N][G][2] (mean, rstd) is what the backward needs, NULL where it is not wanted.  C <= 8192. */
+ * stats fp32 [N][G][2] (mean, rstd) is what the backward needs, NULL where it is not wanted.  C <= 8192, N < 2^20, N G < 2^24. */
 enum { LSAM_ACT_NONE = 0, LSAM_ACT_RELU = 1, LSAM_ACT_SILU = 2, LSAM_ACT_GELU = 3 };
 size_t lsam_group_norm_act_ws_bytes(int N, int P, int C, int G, int backward);
 int lsam_group_norm_act_fwd(int dtype, const void* x, long sx, long px, const float* gamma, const float* beta, int N, int P, int C, int G,

@@ -259,3 +259,10 @@ def test_refusals():
                      ((x, 2, w.cpu()), {}), ((x, 2), dict(act="tanh")), ((torch.zeros(1, 8200, 2, 2, device="cuda"), 2), {})):
         with pytest.raises(LsamError):
             group_norm_act(*args, **kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_samples(dtype):
+    # rows of features: with the fewest groups a workgroup the launch would have 2^32 threads and more, which the runtime cuts short
+    x, dy, w, b = make(300_000, 256, 1, 1, dtype, 35)
+    check(x, dy, w, b, 32, "silu")

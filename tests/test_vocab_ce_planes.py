@@ -1,0 +1,73 @@
+"""How close loss_fns.linear_cross_entropy comes in fp32, where operands are multiplied as three bf16 planes: relative L2 errors against
+float64.  Element by element bounds grow with the sums' lengths and would not see a plane that is missing or out of place; the norms do.
+
+In units of 2^-24: losing the third plane of one operand leaves it rounded to 16 bits, a relative error spread over +-2^-17 that the L2 norm
+of a product keeps: 25 to 45 of the product itself, over 10 of the loss where it is the scores'.  Three planes with sums in fp32 come to
+at most 7.5 in dx and dW, 4.5 in db and 2.7 in the loss at these sizes, fp32 products to 9.3, 9.3, 7.1 and 4.  The bounds lie half way to a
+lost plane (emulate() on the CPU shows both sides)."""
+import pytest
+import torch
+
+BOUND = {"loss": 6, "dx": 14, "dw": 14, "db": 9}
+
+
+def make(M, D, V):
+    g = torch.Generator().manual_seed(M + D + V)
+    w = torch.randn(V, D, generator=g) * (2 / D ** 0.5)
+    t = torch.randint(0, V, (M,), generator=g)
+    x = torch.randn(M, D, generator=g) + w[t] * (0.5 * D ** 0.5) * torch.rand(M, 1, generator=g)
+    return x, w, t, torch.randn(V, generator=g)
+
+
+def step(x, w, t, b, product):
+    """Row losses and the gradients of their sum; `product` forms the three matrix products."""
+    rows = torch.arange(len(t), device=t.device)
+    z = product(x, w.t(), "z") + b
+    top = z.amax(1, keepdim=True)
+    e = torch.exp(z - top)
+    s = e.sum(1, keepdim=True)
+    dz = e / s
+    dz[rows, t] -= 1
+    return {"loss": (top + s.log())[:, 0] - z[rows, t], "dx": product(dz, w, "dx"), "dw": product(dz.t(), x, "dw"), "db": dz.sum(0)}
+
+
+def errors(got, x, w, t, b):
+    want = step(x.double(), w.double(), t, b.double(), lambda a, c, name: a @ c)
+    return {k: float((got[k].double() - v).norm() / v.norm()) * 2.0 ** 24 for k, v in want.items()}
+
+
+def emulate(lost=None):
+    """A product of three bf16 planes an operand, the six of nine terms that count; `lost`: the product and the operand (0, 1) without its third."""
+    def planes(a, n):
+        out = []
+        for _ in range(n):
+            out.append(a.bfloat16().float())
+            a = a - out[-1]
+        return out
+
+    def product(a, c, name):
+        A, B = (planes(v, 2 if lost == (name, i) else 3) for i, v in enumerate((a, c)))
+        return sum(A[i] @ B[j] for i, j in ((2, 0), (0, 2), (1, 1), (1, 0), (0, 1), (0, 0)) if i < len(A) and j < len(B))
+    return product
+
+
+def test_bounds_see_a_lost_plane():
+    x, w, t, b = make(300, 252, 1000)
+    assert all(e <= BOUND[k] for k, e in errors(step(x, w, t, b, emulate()), x, w, t, b).items())
+    for name, seen in (("z", "loss"), ("dx", "dx"), ("dw", "dw")):
+        for operand in (0, 1):
+            assert errors(step(x, w, t, b, emulate((name, operand))), x, w, t, b)[seen] > BOUND[seen]
+
+
+# scores / dx / dW in tiles of: 128 x 128 throughout, k cut; 128 x 256 for dx and dW, k cut; 256 x 128, 128 x 256, dW with k whole; 256 x 128, 128 x 128,
+# dW 256 x 128 with k whole; 256 x 128 for dx and dW, k cut; 256 x 128, dx with k whole
+@pytest.mark.gpu
+@pytest.mark.parametrize("M, D, V", [(300, 252, 1000), (500, 64, 8000), (500, 64, 33000), (500, 300, 12000), (1000, 256, 3000), (8000, 600, 3000)])
+def test_fp32_is_as_close_as_fp32_products(M, D, V):
+    from image_segmentation_amd import linear_cross_entropy
+    x, w, t, b = (v.cuda() for v in make(M, D, V))
+    leaves = [v.requires_grad_(True) for v in (x, w, b)]
+    loss = linear_cross_entropy(x, w, t, bias=b, reduction="none")
+    got = dict(zip(("loss", "dx", "dw", "db"), (loss.detach(), *torch.autograd.grad(loss.sum(), leaves))))
+    e = errors(got, x.detach(), w.detach(), t, b.detach())
+    assert all(e[k] <= BOUND[k] for k in BOUND), e

@@ -25,6 +25,24 @@ using lds_p = __attribute__((address_space(3))) void*;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int ROW_BAD = -1;   // target outside [0, V): the row's loss and gradient become NaN
 
+// Exponentials are taken as 2^(z log2e - base) with a whole-number base: one fused multiply-add an element, and bases of different tiles
+// differ by exact powers of two.  Where the highest score is beyond 2^30 the rounding of z log2e to a base would be a step of 2^64 and more;
+// there neighbouring fp32 scores lie 128 apart, so that all but the highest itself count nothing, and exponentials are taken as
+// 2^(z - max), exactly 1 for it.  The base is 2 max then: beyond every whole-number base, in the same order, and two of them, or one of
+// either kind, are as far apart as their exponentials need.  Up to 1.7e38.
+constexpr float FAR_Z = 0x1p30f, FAR_BASE = 0x1p31f;
+struct Base {   // 2^(z mul - sub)
+    float mul, sub;
+    __device__ __forceinline__ explicit Base(float base) {
+        const bool far = fabsf(base) > FAR_BASE;
+        mul = far ? 1.f : LOG2E;
+        sub = far ? 0.5f * base : base;
+    }
+    static __device__ __forceinline__ float of(float mx) { return fabsf(mx) > FAR_Z ? 2.f * mx : __builtin_ceilf(mx * LOG2E); }
+};
+constexpr float MASK = 1e38f;       // finite biases beyond it count as that: their scores' bases stay finite
+constexpr float Z_SCALE = 0x1p-30f; // sums of scores are kept in units of 2^30: neither masks nor many classes leave the range
+
 // ---------------------------------------------------------------------------------------------------------------------
 // The product: Out[j][i] = sum_k A(i, k) B(j, k), i contiguous in Out.  An operand is stored "KC" ([i][k], k contiguous) or
 // transposed ([k][i]).  Tile IT x JT, k-tiles of 128 bytes, two LDS stages filled by LDS-DMA.
@@ -55,7 +73,7 @@ struct CeArgs {
     const int* tgt;            // [rows]
     int i_base;                // class of column 0
     float smooth_z;            // != 0: the sum of z over the classes is wanted too
-    float* part;               // STATS: planes [tiles_i][rows_cap] of (base, sum of exponentials, sum of z)
+    float* part;               // STATS: planes [tiles_i][rows_cap] of (base, sum of exponentials, sum of z in units of 1 / Z_SCALE)
     float* zt;                 // STATS: z of the target
     const float* base2;        // DZ: the row's base and its sum of exponentials
     const float* sum;
@@ -418,9 +436,8 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
             __shared__ float rbase[JT], rw[JT], rs[JT];
             __shared__ int rt[JT];
             __shared__ __attribute__((aligned(16))) float red[MODE == STATS ? WI * 3 * JT : WJ * IT];
-            // a class masked with the type's lowest value: a base of its size would not be a whole number's step away from its
-            // scores; -inf and NaN stay what they are
-            if (fabsf(col_b) > 1e9f && fabsf(col_b) != INFINITY) col_b = copysignf(1e9f, col_b);
+            // a class masked with the type's lowest value; -inf and NaN stay what they are
+            if (fabsf(col_b) > MASK && fabsf(col_b) != INFINITY) col_b = copysignf(MASK, col_b);
             if (tid_e < IT) col[tid_e] = col_b;
             if (tid_e < JT) {
                 rt[tid_e] = row_t;
@@ -460,26 +477,24 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
 #pragma unroll
                             for (int x = 0; x < TI; ++x)
 #pragma unroll
-                                for (int r = 0; r < 4; ++r) zs += ib + 16 * x + r < p.I ? acc[x][y][r] : 0.f;
+                                for (int r = 0; r < 4; ++r) zs = fmaf(ib + 16 * x + r < p.I ? acc[x][y][r] : 0.f, Z_SCALE, zs);
                         } else {
 #pragma unroll
                             for (int x = 0; x < TI; ++x)
 #pragma unroll
-                                for (int r = 0; r < 4; ++r) zs += acc[x][y][r];
+                                for (int r = 0; r < 4; ++r) zs = fmaf(acc[x][y][r], Z_SCALE, zs);
                         }
                         zs = group4_sum(zs);
                     }
-                    // exponentials are taken as 2^(z log2e - base) with a whole-number base: one fused multiply-add an element, and
-                    // bases of different tiles differ by exact powers of two.  (Scores beyond 1e9 would need z - max in a step of its own.)
-                    mx = group4_max(mx);
-                    const float base = __builtin_ceilf(mx * LOG2E);
-                    const float sub = base == -INFINITY ? 0.f : base;   // every class of the tile at -inf: its exponentials are 0
+                    const float base = Base::of(group4_max(mx));
+                    Base to(base);
+                    if (base == -INFINITY) to.sub = 0.f;   // every class of the tile at -inf: its exponentials are 0
                     float s = 0.f;
 #pragma unroll
                     for (int x = 0; x < TI; ++x) {   // four at a time: an exponential's result can be used two instructions later
                         f32x4 e;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(acc[x][y][r], LOG2E, -sub));
+                        for (int r = 0; r < 4; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(acc[x][y][r], to.mul, -to.sub));
                         s += (e[0] + e[1]) + (e[2] + e[3]);
                     }
                     s = group4_sum(s);
@@ -514,12 +529,13 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void ce_gemm_kernel(const CeArgs p
                 for (int y = 0; y < TJ; ++y) {
                     const int c = (wj * TJ + y) * 16 + lr_e, m = j0 + c;
                     const bool ok = m < J;
-                    const float base = rbase[c], w = rw[c], cs = rs[c], low = -w * p.sm;
+                    const Base to(rbase[c]);
+                    const float w = rw[c], cs = rs[c], low = -w * p.sm;
                     const int t = rt[c] - ib;
 #pragma unroll
                     for (int x = 0; x < TI; ++x)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[x][y][r] = fmaf(__builtin_amdgcn_exp2f(fmaf(acc[x][y][r], LOG2E, -base)), cs, low);
+                        for (int r = 0; r < 4; ++r) acc[x][y][r] = fmaf(__builtin_amdgcn_exp2f(fmaf(acc[x][y][r], to.mul, -to.sub)), cs, low);
                     if (__any(t >= 0 && t < TI * 16)) {
 #pragma unroll
                         for (int x = 0; x < TI; ++x)
@@ -625,7 +641,7 @@ struct CeState {   // what the forward leaves for the backward
     int* idx;      // [M] compact row -> row
     int* pos;      // [M] row -> compact row, -1 where ignored
     int* tgt;      // [M] compact; ROW_BAD outside [0, V)
-    float* base2;  // [M] compact: lse = (base2 + log2(sum)) / log2(e)
+    float* base2;  // [M] compact: lse = base2 / log2(e) + ln(sum), or base2 / 2 + ln(sum) where |base2| > FAR_BASE
     float* sum;
     char* xc;      // bf16 [M][Dp] compact rows, columns padded with zeros; fp32: three planes
 };
@@ -740,7 +756,7 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(const long long* __restri
 }
 
 // 16 rows a workgroup, 64 threads a row: joins the tiles' (base, sum) pairs; the loss of the row.  With one workgroup the sum over
-// the rows too.  base + log2(sum) and the target's score are subtracted in 64 bits: a learned row's loss is their small difference.
+// the rows too.  The logarithm of the sum and the target's score are subtracted in 64 bits: a learned row's loss is their small difference.
 __global__ __launch_bounds__(1024) void ce_loss_kernel(const float* __restrict__ part, const float* __restrict__ zt, int tiles, int cap, int V,
                                                        float smooth, CeState st, float* __restrict__ row_loss, float* __restrict__ loss,
                                                        int reduction) {
@@ -773,9 +789,9 @@ __global__ __launch_bounds__(1024) void ce_loss_kernel(const float* __restrict__
             }
             st.base2[r] = B;
             st.sum[r] = S;
-            const double L = (double)LOG2E, l2 = (double)B + log2((double)S);
+            const double L = (double)LOG2E, top = fabsf(B) > FAR_BASE ? 0.5 * (double)B : (double)B / L, rest = log2((double)S) / L;
             if (st.tgt[r] == ROW_BAD) out = (double)NAN;
-            else out = (l2 - L * (double)zt[r]) / L * (1. - (double)smooth) + (smooth != 0.f ? (double)smooth * (l2 / L - (double)Z / V) : 0.);
+            else out = (top - (double)zt[r] + rest) * (1. - (double)smooth) + (smooth != 0.f ? (double)smooth * (top - (double)Z / Z_SCALE / V + rest) : 0.);
             if (reduction == LSAM_REDUCE_NONE) loss[st.idx[r]] = (float)out;
             else row_loss[r] = (float)out;
         }

@@ -84,8 +84,8 @@ def linear_cross_entropy(inputs, weight, targets, bias=None, ignore_index: int =
 
     inputs [..., D] and weight [V, D]: both float32 or both bfloat16 (sums and statistics are fp32 either way; float32 values go through
     the matrix pipes as three bfloat16 terms, which together are exact for magnitudes from 1e-30 to 3.3e38; larger ones count as infinite);
-    targets [...] integer; bias [V] any float type: -inf takes a class out, finite values beyond +-1e9 (masks) count as that.  The loss is
-    fp32: targets' shape under reduction="none" (0 where ignored), one value otherwise.
+    targets [...] integer; bias [V] any float type: -inf takes a class out, finite values beyond +-1e38 count as that.  Scores of any size
+    up to 1.7e38 are kept as fp32 holds them.  The loss is fp32: targets' shape under reduction="none" (0 where ignored), one value otherwise.
     Rows whose target is `ignore_index` cost nothing and pass nothing on, whatever they hold.  A target outside [0, V) makes the loss
     NaN (F.cross_entropy stops the process there); with no row left, "mean" is NaN and the gradients are zero."""
     if not inputs.is_cuda:

@@ -8,6 +8,8 @@ A_m = max_v sum_k |x_mk w_vk| + |b_v|:
   a softmax value p is off by 2 t p; a gradient of the scores g = c (p - keep [v = t] - s) is then off by
                                                                      E = |c| (2 t p + 4 e (p + keep + s)) + u |g|  (g is held in T)
   a product over n of them adds n e of the sum of magnitudes, and the output's own rounding u |out|."""
+import math
+
 import pytest
 import torch
 import torch.nn.functional as F
@@ -341,3 +343,60 @@ def test_refusals():
         linear_cross_entropy(x, w, t, reduction="max")
     with pytest.raises(ValueError):
         linear_cross_entropy(x, w, t, label_smoothing=1.1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("power", [0, 20, 24, 25, 26, 31, 40, 80, 117])
+@pytest.mark.parametrize("smoothing", [0.0, 0.1])
+def test_scores_of_any_size(power, smoothing, dtype):
+    """One column, whole numbers times 2^power: every score is exact in fp32, and so is what a bias of such numbers makes of it.  What is left:
+    an exponential's argument is rounded where it is 64 at most (2^-17), the exponentials are good to a step, their sum has 700 terms:
+    2^-13 of the sum in all.  The mean of the scores is a sum of 700 terms in fp32."""
+    g = torch.Generator().manual_seed(power)
+    M, V = 60, 700
+    w = torch.randint(0, 50, (V, 1), generator=g).double()
+    w[[3, 200, 301, 640]] = 50.0                               # ties of the highest score, in several tiles
+    x = (torch.randint(1, 4, (M, 1), generator=g) * (1 - 2 * torch.randint(0, 2, (M, 1), generator=g))).double() * 2.0 ** power
+    t = torch.randint(0, V, (M,), generator=g).cuda()
+    t[:4] = torch.tensor([3, 640, 5, -100])
+    x, w = x.to("cuda", dtype), w.to("cuda", dtype)
+    b = (torch.randint(-3, 4, (V,), generator=g).double() * 2.0 ** power).float().cuda()
+    b[[3, 200, 301, 640]] = 0.0
+    gout = torch.rand(M, generator=g).cuda()
+    leaves = [v.detach().requires_grad_(True) for v in (x, w, b)]
+    loss = linear_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2], label_smoothing=smoothing, reduction="none")
+    grads = torch.autograd.grad(loss, leaves, gout)
+    X, W, B = (v.detach().double().requires_grad_(True) for v in (x, w, b))
+    Z = X @ W.t() + B
+    ref = F.cross_entropy(Z, t, label_smoothing=smoothing, reduction="none")
+    want = torch.autograd.grad(ref, (X, W, B), gout.double())
+    z = Z.detach()
+    assert torch.isfinite(loss).all()
+    assert ((loss - ref.detach()).abs() <= 2.0 ** -13 + 8 * E * ref.detach().abs() + smoothing * V * E * z.abs().amax(1)).all()
+    u = 2.0 ** -8 if dtype == torch.bfloat16 else E
+    rows = t >= 0
+    size = torch.softmax(z, 1) + F.one_hot(t.clamp_min(0), V).double() + smoothing / V
+    size = torch.where(rows, gout.double(), 0.0)[:, None] * size
+    X, W = X.detach().abs(), W.detach().abs()
+    for got, exp, lim in zip(grads, want, (size @ W, size.t() @ X, size.sum(0))):
+        assert ((got.double() - exp).abs() <= (2.0 ** -12 + u) * lim + u * exp.abs() + 1e-30).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mask", [-1e9, -3e9, -1e20, -1e38])
+def test_masks_of_any_size(mask, dtype):
+    # finite masks are the bias that they say: the loss of a masked target, and the mean of the scores that smoothing takes.  A score next to a mask
+    # keeps fp32's 24 bits of the larger one
+    x, w, t, b, _ = make(50, 24, 600, dtype, True, 47, ignored=0.0)
+    b[100:400] = mask
+    t[:8] = 150
+    z = x.double() @ w.double().t() + b.double()
+    for smoothing in (0.0, 0.1):
+        loss = linear_cross_entropy(x, w, t, bias=b, label_smoothing=smoothing, reduction="none")
+        ref = F.cross_entropy(z, t, label_smoothing=smoothing, reduction="none")
+        assert ((loss - ref).abs() <= 1e-4 + (600 * smoothing + 8) * E * ref.abs()).all()
+    # nothing but the type's lowest value: fp32 scores are all alike there
+    leaves = [v.detach().requires_grad_(True) for v in (x, w, torch.full_like(b, torch.finfo(torch.float32).min))]
+    loss = linear_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2])
+    assert abs(float(loss.detach()) - math.log(600)) < 1e-4
+    assert all(torch.isfinite(v).all() for v in torch.autograd.grad(loss, leaves))

@@ -1173,7 +1173,7 @@ int launch_linear_ce_bwd(const void* w, long ldw, const float* bias, const float
             if (rest) LSAM_TRY(weight_grad(nv - rest, rest, true, pl.splits((long)cdiv(rest, 256) * cdiv(pl.Dp, 256), M, false)));
         }
     }
-    if (dx || db)
+    if ((dx && M > 0) || db)
         LSAM_TRY(finish(Finish{b.dx, (long)M * pl.Dp, pl.s_dx, st.pos, nullptr, dx ? M : 0, D, pl.Dp, {}, dx, lddx, 0, V, pl.tile_m, b.dbp, db, 1},
                         dx ? (long)M * pl.Dp : 0));
     return LSAM_OK;

@@ -1036,7 +1036,9 @@ template <typename T> int gather(const Gather<T>& g, const int* n, int rows, hip
 
 int ce_check(int M, int D, int V, int reduction, float smooth) {
     LSAM_REQUIRE(M >= 0 && D > 0 && V > 0, LSAM_ERR_BAD_ARG, "linear_ce: %d rows, %d columns, %d classes", M, D, V);
-    LSAM_REQUIRE(M <= (1 << 28) && V <= (1 << 28) && D <= (1 << 18), LSAM_ERR_UNSUPPORTED, "linear_ce: %d rows, %d columns, %d classes", M, D, V);
+    // launches stay below 2^32 threads (64 a row in the loss's kernel, 512 a tile of dx): the runtime cuts a longer one short without an error
+    LSAM_REQUIRE(M <= (1 << 26) - 16 && V <= (1 << 28) && D <= (1 << 18) && (long)cdiv(M, 128) * cdiv(D, 128) < (1l << 23),
+                 LSAM_ERR_UNSUPPORTED, "linear_ce: %d rows, %d columns, %d classes", M, D, V);
     LSAM_REQUIRE(((long)M / 128 + 1) * ((long)V / 128 + 1) < (1l << 30), LSAM_ERR_UNSUPPORTED, "linear_ce: %d rows x %d classes", M, V);
     LSAM_REQUIRE(reduction >= 0 && reduction <= 2, LSAM_ERR_BAD_ARG, "linear_ce: reduction %d", reduction);
     LSAM_REQUIRE(smooth >= 0.f && smooth <= 1.f, LSAM_ERR_BAD_ARG, "linear_ce: label smoothing %g outside [0, 1]", (double)smooth);

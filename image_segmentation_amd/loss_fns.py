@@ -87,7 +87,7 @@ def linear_cross_entropy(inputs, weight, targets, bias=None, ignore_index: int =
     targets [...] integer; bias [V] any float type: -inf takes a class out, finite values beyond +-1e38 count as that.  Scores of any size
     up to 1.7e38 are kept as fp32 holds them.  The loss is fp32: targets' shape under reduction="none" (0 where ignored), one value otherwise.
     Rows whose target is `ignore_index` cost nothing and pass nothing on, whatever they hold.  A target outside [0, V) makes the loss
-    NaN (F.cross_entropy stops the process there); with no row left, "mean" is NaN and the gradients are zero."""
+    NaN (F.cross_entropy stops the process there); with no row left, "mean" is NaN and the gradients are zero.  At most 2^26 - 16 rows."""
     if not inputs.is_cuda:
         raise LsamError("linear_cross_entropy runs on the MI355X only (no CPU or PyTorch fallback)")
     if inputs.dim() < 1 or weight.dim() != 2 or inputs.shape[-1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:

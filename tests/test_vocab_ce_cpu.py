@@ -53,3 +53,14 @@ def test_sizes_without_rows():
         assert L.lsam_linear_ce_state_bytes(dtype, 0, 16) > 0
         for grads in range(8):
             assert L.lsam_linear_ce_ws_bytes(dtype, 0, 16, 40, 256, 16, 0.0, grads) > 0
+
+
+@pytest.mark.parametrize("M, D, V, rc", [
+    ((1 << 26) - 16, 8, 5, -4), ((1 << 26) - 15, 8, 5, -2), (1 << 26, 8, 5, -2), (1 << 28, 8, 5, -2),
+    ((1 << 26) - 16, 1920, 5, -4), ((1 << 26) - 16, 1921, 5, -2),   # 2^19 x 15 tiles of 512 threads, and 2^19 x 16
+])
+def test_rows_of_a_launch(M, D, V, rc):
+    # a launch may have 2^32 - 1 threads; the next check to fail is the workspace's
+    L = _C.lib()
+    assert L.lsam_linear_ce_fwd(_C.BF16, 256, D, 256, D, 0, 256, M, D, V, -100, 0.0, 1, 256, 256, 256, 0, 0) == rc
+    assert L.lsam_linear_ce_bwd(_C.BF16, 256, D, 0, 256, M, D, V, 0.0, 1, 256, 256, D, 256, D, 0, 256, 0, 0) == rc

@@ -34,7 +34,7 @@ def clip_grads_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float
     fp32 / bf16 tensors of any mix on one GPU; `out` may have other types than `grads` (bf16 gradients into fp32 buffers).  norm_type
     2 or inf.  Squares are summed in fp64.  A norm that is not finite makes the factor what torch.nn.utils.clip_grad_norm_ makes it
     (NaN, or 0 for an infinite one); error_if_nonfinite looks at the norm on the host first and raises, with nothing changed.
-    max_norm = inf: the norm alone.  Contiguous tensors that share memory are refused where anything would be written, and so are others
+    max_norm = inf: the norm alone, of tensors of any layout, and nothing is written.  Contiguous tensors that share memory are refused where anything would be written, and so are others
     that begin at one address or repeat their elements (expanded ones)."""
     grads = list(grads)
     inf_norm = float(norm_type) == float("inf")
@@ -54,7 +54,8 @@ def clip_grads_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float
     dense = torch.Tensor.is_contiguous
     src = grads if all(map(dense, grads)) else [g.contiguous() for g in grads]   # another layout goes through a contiguous copy
     dst = src if out is None else into if all(map(dense, into)) else [t.contiguous() for t in into]
-    if dst is not into and (max_norm != float("inf") or grad_scale != 1.0 or out is not None):   # copies hide what the kernel's check sees
+    writes = out is not None or max_norm != float("inf") or grad_scale != 1.0
+    if writes and dst is not into:                             # copies hide what the kernel's check sees
         starts = [t.data_ptr() for t in into if t.numel()]
         if len(set(starts)) != len(starts) or any(n > 1 and s == 0 for t in into for n, s in zip(t.shape, t.stride())):
             raise ops._C.LsamError("clip_grads_: tensors that share memory, or repeat their elements")
@@ -63,7 +64,7 @@ def clip_grads_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float
         if not bool(torch.isfinite(norm)):
             raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so it cannot be clipped.")
     norm = ops._clip_grads(src, dst, max_norm, inf_norm, grad_scale)[0]
-    if dst is not into:
+    if writes and dst is not into:
         for t, d in zip(into, dst):
             if t is not d:
                 t.copy_(d)

@@ -225,3 +225,22 @@ def test_reducer_clips_the_mean(tmp_path):
         check_scaled([p.grad for p in params], src, 0.3 * want / (want + 1e-6))
     finally:
         dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("kw", [{}, dict(error_if_nonfinite=True)])
+def test_norm_alone_writes_nothing(kw):
+    # tensors of any layout, expanded ones and ones that share memory among them: read, and neither written nor marked as written
+    base = make([24, 6, 5], [FP, BF, FP], 41)
+    grads = [base[0].view(4, 6).t(), base[0].view(4, 6), base[1].expand(3, 6), base[2][::2]]
+    want = total(grads)
+    versions = [g._version for g in base]
+    norm = clip_grads_(grads, math.inf, **kw)
+    assert abs(float(norm) - want) <= 2 * E * want
+    assert versions == [g._version for g in base] and all(torch.equal(g, s) for g, s in zip(base, make([24, 6, 5], [FP, BF, FP], 41)))
+    # what is saved for a backward stays good
+    x = torch.ones(2, 3, device="cuda").t().clone(memory_format=torch.preserve_format).requires_grad_(True)
+    y = x * 2
+    z = y * y
+    clip_grads_([y.detach()], math.inf)
+    z.sum().backward()
+    assert (x.grad == 8).all()

@@ -185,6 +185,10 @@ class LoRAGradReducer:
         if max_norm is not None and not (float(max_norm) >= 0.0 and self.flat.is_cuda):   # before any exchange, on every rank alike
             raise ops._C.LsamError(f"LoRAGradReducer.reduce: max_norm {max_norm} on {self.flat.device}; a norm >= 0 on the MI355X (there is "
                                    "no CPU fallback)")
+        if max_norm is not None:
+            for p in self.params:
+                if p.dtype not in (torch.float32, torch.bfloat16):
+                    raise ops._C.LsamError(f"LoRAGradReducer.reduce: max_norm with a parameter of {p.dtype}; float32 and bfloat16 are built")
         if not self.active():
             return None if max_norm is None else clip_grad_norm_(self.params, max_norm)
         ws = self.world_size()

@@ -244,3 +244,21 @@ def test_norm_alone_writes_nothing(kw):
     clip_grads_([y.detach()], math.inf)
     z.sum().backward()
     assert (x.grad == 8).all()
+
+
+def test_reducer_refuses_types_before_the_exchange(tmp_path):
+    # a gradient that cannot be clipped is refused while every rank's buckets are as they were, not behind the exchange
+    import torch.distributed as dist
+    params = [torch.nn.Parameter(torch.zeros(5, device="cuda")), torch.nn.Parameter(torch.zeros(4, device="cuda", dtype=torch.float16))]
+    dist.init_process_group("nccl", init_method=f"file://{tmp_path}/rendezvous", rank=0, world_size=1)
+    try:
+        red = LoRAGradReducer(params)
+        for p in params:
+            p.grad = torch.ones_like(p)
+        with pytest.raises(_C.LsamError, match="float16"):
+            red.reduce(max_norm=1.0)
+        assert red.stats["all_reduce"] == 0 and all((p.grad == 1).all() for p in params)
+        red.reduce()
+        assert red.stats["all_reduce"] == 1 and all((p.grad == 1).all() for p in params)
+    finally:
+        dist.destroy_process_group()

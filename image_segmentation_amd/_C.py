@@ -165,6 +165,7 @@ def lib() -> C.CDLL:
         L.lsam_group_norm_act_ws_bytes.argtypes = [i] * 5
         L.lsam_group_norm_act_fwd.argtypes = [i, vp, l, l, vp, vp, i, i, i, i, f, i, vp, vp, vp, sz, vp]
         L.lsam_group_norm_act_bwd.argtypes = [i, vp, l, l, vp, l, l, vp, vp, vp, i, i, i, i, i, vp, vp, vp, vp, sz, vp]
+        L.lsam_group_norm_act_bwd_params.argtypes = [i, vp, l, l, vp, l, l, vp, vp, vp, i, i, i, i, i, vp, vp, vp, sz, vp]
         L.lsam_clip_grads_ws_bytes.argtypes = [vp, i]
         L.lsam_clip_grads.argtypes = [vp, vp, vp, vp, i, C.c_double, i, C.c_double, vp, vp, sz, vp]
         L.lsam_prof_arm.argtypes = [i]
@@ -221,6 +222,7 @@ EXPORTED = [
     "lsam_qkv_window4_attention_image_bytes", "lsam_qkv_window4_attention_pack", "lsam_qkv_window4_attention_fwd",
     "lsam_stream_linear_image_bytes", "lsam_stream_linear_pack", "lsam_stream_linear_fwd",
     "lsam_linear_ce_state_bytes", "lsam_linear_ce_ws_bytes", "lsam_linear_ce_fwd", "lsam_linear_ce_bwd",
-    "lsam_group_norm_act_ws_bytes", "lsam_group_norm_act_fwd", "lsam_group_norm_act_bwd", "lsam_clip_grads_ws_bytes", "lsam_clip_grads",
+    "lsam_group_norm_act_ws_bytes", "lsam_group_norm_act_fwd", "lsam_group_norm_act_bwd",
+    "lsam_group_norm_act_bwd_params", "lsam_clip_grads_ws_bytes", "lsam_clip_grads",
     "lsam_outer_reduce_static_max_ws", "lsam_outer_reduce_static_init", "lsam_outer_reduce_static",
 ]

@@ -398,8 +398,16 @@ int lsam_group_norm_act_bwd(int dtype, const void* dy, long sy, long py, const v
                             float* dbeta, void* ws, size_t ws_bytes, lsam_stream_t stream) {
     hipStream_t s = static_cast<hipStream_t>(stream);
     DISPATCH(dtype,
-             launch_group_norm_act_bwd<float>(dy, sy, py, x, sx, px, gamma, beta, stats, N, P, C, G, act, dx, dgamma, dbeta, ws, ws_bytes, s),
-             launch_group_norm_act_bwd<bf16>(dy, sy, py, x, sx, px, gamma, beta, stats, N, P, C, G, act, dx, dgamma, dbeta, ws, ws_bytes, s));
+             launch_group_norm_act_bwd<float>(dy, sy, py, x, sx, px, gamma, beta, stats, N, P, C, G, act, true, dx, dgamma, dbeta, ws, ws_bytes, s),
+             launch_group_norm_act_bwd<bf16>(dy, sy, py, x, sx, px, gamma, beta, stats, N, P, C, G, act, true, dx, dgamma, dbeta, ws, ws_bytes, s));
+}
+int lsam_group_norm_act_bwd_params(int dtype, const void* dy, long sy, long py, const void* x, long sx, long px, const float* gamma,
+                                   const float* beta, const float* stats, int N, int P, int C, int G, int act, float* dgamma, float* dbeta,
+                                   void* ws, size_t ws_bytes, lsam_stream_t stream) {
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    DISPATCH(dtype,
+             launch_group_norm_act_bwd<float>(dy, sy, py, x, sx, px, gamma, beta, stats, N, P, C, G, act, false, nullptr, dgamma, dbeta, ws, ws_bytes, s),
+             launch_group_norm_act_bwd<bf16>(dy, sy, py, x, sx, px, gamma, beta, stats, N, P, C, G, act, false, nullptr, dgamma, dbeta, ws, ws_bytes, s));
 }
 
 size_t lsam_clip_grads_ws_bytes(const long long* host_n, int count) { return clip_ws_bytes(host_n, count); }

@@ -598,7 +598,7 @@ template <typename T, int V, int UMAX, int ACT> __global__ __launch_bounds__(ST)
         grp[2 * g + 1] = rstd * rstd * s2 / m;
     }
     __syncthreads();
-    if (!mine) return;
+    if (!mine || !p.out) return;   // no map wanted: the parameters' sums were all
     float c1[V], c2[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -708,6 +708,11 @@ template <typename T, int V> int run_bwd(GnArgs& p, hipStream_t s) {
     LSAM_LAUNCH_CHECK();
     gn_bwd_join_kernel<<<p.N * p.G, NT, 0, s>>>(p);
     LSAM_LAUNCH_CHECK();
+    if (!p.out) {   // 16 x 256 x 256 x 256 bf16: the second pass is more than half of the backward
+        gn_params_kernel<<<cdiv(p.C, NT), NT, 0, s>>>(p);
+        LSAM_LAUNCH_CHECK();
+        return LSAM_OK;
+    }
     auto a = p.act == LSAM_ACT_RELU   ? gn_bwd_apply_kernel<T, V, LSAM_ACT_RELU>
              : p.act == LSAM_ACT_SILU ? gn_bwd_apply_kernel<T, V, LSAM_ACT_SILU>
              : p.act == LSAM_ACT_GELU ? gn_bwd_apply_kernel<T, V, LSAM_ACT_GELU>
@@ -756,8 +761,8 @@ int launch_group_norm_act_fwd(const void* x, long sx, long px, const float* gamm
 
 template <typename T>
 int launch_group_norm_act_bwd(const void* dy, long sy, long py, const void* x, long sx, long px, const float* gamma, const float* beta,
-                              const float* stats, int N, int P, int C, int G, int act, void* dx, float* dgamma, float* dbeta, void* ws,
-                              size_t ws_bytes, hipStream_t s) {
+                              const float* stats, int N, int P, int C, int G, int act, bool want_dx, void* dx, float* dgamma, float* dbeta,
+                              void* ws, size_t ws_bytes, hipStream_t s) {
     LSAM_TRY(gn_check(N, P, C, G, act, sx, px));
     LSAM_TRY(gn_check(N, P, C, G, act, sy, py));
     GnArgs p{};
@@ -765,7 +770,8 @@ int launch_group_norm_act_bwd(const void* dy, long sy, long py, const void* x, l
     LSAM_REQUIRE(ws && aligned16(ws), LSAM_ERR_BAD_ARG, "group_norm_act: null workspace or off its 16-byte alignment");
     LSAM_REQUIRE(ws_bytes >= gn_ws_bytes(N, P, C, G, 1), LSAM_ERR_WORKSPACE, "group_norm_act: workspace too small");
     p.x = x; p.sx = sx; p.px = px; p.dy = dy; p.sy = sy; p.py = py; p.gamma = gamma; p.beta = beta; p.stats = const_cast<float*>(stats);
-    p.out = dx; p.dgamma = dgamma; p.dbeta = dbeta;
+    p.out = want_dx ? dx : nullptr; p.dgamma = dgamma; p.dbeta = dbeta;
+    if (!want_dx && !dgamma && !dbeta) return LSAM_OK;
     p.chan = static_cast<float*>(ws);
     p.coef = p.chan + (size_t)(N > 0 ? N : 1) * C * 2;
     p.part = p.coef + (size_t)(N > 0 ? N : 1) * G * 2;
@@ -776,7 +782,7 @@ int launch_group_norm_act_bwd(const void* dy, long sy, long py, const void* x, l
         LSAM_LAUNCH_CHECK();
         return LSAM_OK;
     }
-    LSAM_REQUIRE(x && dy && dx && stats, LSAM_ERR_BAD_ARG, "group_norm_act: null operand");
+    LSAM_REQUIRE(x && dy && (dx || !want_dx) && stats, LSAM_ERR_BAD_ARG, "group_norm_act: null operand");
     const int V = vec_of(sizeof(T), p, true);
     return V > 1 ? run_bwd<T, 16 / sizeof(T)>(p, s) : run_bwd<T, 1>(p, s);
 }
@@ -784,7 +790,7 @@ int launch_group_norm_act_bwd(const void* dy, long sy, long py, const void* x, l
     template int launch_group_norm_act_fwd<T>(const void*, long, long, const float*, const float*, int, int, int, int, float, int, void*,       \
                                               float*, void*, size_t, hipStream_t);                                                             \
     template int launch_group_norm_act_bwd<T>(const void*, long, long, const void*, long, long, const float*, const float*, const float*, int,  \
-                                              int, int, int, int, void*, float*, float*, void*, size_t, hipStream_t);
+                                              int, int, int, int, bool, void*, float*, float*, void*, size_t, hipStream_t);
 GN_INST(float)
 GN_INST(bf16)
 }  // namespace lsam

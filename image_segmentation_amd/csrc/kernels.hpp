@@ -254,8 +254,8 @@ int launch_group_norm_act_fwd(const void* x, long sx, long px, const float* gamm
                               void* y, float* stats, void* ws, size_t ws_bytes, hipStream_t s);
 template <typename T>
 int launch_group_norm_act_bwd(const void* dy, long sy, long py, const void* x, long sx, long px, const float* gamma, const float* beta,
-                              const float* stats, int N, int P, int C, int G, int act, void* dx, float* dgamma, float* dbeta, void* ws,
-                              size_t ws_bytes, hipStream_t s);
+                              const float* stats, int N, int P, int C, int G, int act, bool want_dx, void* dx, float* dgamma, float* dbeta,
+                              void* ws, size_t ws_bytes, hipStream_t s);
 
 // global norm of a list of tensors and clipping by it (grad_clip.hip); the arrays are host memory, the addresses in them device
 size_t clip_ws_bytes(const long long* n, int count);

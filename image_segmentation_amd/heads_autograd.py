@@ -301,10 +301,9 @@ class GroupNormActFn(torch.autograd.Function):
     def backward(ctx, g):
         _once("group_norm_act")
         x, stats, weight, bias = ctx.saved_tensors
-        want = ctx.needs_input_grad[:3]
-        dx, dw, db = ops.group_norm_act_bwd(g, x, stats, weight, bias, ctx.act, want)
+        dx, dw, db = ops.group_norm_act_bwd(g, x, stats, weight, bias, ctx.act, ctx.needs_input_grad[:3])
         if dw is not None and weight.dtype != torch.float32:
             dw = dw.to(weight.dtype)
         if db is not None and bias.dtype != torch.float32:
             db = db.to(bias.dtype)
-        return dx if want[0] else None, dw, db, None, None, None
+        return dx, dw, db, None, None, None

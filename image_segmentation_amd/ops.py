@@ -906,8 +906,10 @@ def group_norm_act_fwd(x: torch.Tensor, groups: int, weight: Optional[torch.Tens
 
 def group_norm_act_bwd(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
                        act: str = "none", want=(True, True, True)):
-    """(dx T channels last, dweight fp32, dbias fp32) of group_norm_act_fwd, the parameters' None where not wanted; dy of any layout
-    (copied to channels last if it is not)."""
+    """(dx T channels last, dweight fp32, dbias fp32) of group_norm_act_fwd, None where not wanted; dy of any layout (copied to channels
+    last if it is not)."""
+    if not any(want):
+        return None, None, None
     dev, on = _on_device(dy, x, stats, weight, bias)
     with on:
         lay = channels_last_rows(x)
@@ -919,14 +921,15 @@ def group_norm_act_bwd(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, w
             lay_y = channels_last_rows(dy)
         N, P, sx, px = lay
         Cc, G, w, b, L, device = x.shape[1], stats.shape[1], _vec(weight), _vec(bias), lib(), x.device
-        dx = _channels_last_like(x, lay)
+        dx = _channels_last_like(x, lay) if want[0] else None
         dw = torch.empty(Cc, dtype=torch.float32, device=device) if want[1] else None
         db = torch.empty(Cc, dtype=torch.float32, device=device) if want[2] else None
         nws = L.lsam_group_norm_act_ws_bytes(N, P, Cc, G, 1)
         ws = torch.empty(nws, dtype=torch.uint8, device=device)
-        check(L.lsam_group_norm_act_bwd(dtype_code(x.dtype), dy.data_ptr(), lay_y[2], lay_y[3], x.data_ptr(), sx, px, ptr(w), ptr(b),
-                                        stats.data_ptr(), N, P, Cc, G, ACTIVATIONS[act], dx.data_ptr(), ptr(dw), ptr(db),
-                                        ws.data_ptr(), nws, stream_of(dev)))
+        maps = (dtype_code(x.dtype), dy.data_ptr(), lay_y[2], lay_y[3], x.data_ptr(), sx, px, ptr(w), ptr(b), stats.data_ptr(), N, P, Cc, G,
+                ACTIVATIONS[act])
+        rest = (ptr(dw), ptr(db), ws.data_ptr(), nws, stream_of(dev))
+        check(L.lsam_group_norm_act_bwd_params(*maps, *rest) if dx is None else L.lsam_group_norm_act_bwd(*maps, dx.data_ptr(), *rest))
     return dx, dw, db
 
 

@@ -523,6 +523,10 @@ int lsam_group_norm_act_fwd(int dtype, const void* x, long sx, long px, const fl
 int lsam_group_norm_act_bwd(int dtype, const void* dy, long sy, long py, const void* x, long sx, long px, const float* gamma,
                             const float* beta, const float* stats, int N, int P, int C, int G, int act, void* dx, float* dgamma,
                             float* dbeta, void* ws, size_t ws_bytes, lsam_stream_t stream);
+/* The parameters' gradients alone, the same values: no map is written, and x and dy are read once. */
+int lsam_group_norm_act_bwd_params(int dtype, const void* dy, long sy, long py, const void* x, long sx, long px, const float* gamma,
+                                   const float* beta, const float* stats, int N, int P, int C, int G, int act, float* dgamma, float* dbeta,
+                                   void* ws, size_t ws_bytes, lsam_stream_t stream);
 
 /* ---- global norm of a list of tensors, and clipping by it ------------------------------------------------------------------------
  * total = |scale| * (sum g^2)^(1/2) over all tensors, or |scale| * max |g| with inf != 0;  c = min(1, max_norm / (total + 1e-6));

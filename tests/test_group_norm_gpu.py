@@ -11,7 +11,7 @@ import pytest
 import torch
 import torch.nn.functional as F
 
-from image_segmentation_amd import GroupNormAct, group_norm_act
+from image_segmentation_amd import GroupNormAct, _C, group_norm_act, ops
 from image_segmentation_amd._C import LsamError
 
 pytestmark = pytest.mark.gpu
@@ -266,3 +266,31 @@ def test_many_samples(dtype):
     # rows of features: with the fewest groups a workgroup the launch would have 2^32 threads and more, which the runtime cuts short
     x, dy, w, b = make(300_000, 256, 1, 1, dtype, 35)
     check(x, dy, w, b, 32, "silu")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N, C, size", [(1, 24, 6), (3, 24, 6), (2, 24, 150)])
+def test_parameter_gradients_alone(N, C, size, dtype):
+    # a norm on maps that want no gradient: the same sums, and no map is allocated or written
+    x, dy, w, b = make(N, C, size, size, dtype, 37)
+    full = ops.group_norm_act_bwd(dy, x, ops.group_norm_act_fwd(x, 4, w, b, act="gelu", want_stats=True)[1], w, b, "gelu")
+    stats = ops.group_norm_act_fwd(x, 4, w, b, act="gelu", want_stats=True)[1]
+    for want in ((False, True, True), (False, True, False), (False, False, True), (False, False, False)):
+        got = ops.group_norm_act_bwd(dy, x, stats, w, b, "gelu", want)
+        assert got[0] is None
+        for g, f, on in zip(got[1:], full[1:], want[1:]):
+            assert torch.equal(g, f) if on else g is None
+    leaves = [w.detach().requires_grad_(True), b.detach().requires_grad_(True)]
+    y = group_norm_act(x, 4, leaves[0], leaves[1], act="gelu")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    grads = torch.autograd.grad(y, leaves, dy)
+    assert all(torch.equal(g, f) for g, f in zip(grads, full[1:]))
+    if size == 150:                                            # sums of ranges, not a map
+        ws = _C.lib().lsam_group_norm_act_ws_bytes(N, size * size, C, 4, 1)
+        assert torch.cuda.max_memory_allocated() - before <= ws + 4096
+    # no pixels: zero sums
+    e = x[:, :, :0]
+    got = ops.group_norm_act_bwd(dy[:, :, :0], e, stats, w, b, "gelu", (False, True, True))
+    assert got[0] is None and (got[1] == 0).all() and (got[2] == 0).all()

@@ -118,3 +118,13 @@ def test_reducer_refuses_before_the_exchange(max_norm):
     assert p.grad is None and red.stats["all_reduce"] == 0
     red.reduce()                                              # without it, as before
     assert p.grad is None
+
+
+@pytest.mark.parametrize("change, rc", [
+    (dict(C=0), -1), (dict(G=3), -1), (dict(act=4), -1), (dict(sx=-1), -1), (dict(x=0), -1), (dict(ws=0), -1), (dict(ws_bytes=0), -4),
+    (dict(C=8200, G=2), -2), (dict(dtype=9), -1),
+])
+def test_group_norm_parameter_gradients_refuse(change, rc):
+    a = dict(GN, **change)
+    assert _C.lib().lsam_group_norm_act_bwd_params(a["dtype"], a["x"], a["sx"], a["px"], 256, 64, 8, 0, 0, 256, a["N"], a["P"], a["C"], a["G"],
+                                                   a["act"], 256, 256, a["ws"], a["ws_bytes"], 0) == rc

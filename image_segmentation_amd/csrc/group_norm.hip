@@ -444,6 +444,25 @@ __device__ __forceinline__ void fold(float* a, int rows, int cols) {
     }
 }
 
+// put(g, sum of f(c) over the cpg channels c of group g) for the groups 0 .. gb: a thread a group, a wave where it has many channels (1024 summed
+// by one thread: the sum off by 7 units of its last place, by 0.5 in a wave)
+template <typename F, typename P> __device__ __forceinline__ void group_sums(int gb, int cpg, F f, P put) {
+    if (cpg <= 32) {
+        for (int g = threadIdx.x; g < gb; g += ST) {
+            float a = 0.f;
+            for (int c = 0; c < cpg; ++c) a += f(g * cpg + c);
+            put(g, a);
+        }
+    } else {
+        for (int g = threadIdx.x >> 6; g < gb; g += ST / 64) {
+            float a = 0.f;
+            for (int c = threadIdx.x & 63; c < cpg; c += 64) a += f(g * cpg + c);
+            a = wave_sum(a);
+            if ((threadIdx.x & 63) == 0) put(g, a);
+        }
+    }
+}
+
 template <typename T, int V> struct Piece { using type = uint4; };
 template <> struct Piece<float, 1> { using type = float; };
 template <> struct Piece<bf16, 1> { using type = bf16; };
@@ -487,18 +506,13 @@ template <typename T, int V, int UMAX, int ACT> __global__ __launch_bounds__(ST)
     };
     const float cnt = (float)p.P * (float)cpg;
     total([](float a, int) { return a; });
-    for (int g = tid; g < gb; g += ST) {
-        float a = 0.f;
-        for (int c = 0; c < cpg; ++c) a += sm[g * cpg + c];
-        grp[2 * g] = a / cnt;
-    }
+    auto sum = [&](int c) { return sm[c]; };
+    group_sums(gb, cpg, sum, [&](int g, float a) { grp[2 * g] = a / cnt; });
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < V; ++j) m[j] = grp[2 * ((tx * V + j) / cpg)];
     total([&](float a, int j) { return (a - m[j]) * (a - m[j]); });
-    for (int g = tid; g < gb; g += ST) {
-        float a = 0.f;
-        for (int c = 0; c < cpg; ++c) a += sm[g * cpg + c];
+    group_sums(gb, cpg, sum, [&](int g, float a) {
         const float rstd = 1.f / sqrtf(a / cnt + p.eps);
         grp[2 * g + 1] = rstd;
         if (p.stats) {
@@ -506,7 +520,7 @@ template <typename T, int V, int UMAX, int ACT> __global__ __launch_bounds__(ST)
             o[0] = grp[2 * g];
             o[1] = rstd;
         }
-    }
+    });
     __syncthreads();
     if (!mine) return;
     float sl[V], be[V];
@@ -577,26 +591,21 @@ template <typename T, int V, int UMAX, int ACT> __global__ __launch_bounds__(ST)
     __syncthreads();
     fold(sm, rows, p.cb);
     const float m = (float)p.P * (float)cpg;
-    for (int g = tid; g < gb; g += ST) {
-        const float rstd = p.stats[((size_t)n * p.G + c0 / cpg + g) * 2 + 1];
-        float s1 = 0.f, s2 = 0.f;
-        for (int i = 0; i < cpg; ++i) {
-            const int c = g * cpg + i;
-            const float gm = p.gamma ? p.gamma[c0 + c] : 1.f, t = sm[c] * rstd;
-            s1 = fmaf(gm, sa[c], s1);
-            s2 = fmaf(gm, t, s2);
-            if (p.N == 1) {
-                if (p.dbeta) p.dbeta[c0 + c] = sa[c];
-                if (p.dgamma) p.dgamma[c0 + c] = t;
-            } else {
-                float* o = p.chan + ((size_t)n * p.C + c0 + c) * 2;
-                o[0] = sa[c];
-                o[1] = t;
-            }
+    const float* st = p.stats + ((size_t)n * p.G + c0 / cpg) * 2;
+    for (int c = tid; c < p.cb; c += ST) {
+        const float t = sm[c] * st[2 * (c / cpg) + 1];
+        if (p.N == 1) {
+            if (p.dbeta) p.dbeta[c0 + c] = sa[c];
+            if (p.dgamma) p.dgamma[c0 + c] = t;
+        } else {
+            float* o = p.chan + ((size_t)n * p.C + c0 + c) * 2;
+            o[0] = sa[c];
+            o[1] = t;
         }
-        grp[2 * g] = rstd * s1 / m;
-        grp[2 * g + 1] = rstd * rstd * s2 / m;
     }
+    auto gamma = [&](int c) { return p.gamma ? p.gamma[c0 + c] : 1.f; };
+    group_sums(gb, cpg, [&](int c) { return gamma(c) * sa[c]; }, [&](int g, float a) { grp[2 * g] = st[2 * g + 1] * a / m; });
+    group_sums(gb, cpg, [&](int c) { return gamma(c) * sm[c]; }, [&](int g, float a) { grp[2 * g + 1] = st[2 * g + 1] * st[2 * g + 1] * (st[2 * g + 1] * a) / m; });
     __syncthreads();
     if (!mine || !p.out) return;   // no map wanted: the parameters' sums were all
     float c1[V], c2[V];

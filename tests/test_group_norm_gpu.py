@@ -294,3 +294,20 @@ def test_parameter_gradients_alone(N, C, size, dtype):
     e = x[:, :, :0]
     got = ops.group_norm_act_bwd(dy[:, :, :0], e, stats, w, b, "gelu", (False, True, True))
     assert got[0] is None and (got[1] == 0).all() and (got[2] == 0).all()
+
+
+@pytest.mark.parametrize("N, C, H, W, G", [(8, 8192, 1, 1, 8), (4, 8192, 2, 2, 4), (8, 4096, 2, 2, 4), (8, 1024, 3, 3, 1)])
+def test_wide_groups_far_from_zero(N, C, H, W, G):
+    """Over a thousand channels a group, summed in LDS.  In L2, with e = 2^-24 and a mean of 1000 times the spread: a pairwise sum is off by
+    0.5 e |mean|, its division and rounding by as much again (sums by one thread: 7 e |mean| at 1024 channels, 20 at 8192); three times that, and
+    32 e for all that does not grow with the mean.  In dx the mean of dy is multiplied and added once more."""
+    g = torch.Generator().manual_seed(C)
+    far = lambda m: (torch.randn(N, H, W, C, generator=g) + m).cuda().permute(0, 3, 1, 2)
+    x = far(1000.0)
+    ref = F.group_norm(x.double(), G)
+    assert (group_norm_act(x, G).double() - ref).norm() <= (3 * 1000 + 32) * E * ref.norm()
+    x, dy = far(0.0).requires_grad_(True), far(1000.0)
+    (gx,) = torch.autograd.grad(group_norm_act(x, G), x, dy)
+    X = x.detach().double().requires_grad_(True)
+    (ref,) = torch.autograd.grad(F.group_norm(X, G), X, dy.double())
+    assert (gx.double() - ref).norm() <= (4 * 1000 + 32) * E * ref.norm()

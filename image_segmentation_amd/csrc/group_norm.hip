@@ -384,6 +384,41 @@ __device__ __forceinline__ void params(const GnArgs& p, int c) {   // dgamma, db
 }
 __global__ __launch_bounds__(NT) void gn_params_kernel(const GnArgs p) { params(p, blockIdx.x * NT + threadIdx.x); }
 
+// the same over many samples (rows of features): 16 channels a workgroup, 64 threads a channel
+constexpr int FEW_SAMPLES = 64;
+__global__ __launch_bounds__(1024) void gn_params_many_kernel(const GnArgs p) {
+    __shared__ float2 sh[64][16];
+    const int x = threadIdx.x & 15, y = threadIdx.x >> 4, c = blockIdx.x * 16 + x;
+    float2 s = make_float2(0.f, 0.f);
+    if (c < p.C) {
+#pragma unroll 8
+        for (int n = y; n < p.N; n += 64) {
+            const float2 v = *reinterpret_cast<const float2*>(p.chan + ((size_t)n * p.C + c) * 2);
+            s.x += v.x;
+            s.y += v.y;
+        }
+    }
+    sh[y][x] = s;
+    for (int h = 32; h; h >>= 1) {
+        __syncthreads();
+        if (y < h) {
+            sh[y][x].x += sh[y + h][x].x;
+            sh[y][x].y += sh[y + h][x].y;
+        }
+    }
+    if (y || c >= p.C) return;
+    if (p.dbeta) p.dbeta[c] = sh[0][x].x;
+    if (p.dgamma) p.dgamma[c] = sh[0][x].y;
+}
+int sum_params(const GnArgs& p, hipStream_t s) {
+    if (!p.dgamma && !p.dbeta) return LSAM_OK;
+    // 300,000 rows of 256: 1.1 ms, 35.7 with a thread a channel
+    if (p.N > FEW_SAMPLES) gn_params_many_kernel<<<cdiv(p.C, 16), 1024, 0, s>>>(p);
+    else gn_params_kernel<<<cdiv(p.C, NT), NT, 0, s>>>(p);
+    LSAM_LAUNCH_CHECK();
+    return LSAM_OK;
+}
+
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(NT) void gn_bwd_apply_kernel(const GnArgs p) {
     const int tid = threadIdx.x;
@@ -702,11 +737,7 @@ template <typename T, int V> int run_bwd(GnArgs& p, hipStream_t s) {
                                           : gn_one_bwd_kernel<T, V, UB, LSAM_ACT_NONE>;
         k<<<p.N * (p.C / p.cb), ST, (ST * V + 3 * p.cb) * sizeof(float), s>>>(p);
         LSAM_LAUNCH_CHECK();
-        if (p.N > 1 && (p.dgamma || p.dbeta)) {
-            gn_params_kernel<<<cdiv(p.C, NT), NT, 0, s>>>(p);
-            LSAM_LAUNCH_CHECK();
-        }
-        return LSAM_OK;
+        return p.N > 1 ? sum_params(p, s) : LSAM_OK;
     }
     ranges(p, V, WG_REST);
     auto k = p.act == LSAM_ACT_RELU   ? gn_bwd_sums_kernel<T, V, LSAM_ACT_RELU>
@@ -717,16 +748,13 @@ template <typename T, int V> int run_bwd(GnArgs& p, hipStream_t s) {
     LSAM_LAUNCH_CHECK();
     gn_bwd_join_kernel<<<p.N * p.G, NT, 0, s>>>(p);
     LSAM_LAUNCH_CHECK();
-    if (!p.out) {   // 16 x 256 x 256 x 256 bf16: the second pass is more than half of the backward
-        gn_params_kernel<<<cdiv(p.C, NT), NT, 0, s>>>(p);
-        LSAM_LAUNCH_CHECK();
-        return LSAM_OK;
-    }
+    if (!p.out) return sum_params(p, s);   // 16 x 256 x 256 x 256 bf16: the second pass is more than half of the backward
+    if (p.N > FEW_SAMPLES) LSAM_TRY(sum_params(p, s));
     auto a = p.act == LSAM_ACT_RELU   ? gn_bwd_apply_kernel<T, V, LSAM_ACT_RELU>
              : p.act == LSAM_ACT_SILU ? gn_bwd_apply_kernel<T, V, LSAM_ACT_SILU>
              : p.act == LSAM_ACT_GELU ? gn_bwd_apply_kernel<T, V, LSAM_ACT_GELU>
                                       : gn_bwd_apply_kernel<T, V, LSAM_ACT_NONE>;
-    a<<<p.N * p.splits + cdiv(p.C, NT), NT, 0, s>>>(p);
+    a<<<p.N * p.splits + (p.N > FEW_SAMPLES ? 0 : cdiv(p.C, NT)), NT, 0, s>>>(p);
     LSAM_LAUNCH_CHECK();
     return LSAM_OK;
 }

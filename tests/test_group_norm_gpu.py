@@ -311,3 +311,21 @@ def test_wide_groups_far_from_zero(N, C, H, W, G):
     X = x.detach().double().requires_grad_(True)
     (ref,) = torch.autograd.grad(F.group_norm(X, G), X, dy.double())
     assert (gx.double() - ref).norm() <= (4 * 1000 + 32) * E * ref.norm()
+
+
+def test_parameter_gradients_of_many_samples():
+    """dbeta is the sum of dy: a thousand times its spread, over 20,000 rows.  64 threads add 313 each, one after another: off by sqrt(313) / 3 = 6 e
+    and less as 64 of them average, against sqrt(20,000) / 3 = 47 e by one thread; bound 16 e, e = 2^-24, in L2 over the channels."""
+    g = torch.Generator().manual_seed(5)
+    x, dy = torch.randn(20_000, 64, generator=g).cuda(), (torch.randn(20_000, 64, generator=g) + 1000).cuda()
+    w, b = torch.ones(64, device="cuda", requires_grad=True), torch.zeros(64, device="cuda", requires_grad=True)
+    (gb,) = torch.autograd.grad(group_norm_act(x, 8, w, b), b, dy)
+    ref = dy.double().sum(0)
+    assert (gb.double() - ref).norm() <= 16 * E * ref.norm()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N, C, H, W, G", [(65, 40, 6, 5, 8), (64, 40, 6, 5, 8), (67, 9, 130, 121, 3), (1000, 24, 2, 2, 24)])
+def test_more_samples_match_float64(N, C, H, W, G, dtype):
+    x, dy, w, b = make(N, C, H, W, dtype, N + C)
+    check(x, dy, w, b, G, "gelu")

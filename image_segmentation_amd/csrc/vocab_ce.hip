@@ -887,7 +887,8 @@ template <typename T> __global__ __launch_bounds__(256) void ce_finish_kernel(co
 // host
 // ---------------------------------------------------------------------------------------------------------------------
 // A piece's dz.  16384 x 256 x 32000 in all: 1560 us with 256 MB (what the last-level cache holds), 1475 with 512, 1337 with 1024: fewer
-// passes over the fp32 sums of dx weigh more than where dz is read from.
+// passes over the fp32 sums of dx weigh more than where dz is read from.  A piece has 256 classes at least: beyond 0.7 M rows in fp32 and
+// 2.1 M in bf16 that is more than this many bytes (512 or 1536 a row).
 constexpr size_t DZ_CAP = (size_t)1 << 30;
 constexpr int CU = 256;
 

@@ -497,7 +497,8 @@ int lsam_hiera_backward_block(lsam_hiera_t* h, const float* grad_out, int batch,
  *   loss_m = (1 - smooth)(lse_m - z_mt) + smooth (lse_m - mean_v z_mv);  MEAN divides the sum by the rows that count (0 / 0 = NaN).
  * loss fp32: [M] under LSAM_REDUCE_NONE (0 where ignored), one value otherwise.  `state` (lsam_linear_ce_state_bytes) is what the
  * backward needs of the forward: row selection, statistics, and the selected rows of x.  `ws`: lsam_linear_ce_ws_bytes with grads = 0
- * for the forward, else the sum of LSAM_CE_D{X,W,B} for the gradients wanted; the same w / ldw as in the call. */
+ * for the forward, else the sum of LSAM_CE_D{X,W,B} for the gradients wanted; the same w / ldw as in the call.  Most of the latter is a
+ * piece of the scores' gradients: 1 GiB at most, or 512 bytes a row (LSAM_F32: 1536) where that is more (2.1 M rows, 0.7 M). */
 enum { LSAM_REDUCE_NONE = 0, LSAM_REDUCE_MEAN = 1, LSAM_REDUCE_SUM = 2 };
 enum { LSAM_CE_DX = 1, LSAM_CE_DW = 2, LSAM_CE_DB = 4 };
 size_t lsam_linear_ce_state_bytes(int dtype, int M, int D);

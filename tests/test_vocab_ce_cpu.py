@@ -64,3 +64,14 @@ def test_rows_of_a_launch(M, D, V, rc):
     L = _C.lib()
     assert L.lsam_linear_ce_fwd(_C.BF16, 256, D, 256, D, 0, 256, M, D, V, -100, 0.0, 1, 256, 256, 256, 0, 0) == rc
     assert L.lsam_linear_ce_bwd(_C.BF16, 256, D, 0, 256, M, D, V, 0.0, 1, 256, 256, D, 256, D, 0, 256, 0, 0) == rc
+
+
+@pytest.mark.parametrize("dtype, row", [(_C.BF16, 512), (_C.F32, 1536)])
+@pytest.mark.parametrize("M", [100_000, 1 << 20, 1 << 21, 1 << 22])
+def test_workspace_of_many_rows(M, dtype, row):
+    """The weight gradient's workspace: a piece of the scores' gradients (1 GiB, or 256 classes' worth), partial sums of 512 x 128 x 128 or 256 x 256 x 256
+    fp32 values at most, in fp32 the table's three planes, and each part's alignment."""
+    D, V = 256, 32000
+    piece = max(1 << 30, M * row)
+    got = _C.lib().lsam_linear_ce_ws_bytes(dtype, M, D, V, 256, D, 0.0, 2)
+    assert piece - M * row < got <= piece + 4 * 256 ** 3 + (6 * V * D if dtype == _C.F32 else 0) + 4096

@@ -8,12 +8,14 @@
 // terms, see mma), and two more products read it.  Rows whose target is ignored are taken out first (order kept): they cost nothing,
 // and what they hold (NaN included) reaches no gradient.
 //
-// Bound by the matrix pipes: 2 M D V operations forward, 6 M D V backward, against (M + V) D values read.  With the scores in memory the
-// plain form moves 2 to 4 bytes of each several times over and takes the sum of three library products besides.  Measured, bf16, rows x
-// D x classes, forward and gradients: 16384 x 256 x 32000 in 1.23 ms (plain 10.6; scores 347 us, dz 440, dx 282, dW 242), 8192 x 896 x
-// 50257 in 2.4 ms (plain 19.2; scores 618, dz 688, dx 615, dW 645); forward alone 4096 x 448 x 65536 in 219 us (plain 2930); few rows
-// are bound by the table's bytes, read three times and its gradient written once: 1 x 896 x 50257 in 110 us (3.3 TB/s).  The
-// products run at 0.9 to 1.2 PFLOP/s; the scores' and dz's epilogues (an exponential a score) are what D = 256 adds to them.
+// 2 M D V operations forward, 6 M D V backward, against (M + V) D values read: wide rows are bound by the matrix pipes.  Narrow ones are
+// not: the scores' and dz's epilogues (an exponential a score) stay what they are, and dz, written once and read twice, gives D operations
+// a byte to each of dx and dW -- 256 of them where this card's copy and its matrix product balance at 312.  With the scores in memory the
+// plain form moves 2 to 4 bytes of each several times over and takes the sum of three library products besides.  Measured, bf16, rows (one
+// in ten ignored) x D x classes, forward and gradients: 16384 x 256 x 32000 in 1.25 ms (plain 10.6; scores 350 us, dz 436, dx 281, dW 244:
+// 0.69, 0.55, 0.86 and 0.99 PFLOP/s of the rows that count; dz alone is 0.94 GB, 186 us a pass at a copy's rate), 8192 x 896 x 50257 in
+// 2.44 ms (plain 19.3; scores 625, dz 684, dx 625, dW 661: 0.97 to 1.06); forward alone 4096 x 448 x 65536 in 223 to 234 us (plain 2945);
+// few rows are bound by the table's bytes, read three times and its gradient written once: 1 x 896 x 50257 in 110 us (3.3 TB/s).
 #include <type_traits>
 
 #include "kernels.hpp"
@@ -53,6 +55,9 @@ enum Mode { STATS, DZ, ACC, OUT, PART };   // PART: OUT in fp32
 // what dominates them -- the target's entry of a row that is not learned yet -- is exactly -1 under MEAN and SUM.  Rounded to bf16 at its
 // own size, (1 - e) g / n, that entry would be off by the same fraction in every row, and the fraction would come through the sums
 // whole.  The factor is applied to the fp32 sums; without rows every sum is 0 and stays it, whatever 1 / n is.
+// Rounded all the same, once, where the operands are bf16: the matrix pipes multiply what they are given, and a second term would double
+// both products.  Every entry is off by up to 2^-9 of itself, and dx and dW in L2 by 0.0019 to 0.0021 where their own rounding alone makes
+// 0.0017 (a single row of two classes, where nothing averages: 0.0037 against 0.0027).  db is summed from the values before it.
 struct Grad {
     const float* gout;
     int reduction;
@@ -99,7 +104,7 @@ __device__ __forceinline__ void mma(const uint4& a, const uint4& b, f32x4& c) {
 // rounded to the nearest 8.  |x1| <= 2^-9 |x|, |x2| <= 2^-18 |x|, so of the nine products the three left out, x1 y2, x2 y1 and x2 y2, come
 // to at most 2^-25 |x y|: half of what rounding one fp32 product costs.  Six bf16 products at 16 times the fp32 instructions' rate; of a
 // k-tile the small ones go first.  A k-tile holds all three planes of both operands, so that each is fetched and read once for its six
-// products.  (2011 x 252 x 10007 forward and gradient: 305 us; 416 with
+// products.  (2011 x 252 x 10007 forward and gradient: 303 to 317 us; 416 with
 // fp32 matrix instructions, 357 with k run through once a product.)
 
 // One operand's tile in LDS.  KC: R rows of KE values, 16-byte chunk c of row r at c ^ (r & 7) (KE = 32, four chunks: c ^ (r / 4 & 3)), so

@@ -82,8 +82,10 @@ def linear_cross_entropy(inputs, weight, targets, bias=None, ignore_index: int =
     targets, ...) defines it, without the scores ever in memory: forward and backward form them a tile, then a piece of the classes,
     at a time (`lsam_linear_ce_fwd` / `_bwd`).
 
-    inputs [..., D] and weight [V, D]: both float32 or both bfloat16 (sums and statistics are fp32 either way; float32 values go through
-    the matrix pipes as three bfloat16 terms, which together are exact for magnitudes from 1e-30 to 3.3e38; larger ones count as infinite);
+    inputs [..., D] and weight [V, D]: both float32 or both bfloat16.  Scores, sums and statistics are fp32 either way; float32 values go
+    through the matrix pipes as three bfloat16 terms, which together are exact for magnitudes from 1e-30 to 3.3e38 (larger ones count as
+    infinite).  With bfloat16 operands the gradients of the scores are rounded to bfloat16, once, before the products with weight and
+    inputs (up to 2^-9 of each), beside the results' own rounding; the bias gradient is summed before it.
     targets [...] integer; bias [V] any float type: -inf takes a class out, finite values beyond +-1e38 count as that.  Scores of any size
     up to 1.7e38 are kept as fp32 holds them.  The loss is fp32: targets' shape under reduction="none" (0 where ignored), one value otherwise.
     Rows whose target is `ignore_index` cost nothing and pass nothing on, whatever they hold.  A target outside [0, V) makes the loss

@@ -492,6 +492,7 @@ int lsam_hiera_backward_block(lsam_hiera_t* h, const float* grad_out, int batch,
  * x T [M][ldx], w T [V][ldw] (D columns each), bias fp32 [V] or NULL, target int64 [M].  Rows whose target is `ignore` take no part;
  * a target outside [0, V) makes its row's loss and gradient NaN (nothing is read out of range).
  * A bias of -inf takes its class out; finite ones beyond +-1e38 count as that.  Scores may reach 1.7e38.
+ * LSAM_BF16: the scores' gradients are rounded to bf16 once before the products that make dx and dw (db is summed before it).
  * LSAM_F32 operands are multiplied as three bf16 terms each (exact together for magnitudes from 1e-30 to 3.3e38; larger count as
  * infinite) in six products summed in fp32: as close to the exact product as fp32 arithmetic.
  *   loss_m = (1 - smooth)(lse_m - z_mt) + smooth (lse_m - mean_v z_mv);  MEAN divides the sum by the rows that count (0 / 0 = NaN).

@@ -34,8 +34,8 @@ def clip_grads_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float
     fp32 / bf16 tensors of any mix on one GPU; `out` may have other types than `grads` (bf16 gradients into fp32 buffers).  norm_type
     2 or inf.  Squares are summed in fp64.  A norm that is not finite makes the factor what torch.nn.utils.clip_grad_norm_ makes it
     (NaN, or 0 for an infinite one); error_if_nonfinite looks at the norm on the host first and raises, with nothing changed.
-    max_norm = inf: the norm alone, of tensors of any layout, and nothing is written.  Contiguous tensors that share memory are refused where anything would be written, and so are others
-    that begin at one address or repeat their elements (expanded ones)."""
+    max_norm = inf: the norm alone, of tensors of any layout, and nothing is written.  Contiguous tensors that share memory are refused
+    where anything would be written, and so are others that begin at one address or repeat their elements (expanded ones)."""
     grads = list(grads)
     inf_norm = float(norm_type) == float("inf")
     if not inf_norm and float(norm_type) != 2.0:

@@ -16,9 +16,10 @@ from ._C import LsamError
 def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                    eps: float = 1e-5, act: str = "none") -> torch.Tensor:
     """act(F.group_norm(x, num_groups, weight, bias, eps)) for x [N, C, *spatial] (float32 or bfloat16) laid out channels last; `act`
-    is "none", "relu", "silu" or "gelu" (the erf form; bfloat16 maps: from a polynomial, off by less than 1.5e-7 |h|).  Statistics, parameters and their gradients are fp32; the result has x's type
-    and is channels last without gaps.  x may be a channel slice of a wider channels-last map; any other layout (an NCHW map of the
-    neck) is copied to channels last first.  At most 8192 channels, fewer than 2^20 samples and 2^24 groups in all."""
+    is "none", "relu", "silu" or "gelu" (the erf form; bfloat16 maps: from a polynomial, off by less than 1.5e-7 |h|). Statistics,
+    parameters and their gradients are fp32; the result has x's type and is channels last without gaps. x may be a channel slice of a
+    wider channels-last map; any other layout (an NCHW map of the neck) is copied to channels last first. At most 8192 channels, fewer
+    than 2^20 samples and 2^24 groups in all."""
     if not x.is_cuda:
         raise LsamError("group_norm_act runs on the MI355X only (no CPU or PyTorch fallback)")
     if x.dim() < 2 or x.dtype not in (torch.float32, torch.bfloat16):

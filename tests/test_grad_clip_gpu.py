@@ -262,3 +262,14 @@ def test_reducer_refuses_types_before_the_exchange(tmp_path):
         assert red.stats["all_reduce"] == 1 and all((p.grad == 1).all() for p in params)
     finally:
         dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("n", [2 ** 30 + 7, 2 ** 32 + 5])
+def test_a_tensor_of_more_than_2_to_30_values(n):
+    g = torch.full((n,), 0.5, dtype=BF, device="cuda")
+    g[-3:] = 64.0
+    want = math.sqrt((n - 3) * 0.25 + 3 * 4096.0)
+    norm = clip_grads_([g], want / 4)
+    assert abs(float(norm) - want) <= 2 * E * want
+    assert (g[:-3] == 0.125).all() and (g[-3:] == 16.0).all()   # a quarter, less 1e-6 of the norm: the nearest bf16 value
+    assert abs(float(clip_grads_([g], math.inf, math.inf)) - 16.0) == 0.0

@@ -329,3 +329,25 @@ def test_parameter_gradients_of_many_samples():
 def test_more_samples_match_float64(N, C, H, W, G, dtype):
     x, dy, w, b = make(N, C, H, W, dtype, N + C)
     check(x, dy, w, b, G, "gelu")
+
+
+def test_a_map_of_more_than_2_to_31_values():
+    # one small map over and over: its statistics, results and gradients over and over
+    x, dy, w, b = make(1, 256, 64, 64, torch.bfloat16, 39)
+    K = 2100
+    y, stats = ops.group_norm_act_fwd(x, 32, w, b, act="gelu", want_stats=True)
+    dx, dw, db = ops.group_norm_act_bwd(dy, x, stats, w, b, "gelu")
+    tall = lambda v: v.permute(0, 2, 3, 1).expand(K, 64, 64, 256).reshape(1, K * 64, 64, 256).permute(0, 3, 1, 2)
+    X, DY = tall(x), tall(dy)
+    assert X.numel() > 2 ** 31
+    Y, S = ops.group_norm_act_fwd(X, 32, w, b, act="gelu", want_stats=True)
+    DX, DW, DB = ops.group_norm_act_bwd(DY, X, S, w, b, "gelu")
+    # fp32 sums in another order; bf16 results may round the other way
+    assert ((S - stats).abs() <= 1e-5 * stats.abs() + 1e-6).all()
+    # K times a channel's sum: terms of 4096 pixels cancel in it, the longer sums' roundings do not
+    for big, small in ((DW, dw), (DB, db)):
+        assert ((big / K - small).abs() <= 1e-5 * 4096).all()
+    for big, small in ((Y, y), (DX, dx)):
+        rows, want = big.permute(0, 2, 3, 1).reshape(K, -1), small.permute(0, 2, 3, 1).reshape(-1).float()
+        for k in (0, 1, K // 2, K - 2, K - 1):
+            assert ((rows[k].float() - want).abs() <= 2.0 ** -7 * want.abs() + 1e-4).all()

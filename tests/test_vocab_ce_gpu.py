@@ -419,3 +419,10 @@ def test_no_rows_at_the_c_boundary(wanted, dtype):
                                 dw.data_ptr() if wanted & 2 else 0, D, db.data_ptr() if wanted & 4 else 0, ws.data_ptr(), ws.numel(), s) == 0
     assert float(loss) == 0.0 and (dx == 7.0).all()
     assert (dw == (0.0 if wanted & 2 else 7.0)).all() and (db == (0.0 if wanted & 4 else 7.0)).all()
+
+
+@pytest.mark.parametrize("M, D, V, dtype", [(2_200_000, 16, 300, torch.bfloat16), (750_000, 16, 300, torch.float32), (9_000_000, 8, 20, torch.bfloat16)])
+def test_rows_beyond_a_piece(M, D, V, dtype):
+    # so many rows that 256 classes' gradients of the scores are more than a GiB, and more than 2^31 of them in the last case
+    x, w, t, b, g = make(M, D, V, dtype, True, V)
+    check(x, w, t, b, g, 0.0, "none")

@@ -1,7 +1,7 @@
 """How close loss_fns.linear_cross_entropy comes in fp32, where operands are multiplied as three bf16 planes: relative L2 errors against
 float64.  Element by element bounds grow with the sums' lengths and would not see a plane that is missing or out of place; the norms do.
 
-In units of 2^-24: losing the third plane of one operand leaves it rounded to 16 bits, a relative error spread over +-2^-17 that the L2 norm
+In units of 2^-24: losing the third plane of one operand leaves it rounded to 16 bits, a relative error spread over +-2^-18 that the L2 norm
 of a product keeps: 25 to 45 of the product itself, over 10 of the loss where it is the scores'.  Three planes with sums in fp32 come to
 at most 7.5 in dx and dW, 4.5 in db and 2.7 in the loss at these sizes, fp32 products to 9.3, 9.3, 7.1 and 4.  The bounds lie half way to a
 lost plane (emulate() on the CPU shows both sides)."""
